@@ -71,6 +71,17 @@ std::vector<at::Tensor> attn_bwd_packed(const at::Tensor& dout, const at::Tensor
 void register_ipc(pybind11::module& m);
 uint64_t bounds_word_rowops(bool reset);
 uint64_t bounds_word_fold(bool reset);
+uint64_t bounds_word_distill(bool reset);
+std::vector<at::Tensor> topk_logprobs(const at::Tensor& logits, int64_t k, double temperature);
+std::vector<at::Tensor> sample_tokens(const at::Tensor& logits, const c10::optional<at::Tensor>& noise,
+                                      const c10::optional<at::Tensor>& temperature_t, double temperature,
+                                      const c10::optional<at::Tensor>& top_k_t, int64_t top_k,
+                                      const c10::optional<at::Tensor>& top_p_t, double top_p,
+                                      const c10::optional<at::Tensor>& min_p_t, double min_p);
+std::vector<at::Tensor> distill_rows_fwd(const at::Tensor& logits, const at::Tensor& ids, const at::Tensor& lp,
+                                         double tau, bool reverse, bool tail);
+void distill_rows_bwd(const at::Tensor& logits, const at::Tensor& slots, const at::Tensor& ref, const at::Tensor& gs,
+                      const at::Tensor& entry, const at::Tensor& grad, double tau, at::Tensor& out);
 void register_pinned(pybind11::module& m);
 void gemm_tc(at::Tensor& out, const at::Tensor& a, const at::Tensor& b, bool a_t, bool b_t, int64_t mode,
              double alpha, const c10::optional<at::Tensor>& residual);
@@ -196,7 +207,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         // failed index checks per source file: {file: (site, index)}; empty when every check passed
         pybind11::dict out;
         const std::pair<const char*, uint64_t (*)(bool)> units[] = {{"rowops", &ts::bounds_word_rowops},
-                                                                   {"fold", &ts::bounds_word_fold}};
+                                                                   {"fold", &ts::bounds_word_fold},
+                                                                   {"distill", &ts::bounds_word_distill}};
         for (const auto& u : units) {
           const uint64_t w = u.second(reset);
           if (w != 0) {
@@ -219,6 +231,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         pybind11::arg("a2"), pybind11::arg("b2"), pybind11::arg("a_t"), pybind11::arg("b_t"), pybind11::arg("mode"),
         pybind11::arg("alpha"), pybind11::arg("residual") = pybind11::none());
   m.def("lmhead_dlogits_tc", &ts::lmhead_dlogits_tc);
+  m.def("topk_logprobs", &ts::topk_logprobs);
+  m.def("sample_tokens", &ts::sample_tokens);
+  m.def("distill_rows_fwd", &ts::distill_rows_fwd);
+  m.def("distill_rows_bwd", &ts::distill_rows_bwd);
   m.def("gdn_bwd", &ts::gdn_bwd);
   m.def("gdn_chunk_fwd", &ts::gdn_chunk_fwd);
   m.def("gdn_chunk_bwd", &ts::gdn_chunk_bwd);

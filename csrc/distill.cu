@@ -1,0 +1,405 @@
+// Distillation from a teacher's top entries: loss rows over student logits [N, V] and the logits' gradient.
+//
+// Per row, with a = z/tau, log p = a - lse(a), S the teacher's entries (token id, log-prob t), q = exp(t):
+//   forward  KL(q || p):  L = sum_S q (t - log p)     [+ Q (log Q - log P)]
+//   reverse  KL(p || q):  L = sum_S p (log p - t)     [+ P (log P - log Q)]
+// P and Q are what p and q give to the tokens outside S, one class together ("tail"). The gradient goes through the
+// log-probs of S alone (dP = -sum dp): with g_k = dL/dlog p_k and G = sum g_k,
+//   dL/dz_j = (g_j [j in S] - G p_j) / tau,
+// in closed form (mass = sum_S q + Q; u = log p - t, u_T = log P - log Q):
+//   forward  entries p mass - q,                    G = Q/P - mass       (without the tail: G = -sum_S q, mass likewise)
+//   reverse  entries p (u - L),                     G = L - u_T
+//            without the tail: p (u + 1 - L - sum_S p),  G = L + sum_S p
+// P is summed over the tokens outside S directly: as 1 - sum_S p it would have no digits left where S holds nearly
+// all of the mass, and the gradient divides by it. The K entries' arithmetic is done in 64 bits for the same reason
+// (Q = 1 - sum q); K numbers against a row of V.
+//
+// Both kernels move each logit once: the forward reads the row (a bitmap of S in shared memory takes its tokens out of
+// the sum), the backward reads it and writes the gradient, then overwrites the entries of S with values that the
+// forward has left per entry.
+#include "bounds.cuh"
+#include "common.cuh"
+#include "vocab.cuh"
+#include "vocab.h"
+
+namespace ts {
+namespace {
+
+namespace cg = cooperative_groups;
+using namespace vocab;
+
+constexpr int kSiteTeacherId = 4;  // bounds site: a teacher token id outside the vocabulary
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kMaxTop = 256;  // teacher entries of a row: one per thread
+constexpr int kMaxParts = 8;
+constexpr double kLeastTail = 1e-7;  // of the teacher: about the resolution of its fp32 log-probs
+
+struct Block2 {
+  double x[kWarps], y[kWarps];
+};
+// Sums of x and of y over the block, to all threads.
+__device__ void block_sum2(Block2& b, double& x, double& y) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    x += __shfl_xor_sync(0xffffffffu, x, o);
+    y += __shfl_xor_sync(0xffffffffu, y, o);
+  }
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) {
+    b.x[threadIdx.x >> 5] = x;
+    b.y[threadIdx.x >> 5] = y;
+  }
+  __syncthreads();
+  x = y = 0.0;
+  for (int w = 0; w < kWarps; ++w) {
+    x += b.x[w];
+    y += b.y[w];
+  }
+}
+
+// The row's loss and gradient coefficients, by one block: thread k holds entry k (logit z, log-prob t; `have` where it
+// counts), the tokens outside S come as (m, s_tail) with s_tail = sum 2^((z - m)·c), m = -inf if there are none.
+__device__ void finish_row(Block2& b, float* red, long long row, int k, float z, float t, bool have, float m,
+                           float s_tail, float c, float tau, bool reverse, bool tail, const DistillOut& out) {
+  const int tid = threadIdx.x;
+  const float m_tail = m;
+  const float wm = warp_max(have ? z : -INFINITY);
+  __syncthreads();
+  if ((tid & 31) == 0) red[tid >> 5] = wm;
+  __syncthreads();
+  for (int w = 0; w < kWarps; ++w) m = fmaxf(m, red[w]);
+  if (m == -INFINITY) m = 0.f;
+  const double st = m_tail == -INFINITY ? (double)s_tail : (double)s_tail * exp2(((double)m_tail - (double)m) * c);
+  const double a2 = ((double)z - (double)m) * c;
+  const double e = have ? exp2(a2) : 0.0;
+  const double q = have ? exp((double)t) : 0.0;
+  double se = e, sq = q;
+  block_sum2(b, se, sq);
+  const double s = st + se;
+  const double ls = log(s);
+  const double logp = a2 * 0.693147180559945309417 - ls;
+  const double p = e / s;
+  const double tp = st / s;
+  const bool with_tail = tail && !(tp == 0.0);
+  double lt = 0.0, tq = 0.0, ltq = 0.0;
+  if (with_tail) {
+    lt = log(st) - ls;
+    tq = fmax(1.0 - sq, kLeastTail);
+    ltq = log(tq);
+  }
+  double l = 0.0;
+  if (have) {
+    if (!reverse) l = q * ((double)t - logp);
+    else if (!(p == 0.0)) l = p * (logp - (double)t);
+  }
+  double sl = l, sp = have ? p : 0.0;
+  block_sum2(b, sl, sp);
+  // The sums over g_k in closed form: g_k - G p_k and G themselves would cancel where P is small.
+  double g, gsum;  // of this entry, and G
+  if (!reverse) {
+    if (with_tail) sl += tq * (ltq - lt);
+    const double mass = sq + tq;
+    g = p * mass - q;
+    gsum = (with_tail ? tq / tp : 0.0) - mass;
+  } else {
+    if (with_tail) sl += tp * (lt - ltq);
+    const double off = with_tail ? sl : sl + sp - 1.0;
+    g = p == 0.0 ? 0.0 : p * (logp - (double)t - off);
+    gsum = with_tail ? off - (lt - ltq) : sl + sp;
+  }
+  if (tid < k) out.entry[row * k + tid] = have ? (float)(g / (double)tau) : 0.f;
+  if (tid == 0) {
+    out.loss[row] = (float)sl;
+    out.ref[row] = m;
+    out.gs[row] = (float)(gsum / (s * (double)tau));
+  }
+}
+
+// Entry k of the row: its token, or -1 where there is none (an id outside [0, V), a log-prob of -inf, or an id that
+// an earlier entry has).
+__device__ int entry_slot(int* ids_s, const int64_t* ids, const float* lp, long long row, int k, int v, float& t) {
+  const int tid = threadIdx.x;
+  int slot = -1;
+  t = 0.f;
+  if (tid < k) {
+    const int64_t id = ids[row * k + tid];
+    t = lp[row * k + tid];
+    if (id >= v || id < -1) TS_BOUND_RECORD(kSiteTeacherId, id);
+    if (id >= 0 && id < v && !(t == -INFINITY)) slot = (int)id;
+    ids_s[tid] = slot;
+  }
+  __syncthreads();
+  if (slot >= 0) {
+    for (int j = 0; j < tid; ++j) {
+      if (ids_s[j] == slot) {
+        slot = -1;
+        break;
+      }
+    }
+  }
+  __syncthreads();
+  if (tid < k) ids_s[tid] = slot;
+  return slot;
+}
+
+struct RowShared {
+  Block2 b;
+  float red[kWarps], wm[kWarps], ws[kWarps];
+  float pm, ps;
+  int ids[kMaxTop];
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) distill_rows_fwd_kernel(const T* __restrict__ logits, long long stride,
+                                                                    int v, const int64_t* __restrict__ ids,
+                                                                    const float* __restrict__ lp, int k, float tau,
+                                                                    bool reverse, bool tail, DistillOut out,
+                                                                    int words) {
+  constexpr int VEC = Slice<T>::kVec;
+  __shared__ RowShared sh;
+  extern __shared__ uint32_t bitmap[];  // bit of token id: id - lo - head + VEC, so a vector's bits share a byte
+  cg::cluster_group cl = cg::this_cluster();
+  const int parts = (int)cl.num_blocks(), part = (int)cl.block_rank();
+  const long long row = blockIdx.x / parts;
+  const int tid = threadIdx.x;
+  const float c = kLog2e / tau;
+  const T* lrow = logits + row * stride;
+  for (int i = tid; i < words; i += kThreads) bitmap[i] = 0;
+  float t;
+  const int slot = entry_slot(sh.ids, ids, lp, row, k, v, t);
+  if (part == 0 && tid < k) out.slots[row * k + tid] = slot;
+  if (!__syncthreads_or(slot >= 0)) {  // the same in every part: a row without entries has no loss
+    if (part == 0) {
+      if (tid < k) out.entry[row * k + tid] = 0.f;
+      if (tid == 0) out.loss[row] = out.ref[row] = out.gs[row] = 0.f;
+    }
+    return;
+  }
+  const float zk = part == 0 && slot >= 0 ? to_f(lrow[slot]) : 0.f;
+  Slice<T> sl(lrow, v, part, parts);
+  if (slot >= sl.lo && slot < sl.lo + sl.n) {
+    const int bit = slot - sl.lo - sl.head + VEC;
+    atomicOr(&bitmap[bit >> 5], 1u << (bit & 31));
+  }
+  __syncthreads();
+  float m = -INFINITY, s = 0.f;
+  if (tid < sl.head + sl.tail) {
+    const int i = tid < sl.head ? tid : sl.nvec * VEC + tid;
+    const int bit = i - sl.head + VEC;
+    if (!((bitmap[bit >> 5] >> (bit & 31)) & 1)) {
+      const float z = to_f(sl.p[i]);
+      stat_raise(m, s, fmaxf(z, -INFINITY), c);
+      s += sum_exp<1>(&z, m, c);
+    }
+  }
+  const T* body = sl.body();
+  const uint8_t* bytes = reinterpret_cast<const uint8_t*>(bitmap);
+  constexpr int U = 16 / VEC;
+  for (int i0 = tid; i0 < sl.nvec; i0 += U * kThreads) {
+    uint4 raw[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j)
+      if (i0 + j * kThreads < sl.nvec) raw[j] = load_stream(body + (long long)(i0 + j * kThreads) * VEC);
+    float z[U * VEC];
+    float zmax = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int i = i0 + j * kThreads;
+      if (i < sl.nvec) {
+        unpack<T>(raw[j], z + j * VEC);
+        const uint32_t in = VEC == 8 ? bytes[i + 1] : (bytes[(i + 1) >> 1] >> (((i + 1) & 1) * 4)) & 15u;
+        if (in) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e)
+            if ((in >> e) & 1) z[j * VEC + e] = -INFINITY;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) z[j * VEC + e] = -INFINITY;
+      }
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) zmax = fmaxf(zmax, z[j * VEC + e]);
+    }
+    stat_raise(m, s, zmax, c);
+    s += sum_exp<U * VEC>(z, m, c);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+    stat_merge(m, s, m2, s2, c);
+  }
+  if ((tid & 31) == 0) {
+    sh.wm[tid >> 5] = m;
+    sh.ws[tid >> 5] = s;
+  }
+  __syncthreads();
+  m = -INFINITY;
+  s = 0.f;
+  for (int w = 0; w < kWarps; ++w) stat_merge(m, s, sh.wm[w], sh.ws[w], c);
+  if (parts > 1) {
+    if (tid == 0) {
+      sh.pm = m;
+      sh.ps = s;
+    }
+    cl.sync();
+    if (part == 0) {
+      for (int r = 1; r < parts; ++r) {
+        RowShared* o = cl.map_shared_rank(&sh, r);
+        stat_merge(m, s, o->pm, o->ps, c);
+      }
+    }
+    cl.sync();  // no part leaves before its sums are read
+    if (part != 0) return;
+  }
+  finish_row(sh.b, sh.red, row, k, zk, t, slot >= 0, m, s, c, tau, reverse, tail, out);
+}
+
+// d[n, j] = -g gs 2^((z - m)·c), and g · entry at the entries of S; rows without a gradient are zeros and are not read.
+template <typename T, typename O>
+__global__ void __launch_bounds__(kThreads) distill_rows_bwd_kernel(const T* __restrict__ logits, long long stride,
+                                                                    int v, const int* __restrict__ slots,
+                                                                    const float* __restrict__ ref,
+                                                                    const float* __restrict__ gs,
+                                                                    const float* __restrict__ entry,
+                                                                    const float* __restrict__ grad, int k, float tau,
+                                                                    int parts, O* __restrict__ out, long long ostride) {
+  constexpr int VEC = Slice<T>::kVec;
+  const long long row = blockIdx.x / parts;
+  const int part = blockIdx.x % parts;
+  const int tid = threadIdx.x;
+  const float c = kLog2e / tau;
+  const float g = grad[row];
+  const float coef = g == 0.f ? 0.f : -g * gs[row];
+  const float m = ref[row];
+  Slice<T> sl(logits + row * stride, v, part, parts);
+  O* o = out + row * ostride + sl.lo;
+  auto d = [&](float z) { return coef * ex2((z - m) * c); };
+  if (tid < sl.head + sl.tail) {
+    const int i = tid < sl.head ? tid : sl.nvec * VEC + tid;
+    o[i] = from_f<O>(coef == 0.f ? 0.f : d(to_f(sl.p[i])));
+  }
+  const T* body = sl.body();
+  O* ob = o + sl.head;
+  constexpr int OB = VEC * sizeof(O);  // output bytes of a vector: 8, 16 or 32
+  const bool wide = (reinterpret_cast<uintptr_t>(ob) % (OB < 16 ? OB : 16)) == 0;
+  constexpr int U = 16 / VEC;
+  for (int i0 = tid; i0 < sl.nvec; i0 += U * kThreads) {
+    uint4 raw[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j)
+      if (coef != 0.f && i0 + j * kThreads < sl.nvec) raw[j] = load_stream(body + (long long)(i0 + j * kThreads) * VEC);
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int i = i0 + j * kThreads;
+      if (i >= sl.nvec) break;
+      float z[VEC];
+      if (coef == 0.f) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) z[e] = 0.f;
+      } else {
+        unpack<T>(raw[j], z);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) z[e] = d(z[e]);
+      }
+      O* w = ob + (long long)i * VEC;
+      if (wide) {
+        union {
+          O e[VEC];
+          uint4 q[OB >= 16 ? OB / 16 : 1];
+          uint2 h;
+        } u;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) u.e[e] = from_f<O>(z[e]);
+        if constexpr (OB == 8) {
+          *reinterpret_cast<uint2*>(w) = u.h;
+        } else {
+#pragma unroll
+          for (int q = 0; q < OB / 16; ++q) reinterpret_cast<uint4*>(w)[q] = u.q[q];
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) w[e] = from_f<O>(z[e]);
+      }
+    }
+  }
+  __syncthreads();
+  if (tid < k) {
+    const int slot = slots[row * k + tid];
+    if (slot >= sl.lo && slot < sl.lo + sl.n)
+      o[slot - sl.lo] = from_f<O>(g == 0.f ? 0.f : g * entry[row * k + tid]);
+  }
+}
+
+// Parts of a row: one where the rows alone fill the SMs, up to eight where there are few.
+int row_parts(int64_t rows, int v, int sms) {
+  int parts = 1;
+  while (parts < kMaxParts && rows * parts < 4 * sms && v / (2 * parts) >= 4096) parts *= 2;
+  return parts;
+}
+
+template <typename T>
+cudaError_t fwd_of(const VocabLaunch& l, const VocabRows& x, const DistillArgs& a, const DistillOut& out) {
+  int parts = row_parts(x.n, x.v, l.sms);
+  while (parts < kMaxParts && x.v / parts > 1000000) parts *= 2;  // the bitmap has to fit
+  const int len = ((x.v + parts - 1) / parts + 63) / 64 * 64;
+  const int words = (len + 16 + 31) / 32 + 1;
+  const cudaError_t e = l.set_smem((const void*)distill_rows_fwd_kernel<T>, words * 4);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(x.n * parts));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = words * 4;
+  cfg.stream = l.stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = parts;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, distill_rows_fwd_kernel<T>, (const T*)x.logits, x.stride, x.v, a.ids, a.lp, a.k, a.tau,
+                            a.reverse, a.tail, out, words);
+}
+
+template <typename T, typename O>
+cudaError_t bwd_of(const VocabLaunch& l, const VocabRows& x, const DistillArgs& a, const DistillOut& f,
+                   const float* grad, void* out, long long ostride) {
+  const int parts = row_parts(x.n, x.v, l.sms);
+  distill_rows_bwd_kernel<T, O><<<(unsigned)(x.n * parts), kThreads, 0, l.stream>>>(
+      (const T*)x.logits, x.stride, x.v, f.slots, f.ref, f.gs, f.entry, grad, a.k, a.tau, parts, (O*)out, ostride);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t distill_rows_forward(const VocabLaunch& l, const VocabRows& x, const DistillArgs& a, const DistillOut& out) {
+  switch (x.type) {
+    case kRowsF32: return fwd_of<float>(l, x, a, out);
+    case kRowsBf16: return fwd_of<__nv_bfloat16>(l, x, a, out);
+    default: return fwd_of<__half>(l, x, a, out);
+  }
+}
+
+cudaError_t distill_rows_backward(const VocabLaunch& l, const VocabRows& x, const DistillArgs& a, const DistillOut& f,
+                                  const float* grad, RowType otype, void* out, long long ostride) {
+  if (x.type == kRowsF32) {
+    if (otype == kRowsF32) return bwd_of<float, float>(l, x, a, f, grad, out, ostride);
+    if (otype == kRowsBf16) return bwd_of<float, __nv_bfloat16>(l, x, a, f, grad, out, ostride);
+    return bwd_of<float, __half>(l, x, a, f, grad, out, ostride);
+  }
+  if (otype != x.type) return cudaErrorInvalidValue;
+  if (x.type == kRowsBf16) return bwd_of<__nv_bfloat16, __nv_bfloat16>(l, x, a, f, grad, out, ostride);
+  return bwd_of<__half, __half>(l, x, a, f, grad, out, ostride);
+}
+
+cudaError_t distill_bounds(unsigned long long* word, bool reset) {
+  cudaError_t e = cudaMemcpyFromSymbol(word, g_bounds_word, sizeof(*word));
+  if (e == cudaSuccess && reset && *word != 0) {
+    const unsigned long long zero = 0;
+    e = cudaMemcpyToSymbol(g_bounds_word, &zero, sizeof(zero));
+  }
+  return e;
+}
+
+}  // namespace ts

@@ -1,0 +1,109 @@
+// Pieces shared by the kernels that walk rows of a vocabulary (csrc/vocab_select.cu, csrc/distill.cu).
+//
+// A row of V logits (fp32, bf16 or fp16; any row stride, any alignment of the type) is cut into `parts` slices, one
+// per CTA of a cluster; a slice is an unaligned head, a body of 16-byte vectors and a tail. Log-sum-exp statistics
+// are kept online as (m, s): the largest logit and s = sum of 2^((z - m)·c), c = log2(e)/temperature.
+#pragma once
+
+#include "common.cuh"
+
+#include <cooperative_groups.h>
+
+namespace ts {
+namespace vocab {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+TS_DEVICE float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 2^((z - m)·c) for z <= m; an m of -inf (nothing but -inf so far) stands for 0
+TS_DEVICE float rel_exp(float z, float m, float c) { return ex2((z - (m == -INFINITY ? 0.f : m)) * c); }
+
+// Sum of rel_exp over N values. z·c - m·c as one multiply-add: the product is exact inside it, so what is rounded is
+// m·c, the same for all values, and the difference. Masks of a type's lowest value (m·c past fp32) subtract first.
+template <int N>
+TS_DEVICE float sum_exp(const float* z, float m, float c) {
+  float s0 = 0.f, s1 = 0.f;
+  if (m > -1e30f) {
+    const float r = m * c;
+#pragma unroll
+    for (int e = 0; e + 1 < N; e += 2) {
+      s0 += ex2(fmaf(z[e], c, -r));
+      s1 += ex2(fmaf(z[e + 1], c, -r));
+    }
+    if (N & 1) s0 += ex2(fmaf(z[N - 1], c, -r));
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) s0 += rel_exp(z[e], m, c);
+  }
+  return s0 + s1;
+}
+
+// (m, s): raise the reference to `to`, or merge another pair. An empty side has m = -inf and s = 0 (or NaN: it stays).
+TS_DEVICE void stat_raise(float& m, float& s, float to, float c) {
+  if (to > m) {
+    if (m != -INFINITY) s *= rel_exp(m, to, c);
+    m = to;
+  }
+}
+TS_DEVICE void stat_merge(float& m, float& s, float m2, float s2, float c) {
+  const float mx = fmaxf(m, m2);
+  s = s * (m == -INFINITY ? 1.f : rel_exp(m, mx, c)) + s2 * (m2 == -INFINITY ? 1.f : rel_exp(m2, mx, c));
+  m = mx;
+}
+
+template <typename T>
+struct Slice {
+  static constexpr int kVec = 16 / sizeof(T);
+  const T* p;  // first element
+  int lo;      // its token id
+  int n, head, nvec, tail;
+
+  TS_DEVICE Slice(const T* row, int v, int part, int parts) {
+    const int len = ((v + parts - 1) / parts + 63) / 64 * 64;
+    lo = (int)min((long long)v, (long long)part * len);
+    n = min(len, v - lo);
+    p = row + lo;
+    const int off = (int)((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));
+    head = min(n, off ? kVec - off : 0);
+    nvec = (n - head) / kVec;
+    tail = n - head - nvec * kVec;
+  }
+  TS_DEVICE const T* body() const { return p + head; }
+};
+
+TS_DEVICE uint4 load_stream(const void* p) {
+  uint4 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p));
+  return r;
+}
+
+template <typename T>
+TS_DEVICE void unpack(const uint4& raw, float* v) {
+  Vec<T> x;
+  x.raw = raw;
+#pragma unroll
+  for (int e = 0; e < Vec<T>::N; ++e) v[e] = to_f(x.e[e]);
+}
+
+// Order of the logits as unsigned integers: larger is greater, equal values (also -0 and +0) are equal, NaN is least.
+TS_DEVICE uint32_t order_key(float v) {
+  const uint32_t u = __float_as_uint(v + 0.f);
+  if (v != v) return 0u;
+  return u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u);
+}
+TS_DEVICE float key_value(uint32_t k) { return __uint_as_float((k >> 31) ? k ^ 0x80000000u : ~k); }
+// Rank of (logit, token) in one word: greater logits first, then lower tokens.
+TS_DEVICE uint64_t rank_key(float v, int id) { return ((uint64_t)order_key(v) << 32) | (uint32_t)~(uint32_t)id; }
+TS_DEVICE int rank_id(uint64_t k) { return (int)~(uint32_t)k; }
+TS_DEVICE float rank_value(uint64_t k) { return key_value((uint32_t)(k >> 32)); }
+
+}  // namespace vocab
+}  // namespace ts

@@ -1,0 +1,271 @@
+"""Distillation from a teacher's top logits: the teacher's entries, and the loss against them with its gradient.
+
+A teacher that scores a position with its ``k`` most likely tokens (ids and log-probs, :func:`topk_logprobs`) says far
+more about it than the log-prob of the one sampled token, at a few hundred bytes per position. The loss compares them
+with the student's distribution ``p = softmax(z / temperature)`` over the whole vocabulary. Per row, with the entries'
+set ``S``, ``q = exp(teacher log-prob)``, and ``P``, ``Q`` what ``p`` and ``q`` give to all other tokens together:
+
+    direction "forward":  sum_S q (log q - log p)  [+ Q (log Q - log P)]      KL(teacher || student)
+    direction "reverse":  sum_S p (log p - log q)  [+ P (log P - log Q)]      KL(student || teacher)
+
+``tail=True`` adds the bracketed term (all other tokens as one class; ``Q`` is held at 1e-7 at least, and the term is
+left out where the student gives the others nothing). The teacher is a constant: no gradient reaches it.
+
+An entry with id -1 or log-prob -inf is no entry, so rows may have fewer than ``K``; of entries with the same id the
+first counts. A row without entries has loss 0 and gradient 0, whatever its logits are. A row whose logits hold NaN,
++inf, or nothing but -inf has loss NaN.
+
+:func:`topk_distill_loss` takes logits that are in memory; :func:`lm_head_topk_distill` takes hidden states and the
+LM-head weight. Sums, softmax statistics and the entries' arithmetic are fp32 or wider; the gradient is rounded once,
+to the logits' type.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from thundersync_b200.ops import sink as _sink
+from thundersync_b200.ops._ext import native
+from thundersync_b200.ops.gemm import gemm, gemm_accumulate
+from thundersync_b200.ops.logprob import DEFAULT_ROWS, _logits_fp32, _row_block
+
+__all__ = ["topk_logprobs", "topk_distill_loss", "lm_head_topk_distill", "MAX_ENTRIES"]
+
+MAX_ENTRIES = 256  # teacher entries of a row (one per thread of a row's block)
+_TAIL_FLOOR = 1e-7
+_NATIVE = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _native_rows(logits: torch.Tensor) -> bool:
+    return logits.is_cuda and logits.dtype in _NATIVE
+
+
+def _rows_contiguous(t: torch.Tensor) -> torch.Tensor:
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+def _check_logits(logits: torch.Tensor) -> None:
+    if logits.dim() != 2 or not logits.is_floating_point():
+        raise ValueError(f"logits must be a floating-point [N, V], got {logits.dtype} {tuple(logits.shape)}")
+    if logits.shape[1] < 1:
+        raise ValueError("logits must have a vocabulary")
+
+
+def _check_teacher(n: int, ids, logprobs, temperature: float, direction: str, device):
+    if ids.dim() != 2 or ids.shape[0] != n or not 1 <= ids.shape[1] <= MAX_ENTRIES:
+        raise ValueError(f"teacher_ids must be [N, K] with N = {n} and K in [1, {MAX_ENTRIES}], got {tuple(ids.shape)}")
+    if ids.is_floating_point() or ids.dtype == torch.bool:
+        raise ValueError("teacher_ids must be integers")
+    if logprobs.shape != ids.shape or not logprobs.is_floating_point():
+        raise ValueError(f"teacher_logprobs must be floating-point {tuple(ids.shape)}, got {logprobs.dtype} "
+                         f"{tuple(logprobs.shape)}")
+    if logprobs.requires_grad:
+        raise ValueError("teacher_logprobs must be detached")
+    if ids.device != device or logprobs.device != device:
+        raise ValueError("the teacher's entries must be on the student's device")
+    if not (temperature > 0 and math.isfinite(temperature)):
+        raise ValueError(f"temperature must be positive, got {temperature}")
+    if direction not in ("forward", "reverse"):
+        raise ValueError(f"direction must be 'forward' or 'reverse', got {direction!r}")
+    wide = torch.float64 if logprobs.dtype == torch.float64 and not ids.is_cuda else torch.float32
+    return ids.to(torch.int64).contiguous(), logprobs.to(wide).contiguous()
+
+
+# ------------------------------------------------------------------ the teacher's side
+def topk_logprobs(logits: torch.Tensor, k: int, *, temperature: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """The ``k`` most likely tokens of each row of ``logits`` [N, V], most likely first: (ids int64 [N, k], log-probs
+    fp32 [N, k] under ``softmax(logits / temperature)``).
+
+    Equal logits: the lower token comes first. NaN counts as less than -inf, and a row that holds NaN or +inf has
+    log-probs NaN; a row of -inf alone has log-probs -inf.
+    """
+    _check_logits(logits)
+    k = int(k)
+    if not 1 <= k <= min(MAX_ENTRIES, logits.shape[1]):
+        raise ValueError(f"k must be in [1, {min(MAX_ENTRIES, logits.shape[1])}], got {k}")
+    if not (temperature > 0 and math.isfinite(temperature)):
+        raise ValueError(f"temperature must be positive, got {temperature}")
+    logits = logits.detach()
+    if _native_rows(logits):
+        ids, lp = native().topk_logprobs(_rows_contiguous(logits), k, float(temperature))
+        return ids, lp
+    return _topk_reference(logits, k, temperature)
+
+
+def _topk_reference(logits, k, temperature):
+    z = logits.to(torch.float64 if logits.dtype == torch.float64 else torch.float32)
+    order = torch.where(z.isnan(), -math.inf, z)
+    top, ids = order.sort(dim=-1, descending=True, stable=True)
+    if bool(z.isnan().any()):  # NaN after -inf
+        last = z.isnan().gather(-1, ids)
+        ids = ids.gather(-1, last.to(torch.int8).sort(dim=-1, stable=True)[1])
+    ids = ids[:, :k].contiguous()
+    m = z.amax(-1, keepdim=True)
+    m = torch.where(m == -math.inf, 0.0, m)
+    total = torch.exp((z - m) / temperature).sum(-1, keepdim=True)
+    lp = (z.gather(-1, ids) - m) / temperature - torch.where(total == 0, 0.0, torch.log(total))
+    return ids, lp.to(torch.float32)
+
+
+# ------------------------------------------------------------------ the loss on logits
+def _slots(ids, logprobs, v: int):
+    """Which entries count: inside the vocabulary, with a probability, first of their id."""
+    have = (ids >= 0) & (ids < v) & (logprobs != -math.inf)
+    k = ids.shape[1]
+    same = (ids[:, :, None] == ids[:, None, :]) & have[:, None, :]
+    earlier = torch.ones(k, k, dtype=torch.bool, device=ids.device).tril(-1)
+    return have & ~(same & earlier).any(-1)
+
+
+def _loss_reference(z, ids, logprobs, temperature, direction, tail):
+    """The definition in plain torch, differentiable in ``z`` [N, V] (fp32 or fp64)."""
+    n, v = z.shape
+    have = _slots(ids, logprobs, v)
+    used = have.any(-1)
+    z = torch.where(used[:, None], z, torch.zeros_like(z))
+    logp = torch.log_softmax(z / temperature, -1)
+    at = torch.where(have, ids, 0)
+    t = torch.where(have, logprobs.to(z.dtype), torch.zeros((), dtype=z.dtype, device=z.device))
+    a = logp.gather(-1, at)
+    if direction == "forward":
+        loss = torch.where(have, t.exp() * (t - a), torch.zeros_like(a)).sum(-1)
+    else:
+        p = a.exp()
+        on = have & ((p > 0) | p.isnan())
+        a = torch.where(on, a, torch.zeros_like(a))
+        loss = torch.where(on, a.exp() * (a - t), torch.zeros_like(a)).sum(-1)
+    if tail:
+        inside = torch.zeros(n, v, dtype=torch.bool, device=z.device)
+        rows = torch.arange(n, device=z.device)[:, None].expand_as(at)
+        inside[rows[have], at[have]] = True
+        rest = logp.masked_fill(inside, -math.inf)
+        some = used & (rest.exp().sum(-1) != 0)  # (NaN stays)
+        lpt = torch.logsumexp(torch.where(some[:, None], rest, torch.zeros_like(rest)), -1)
+        qt = (1.0 - torch.where(have, t.exp(), torch.zeros_like(t)).sum(-1)).clamp(min=_TAIL_FLOOR)
+        more = qt * (qt.log() - lpt) if direction == "forward" else lpt.exp() * (lpt - qt.log())
+        loss = loss + torch.where(some, more, torch.zeros_like(more))
+    return loss
+
+
+class _TopkDistillRows(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, ids, logprobs, temperature, direction, tail):
+        ctx.temperature = temperature
+        loss, slots, ref, gs, entry = native().distill_rows_fwd(logits, ids, logprobs, temperature,
+                                                                direction == "reverse", tail)
+        ctx.save_for_backward(logits, slots, ref, gs, entry)
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        logits, slots, ref, gs, entry = ctx.saved_tensors
+        d = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        native().distill_rows_bwd(logits, slots, ref, gs, entry, g.float().contiguous(), ctx.temperature, d)
+        return d, None, None, None, None, None
+
+
+def topk_distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logprobs: torch.Tensor, *,
+                      temperature: float = 1.0, direction: str = "forward", tail: bool = True) -> torch.Tensor:
+    """Loss [N] (fp32) of student ``logits`` [N, V] against the teacher's entries [N, K], differentiable in ``logits``.
+
+    ``teacher_logprobs`` are under the teacher's distribution at the same ``temperature``."""
+    _check_logits(logits)
+    ids, lp = _check_teacher(logits.shape[0], teacher_ids, teacher_logprobs, temperature, direction, logits.device)
+    if _native_rows(logits):
+        return _TopkDistillRows.apply(_rows_contiguous(logits), ids, lp, float(temperature), direction, bool(tail))
+    z = logits if logits.dtype == torch.float64 else logits.float()
+    return _loss_reference(z, ids, lp, temperature, direction, tail)
+
+
+# ------------------------------------------------------------------ the loss from hidden states
+class _HeadTopkDistill(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, ids, logprobs, rows, temperature, direction, tail):
+        n = hidden.shape[0]
+        ctx.conf = (rows, temperature, direction, tail)
+        ctx.weight = weight
+        ctx.save_for_backward(hidden, ids, logprobs)
+        ctx.blocks = []
+        loss = []
+        for r0 in range(0, n, rows):
+            r1 = min(n, r0 + rows)
+            logits = _logits_fp32(hidden[r0:r1], weight)
+            if _native_rows(logits):
+                part, *kept = native().distill_rows_fwd(logits, ids[r0:r1], logprobs[r0:r1], temperature,
+                                                        direction == "reverse", tail)
+                ctx.blocks.append(kept)
+            else:
+                part = _loss_reference(logits, ids[r0:r1], logprobs[r0:r1], temperature, direction, tail)
+            loss.append(part)
+        return torch.cat(loss) if loss else hidden.new_zeros(0, dtype=torch.float32)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        hidden, ids, logprobs = ctx.saved_tensors
+        weight = ctx.weight
+        rows, temperature, direction, tail = ctx.conf
+        n = hidden.shape[0]
+        need_h, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+        dh = torch.empty_like(hidden) if need_h else None
+        s = _sink.active()
+        sink_w = need_w and s is not None and s.owns(weight)
+        dw = None
+        if need_w and not sink_w:
+            wide = torch.float32 if weight.dtype != torch.float64 else torch.float64
+            dw = torch.zeros(weight.shape, dtype=wide, device=weight.device)
+        g = g.contiguous()
+        for i, r0 in enumerate(range(0, n, rows)):
+            r1 = min(n, r0 + rows)
+            h = hidden[r0:r1]
+            logits = _logits_fp32(h, weight)
+            if _native_rows(logits):
+                d = torch.empty(logits.shape, dtype=hidden.dtype, device=hidden.device)
+                native().distill_rows_bwd(logits, *ctx.blocks[i], g[r0:r1].float(), temperature, d)
+            else:
+                with torch.enable_grad():
+                    z = logits.requires_grad_(True)
+                    part = _loss_reference(z, ids[r0:r1], logprobs[r0:r1], temperature, direction, tail)
+                (d,) = torch.autograd.grad(part, z, g[r0:r1].to(part.dtype))
+                d = d.to(hidden.dtype)
+            del logits
+            if need_h:
+                gemm(d, weight, b_t=False, out=dh[r0:r1])
+            if need_w:
+                if sink_w:
+                    s.addmm_(s.view(weight), d, h)
+                else:
+                    gemm_accumulate(dw, d, h, a_t=True, b_t=False)
+        ctx.weight = None
+        ctx.blocks = None
+        return dh, None if dw is None else dw.to(weight.dtype), None, None, None, None, None, None
+
+
+def lm_head_topk_distill(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torch.Tensor,
+                         teacher_logprobs: torch.Tensor, *, temperature: float = 1.0, direction: str = "forward",
+                         tail: bool = True, rows: int = DEFAULT_ROWS) -> torch.Tensor:
+    """Loss [N] (fp32) of the student ``hidden`` [N, D] · ``weight`` [V, D]ᵀ against the teacher's entries [N, K],
+    differentiable in ``hidden`` and ``weight`` (whose gradient honours an active gradient sink). ``rows`` rows are
+    worked at a time: buffers over the vocabulary hold one block. Hidden rows must be finite (a row without entries
+    gives no gradient, but its zeros meet the hidden row in the weight gradient)."""
+    if hidden.dim() != 2:
+        raise ValueError(f"hidden must be [N, D], got {tuple(hidden.shape)}")
+    if weight.dim() != 2 or weight.shape[1] != hidden.shape[1]:
+        raise ValueError(f"weight {tuple(weight.shape)} does not match hidden dim {hidden.shape[1]}")
+    if weight.dtype != hidden.dtype or weight.device != hidden.device:
+        raise ValueError("hidden and weight must have one dtype and device")
+    ids, lp = _check_teacher(hidden.shape[0], teacher_ids, teacher_logprobs, temperature, direction, hidden.device)
+    n = hidden.shape[0]
+    rows = _row_block(rows, hidden.is_cuda)
+    h = hidden.contiguous()
+    pad = (-n) % 8 if hidden.is_cuda else 0  # the weight gradient's contraction runs over whole groups of 8 rows
+    if pad:
+        h = torch.cat((h, h.new_zeros(pad, h.shape[1])))
+        ids = torch.cat((ids, ids.new_full((pad, ids.shape[1]), -1)))
+        lp = torch.cat((lp, lp.new_zeros(pad, lp.shape[1])))
+    loss = _HeadTopkDistill.apply(h, weight, ids, lp, rows, float(temperature), direction, bool(tail))
+    return loss[:n] if pad else loss
