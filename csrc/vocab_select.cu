@@ -6,10 +6,14 @@
 //   (the smallest of independent exponential times with rates w_i). All three filters keep a prefix of the rank
 //   order (greater logit first, then lower token), which is what the kernels use.
 //
-// One pass over the row. A slice keeps a threshold under which no element can be among its k largest, appends the
-// elements above it to a buffer in shared memory and, when that runs full, cuts it back to the k best (radix select
-// on 64-bit words of logit order and token, so that there are no ties) and raises the threshold. The first tile's
-// threshold is the k-th largest of the threads' own maxima.
+// Both are bound by reading the logits once. A thread copies its own vectors through a private ring in shared memory
+// (cp.async, no barriers), so many loads are in flight without registers. Selection: elements above a threshold that
+// at least k elements reach go to a buffer; when that fills, it is cut back to the k best (radix select on 64-bit
+// words of logit order and token, so that there are no ties) and the threshold rises. The first threshold comes from
+// the threads' maxima over their first vectors.
+//
+// Which rows read the random numbers: with a small kept set only its tokens' (the list of the 256 best usually holds
+// all that is kept); without any filter all of them, in the same single pass as the logits.
 #include "common.cuh"
 #include "vocab.cuh"
 #include "vocab.h"
@@ -20,48 +24,68 @@ namespace {
 namespace cg = cooperative_groups;
 using namespace vocab;
 
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTop = 256;
-constexpr int kPer = 16;                     // elements of a thread in a tile
-constexpr int kTile = kThreads * kPer;       // 4096
-constexpr int kLimit = 1024;                 // entries that are kept before the buffer is cut back
-constexpr int kCap = kLimit + kTile + 32;
 constexpr int kMaxParts = 8;
-static_assert(kMaxParts * kMaxTop <= kCap, "the parts' lists meet in one buffer");
+constexpr int kLimit = 768;                  // entries at which the buffer is cut back, at most
+constexpr int kStep = 4;                     // vectors of a thread between two looks at the buffer
+constexpr int kRing = 6;                     // vectors of a thread in flight
+constexpr float kColdest = 1e-6f;            // colder rows are greedy
 
+// The buffer holds the limit and one vector of each thread (the step of the careful path), and the parts' lists.
+template <typename T, int NT> constexpr int buf_cap() {
+  return kLimit + NT * Slice<T>::kVec + 32 > kMaxParts * kMaxTop ? kLimit + NT * Slice<T>::kVec + 32
+                                                                 : kMaxParts * kMaxTop;
+}
+template <typename T, int NT> constexpr int work_bytes() { return buf_cap<T, NT>() * 8 + kRing * NT * 16; }
+
+template <typename T, int NT>
 struct Shared {
-  uint64_t buf[kCap];
   uint64_t win[kMaxTop];
-  uint32_t hist[256];
-  float wm[kWarps], ws[kWarps];
-  uint64_t wbest[kWarps];
-  // this CTA's partial results, read by its cluster (two sets, used in turn)
+  uint64_t wbest[NT / 32];
+  uint64_t pbest[2];  // this CTA's partial results, read by its cluster (two sets, used in turn)
+  float wm[NT / 32], ws[NT / 32];
+  int wc[NT / 32];
+  uint32_t group[kMaxTop], hist[256];
   float pm[2], ps[2];
-  uint64_t pbest[2];
-  int pcount[2];
-  int count;      // entries in buf
-  int nwin;       // entries in win
+  int pcount[2], pflag[2];
+  int count;          // entries appended to the buffer (may pass its capacity: then they were not stored)
+  int nwin;           // entries in win
   int sel_need, sel_bin, sel_done;
-  int verdict;    // of part 0: 0 done, 1 the general search follows
+  int verdict;        // of part 0: 0 done, else the search over all tokens follows
+  __align__(16) uint8_t work[work_bytes<T, NT>()];
+
+  __device__ uint64_t* buf() { return reinterpret_cast<uint64_t*>(work); }
+  __device__ uint4* ring() { return reinterpret_cast<uint4*>(work + buf_cap<T, NT>() * 8); }
 };
+
+TS_DEVICE void copy16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
+               : "memory");
+}
+TS_DEVICE void copy4(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
+               : "memory");
+}
+TS_DEVICE void copy_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+template <int N> TS_DEVICE void copy_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
 
 struct Stat {
   float m = -INFINITY, s = 0.f;
 };
 
-// Leaves the `k` largest of sh.buf[0, n) in sh.win (unordered) and a lower bound of the smallest in `least`;
-// n >= k. All threads call it after a barrier that follows the last write to buf.
-__device__ void select_k(Shared& sh, int n, int k, uint64_t& least) {
+// Moves the `k` largest of buf[0, n) to sh.win (in no order); `least` is a lower bound of them above which no other
+// entry is. n >= k. All threads call it after a barrier that follows the last write to buf.
+template <typename T, int NT>
+__device__ void select_k(Shared<T, NT>& sh, int n, int k, uint64_t& least) {
   uint64_t prefix = 0;  // decided digits of the k-th largest
   int need = k;
-  int shift = 56;
   const int tid = threadIdx.x;
-  for (;; shift -= 8) {
-    sh.hist[tid] = 0;
+  const uint64_t* buf = sh.buf();
+  for (int shift = 56;; shift -= 8) {
+    if (tid < 256) sh.hist[tid] = 0;
     __syncthreads();
-    for (int i = tid; i < n; i += kThreads) {
-      const uint64_t x = sh.buf[i];
+    for (int i = tid; i < n; i += NT) {
+      const uint64_t x = buf[i];
       if (shift == 56 || (x >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&sh.hist[(x >> shift) & 255], 1u);
     }
     __syncthreads();
@@ -98,8 +122,8 @@ __device__ void select_k(Shared& sh, int n, int k, uint64_t& least) {
   least = prefix;
   if (tid == 0) sh.nwin = 0;
   __syncthreads();
-  for (int i = tid; i < n; i += kThreads) {
-    const uint64_t x = sh.buf[i];
+  for (int i = tid; i < n; i += NT) {
+    const uint64_t x = buf[i];
     if (x >= prefix) {
       const int at = atomicAdd(&sh.nwin, 1);
       if (at < kMaxTop) sh.win[at] = x;
@@ -108,154 +132,239 @@ __device__ void select_k(Shared& sh, int n, int k, uint64_t& least) {
   __syncthreads();
 }
 
-// The slice's k largest (all of it where it is shorter) in sh.win / sh.nwin, and its statistics per thread.
-template <typename T>
-__device__ void scan_slice(Shared& sh, const Slice<T>& sl, int k, float c, Stat& st) {
-  constexpr int VEC = Slice<T>::kVec;
-  constexpr int U = kPer / VEC;
+// A threshold that at least k of the threads' values reach (0: none found), the same in all threads: exact but for
+// the last 12 bits. Values of 32 (k <= 16) or 256 groups of threads; each warp searches them for itself.
+template <typename T, int NT>
+__device__ uint32_t group_threshold(Shared<T, NT>& sh, uint32_t mine, int k) {
   const int tid = threadIdx.x, lane = tid & 31;
-  const T* body = sl.body();
-  if (tid == 0) sh.count = 0;
+  constexpr int kSmall = NT / 32 >= 32 ? 16 : 0;  // 32 groups are a warp each
+  const bool few = k <= kSmall;
+  const int width = few ? NT / 32 : NT / 256;  // threads of a group
+  uint32_t x = mine;
+  for (int o = 1; o < width; o <<= 1) x = max(x, __shfl_xor_sync(0xffffffffu, x, o));
+  if (tid % width == 0) sh.group[tid / width] = x;
   __syncthreads();
-
-  bool open = true;        // no threshold yet: every element is appended
-  uint32_t tkey = 0;       // else: elements whose order is above it (strictly: at equal logits the lower token is in)
-
-  // appends this thread's elements whose bit is set in `take`; returns the entries used so far (of this warp's view)
-  auto append = [&](uint32_t take, auto&& entry) -> int {
-    const int mine = __popc(take);
-    int incl = mine;
+  uint32_t v[8];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += up;
+  for (int j = 0; j < 8; ++j) v[j] = (j == 0 || !few) ? sh.group[lane + 32 * j] : 0u;
+  uint32_t mx = 0, mn = 0xffffffffu;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    mx = max(mx, v[j]);
+    if (j == 0 || !few) mn = min(mn, v[j]);
+  }
+  mx = __reduce_max_sync(0xffffffffu, mx);
+  mn = __reduce_min_sync(0xffffffffu, mn);
+  if (mn == mx) return mx;
+  const int top = 31 - __clz(mn ^ mx);
+  uint32_t lo = top >= 31 ? 0u : (mx >> (top + 1)) << (top + 1);  // the digits that all have
+  for (int bit = top; bit >= 12; --bit) {
+    const uint32_t cand = lo | (1u << bit);
+    int cnt;
+    if (few) {
+      cnt = __popc(__ballot_sync(0xffffffffu, v[0] >= cand));
+    } else {
+      int c = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) c += v[j] >= cand;
+      cnt = (int)__reduce_add_sync(0xffffffffu, (unsigned)c);
     }
-    const int total = __shfl_sync(0xffffffffu, incl, 31);
-    if (total == 0) return 0;
-    int base = 0;
-    if (lane == 31) base = atomicAdd(&sh.count, total);
-    base = __shfl_sync(0xffffffffu, base, 31);
-    int at = base + incl - mine;
-    while (take) {
-      const int e = __ffs(take) - 1;
-      take &= take - 1;
-      if (at < kCap) sh.buf[at] = entry(e);
-      ++at;
-    }
-    return base + total;
+    if (cnt >= k) lo = cand;
+    if (cnt == k) break;
+  }
+  return lo;
+}
+
+// Largest of a vector's values; NaN is left out (-inf if there is nothing else).
+template <int N>
+TS_DEVICE float vec_max(const float* z) {
+  float x = -INFINITY;
+#pragma unroll
+  for (int e = 0; e < N; ++e) x = fmaxf(x, z[e]);
+  return x;
+}
+
+// Leaves the slice's k largest (all of it where it is shorter) in sh.win, sh.nwin entries of which some may be
+// smaller, in no order; and this thread's part of the statistics.
+template <typename T, int NT>
+__device__ void scan_slice(Shared<T, NT>& sh, const Slice<T>& sl, int k, float c, Stat& st) {
+  constexpr int VEC = Slice<T>::kVec;
+  const int tid = threadIdx.x;
+  const T* body = sl.body();
+  uint64_t* buf = sh.buf();
+  uint4* ring = sh.ring() + tid;
+  const int limit = min(kLimit, max(4 * k, 128));
+  if (tid == 0) sh.count = 0;
+
+  bool open = true;     // no threshold yet: every element is appended
+  uint32_t tkey = 0;    // else elements whose order is above it (strictly: at equal logits the lower token is in)
+  float tval = 0.f;     // the same as a logit, for a first look at a vector's maximum
+  bool low = false;     // the threshold is below -inf: look at every vector
+  auto set_threshold = [&](uint32_t key) {
+    open = false;
+    tkey = key;
+    low = key < 0x007fffffu;  // -inf's order
+    // -0 has the order of +0: below that, the next logit down
+    tval = key == 0x7fffffffu ? __uint_as_float(0x80000001u) : key_value(key);
   };
-  auto cut = [&]() {  // all threads; buf complete
-    const int n = sh.count;
-    __syncthreads();  // all have read it before anyone appends again
+  auto push = [&](float z, int id) {
+    if (open || order_key(z) > tkey) {
+      const int at = atomicAdd(&sh.count, 1);
+      if (at < buf_cap<T, NT>()) buf[at] = rank_key(z, id);
+    }
+  };
+  auto push_vec = [&](const float* z, int i) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) push(z[e], sl.lo + sl.head + i * VEC + e);
+  };
+  auto cut = [&](int n) {  // all threads; the buffer is complete
     if (n < k) return;
     uint64_t least;
-    select_k(sh, n, k, least);
-    for (int i = tid; i < k; i += kThreads) sh.buf[i] = sh.win[i];
+    select_k<T, NT>(sh, n, k, least);
+    for (int i = tid; i < k; i += NT) buf[i] = sh.win[i];
     if (tid == 0) sh.count = k;
-    open = false;
-    tkey = (uint32_t)(least >> 32);
+    set_threshold((uint32_t)(least >> 32));
     __syncthreads();
   };
-  // the unaligned ends (fewer elements than a vector): one element of each of the first threads
-  auto edge = [&](int first, int cnt) {
-    uint32_t take = 0;
-    float v = -INFINITY;
-    const int i = first + tid;
+
+  const int nvec = sl.nvec;
+  const int mine = tid < nvec ? (nvec - tid + NT - 1) / NT : 0;  // vectors of this thread
+  const int most = (nvec + NT - 1) / NT;                         // of the first thread
+  auto fetch = [&](int j) {
+    if (j < mine) copy16(&ring[(j % kRing) * NT], body + (long long)(j * NT + tid) * VEC);
+    copy_commit();
+  };
+#pragma unroll
+  for (int j = 0; j < kRing; ++j) fetch(j);
+  __syncthreads();
+
+  auto edge = [&](int first, int cnt) {  // the unaligned ends: less than a vector
     if (tid < cnt) {
-      v = to_f(sl.p[i]);
-      stat_raise(st.m, st.s, fmaxf(v, -INFINITY), c);
-      st.s += sum_exp<1>(&v, st.m, c);
-      take = open || order_key(v) > tkey;
-    }
-    if (tid < 32) append(take, [&](int) { return rank_key(v, sl.lo + i); });
-  };
-
-  if (sl.head > 0) edge(0, sl.head);
-
-  const int tiles = (sl.nvec + U * kThreads - 1) / (U * kThreads);
-  uint4 next[U];
-  auto load = [&](int t) {
-#pragma unroll
-    for (int j = 0; j < U; ++j) {
-      const int i = (t * U + j) * kThreads + tid;
-      if (i < sl.nvec) next[j] = load_stream(body + (long long)i * VEC);
+      const int i = first + tid;
+      const float z = to_f(sl.p[i]);
+      stat_raise(st.m, st.s, fmaxf(z, -INFINITY), c);
+      st.s += sum_exp<1>(&z, st.m, c);
+      push(z, sl.lo + i);
     }
   };
-  if (tiles > 0) load(0);
-  for (int t = 0; t < tiles; ++t) {
-    float v[kPer];
-    uint32_t valid = 0;
+  edge(0, sl.head);
+
+  // the first vectors stay in registers until there is a threshold for them
+  int j = 0;
+  if (most > 0) {
+    constexpr int F = VEC == 4 ? 4 : 2;
+    float z[F][VEC];
+    float zmax = -INFINITY;
+    copy_wait<kRing - F>();
 #pragma unroll
-    for (int j = 0; j < U; ++j) {
-      const int i = (t * U + j) * kThreads + tid;
-      if (i < sl.nvec) {
-        unpack<T>(next[j], v + j * VEC);
-        valid |= ((1u << VEC) - 1u) << (j * VEC);
-      } else {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) v[j * VEC + e] = -INFINITY;
+    for (int q = 0; q < F; ++q) {
+      if (q < mine) {
+        unpack<T>(ring[q * NT], z[q]);
+        zmax = fmaxf(zmax, vec_max<VEC>(z[q]));
       }
     }
-    if (t + 1 < tiles) load(t + 1);
-    float tmax = -INFINITY;
+    stat_raise(st.m, st.s, zmax, c);
+    uint32_t best = 0;
+    if (zmax > -INFINITY) best = order_key(zmax);
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) tmax = fmaxf(tmax, v[e]);
-    stat_raise(st.m, st.s, tmax, c);
-    st.s += sum_exp<kPer>(v, st.m, c);
-    if (t == 0 && open) {
-      // a threshold that at least k of the threads' maxima reach: bitwise from the top, exact to 2^-11 of a logit
-      uint32_t mine = 0;
-      if (tmax > -INFINITY) {
-        mine = order_key(tmax);
-      } else {  // nothing but -inf, NaN (which tmax leaves out) and places past the end
+    for (int q = 0; q < F; ++q) {
+      if (q < mine) {
+        st.s += sum_exp<VEC>(z[q], st.m, c);
+        if (!(zmax > -INFINITY)) {  // nothing but -inf and NaN, which zmax leaves out
 #pragma unroll
-        for (int e = 0; e < kPer; ++e)
-          if ((valid >> e) & 1) mine = max(mine, order_key(v[e]));
-      }
-      uint32_t lo = 0;
-      for (int bit = 31; bit >= 12; --bit) {
-        const uint32_t cand = lo | (1u << bit);
-        const int cnt = __syncthreads_count(mine >= cand);
-        if (cnt >= k) lo = cand;
-        if (cnt == k) break;
-      }
-      if (lo > 0) {
-        tkey = lo - 1;
-            open = false;
+          for (int e = 0; e < VEC; ++e) best = max(best, order_key(z[q][e]));
+        }
       }
     }
-    int used = 0;
-    if (__any_sync(0xffffffffu, open || order_key(tmax) > tkey)) {
-      uint32_t take = 0;
 #pragma unroll
-      for (int e = 0; e < kPer; ++e)
-        if (open || order_key(v[e]) > tkey) take |= 1u << e;
-      used = append(take & valid, [&](int e) {
-        float x = 0.f;
+    for (int q = 0; q < F; ++q) fetch(kRing + q);
+    const uint32_t t0 = group_threshold<T, NT>(sh, best, k);
+    if (t0 > 0) set_threshold(t0 - 1);
 #pragma unroll
-        for (int q = 0; q < kPer; ++q)
-          if (q == e) x = v[q];
-        const int i = (t * U + e / VEC) * kThreads + tid;
-        return rank_key(x, sl.lo + sl.head + i * VEC + e % VEC);
-      });
+    for (int q = 0; q < F; ++q)
+      if (q < mine && (open || low || vec_max<VEC>(z[q]) > tval)) push_vec(z[q], q * NT + tid);
+    j = F;
+    __syncthreads();
+    const int n = sh.count;
+    __syncthreads();
+    if (n > buf_cap<T, NT>()) {
+      // more than fit (very many equal logits): once more, a vector of each thread at a time
+      if (tid == 0) sh.count = 0;
+      __syncthreads();
+      if (tid < sl.head) push(to_f(sl.p[tid]), sl.lo + tid);
+      for (int q = 0; q < F; ++q) {
+        if (q < mine) {
+          float x[VEC];
+          unpack<T>(load_stream(body + (long long)(q * NT + tid) * VEC), x);
+          push_vec(x, q * NT + tid);
+        }
+        __syncthreads();
+        const int now = sh.count;
+        __syncthreads();
+        if (now > limit) cut(now);
+      }
+    } else if (n > limit) {
+      cut(n);
     }
-    if (__syncthreads_or(t == 0 || used > kLimit)) cut();
   }
-  if (sl.tail > 0) edge(sl.head + sl.nvec * VEC, sl.tail);
+  while (j < most) {
+    const int from = sh.count;  // uniform: a barrier has passed since the last append
+    __syncthreads();
+    const int j0 = j;
+#pragma unroll
+    for (int q = 0; q < kStep; ++q, ++j) {
+      copy_wait<kRing - 1>();
+      if (j < mine) {
+        float z[VEC];
+        unpack<T>(ring[(j % kRing) * NT], z);
+        fetch(j + kRing);
+        const float zmax = vec_max<VEC>(z);
+        stat_raise(st.m, st.s, zmax, c);
+        st.s += sum_exp<VEC>(z, st.m, c);
+        if (open || low || zmax > tval) push_vec(z, j * NT + tid);
+      } else {
+        copy_commit();
+      }
+    }
+    __syncthreads();
+    const int n = sh.count;
+    __syncthreads();
+    if (n > buf_cap<T, NT>()) {
+      // these vectors brought more than fits: once more from `from`, one vector of each thread at a time
+      if (tid == 0) sh.count = from;
+      __syncthreads();
+      for (int q = j0; q < j0 + kStep && q < most; ++q) {
+        if (q < mine) {
+          float z[VEC];
+          unpack<T>(load_stream(body + (long long)(q * NT + tid) * VEC), z);
+          push_vec(z, q * NT + tid);
+        }
+        __syncthreads();
+        const int now = sh.count;
+        __syncthreads();
+        if (now > limit) cut(now);
+      }
+    } else if (n > limit) {
+      cut(n);
+    }
+  }
+  copy_wait<0>();
+  edge(sl.head + sl.nvec * VEC, sl.tail);
   __syncthreads();
   const int n = sh.count;
-  if (n > k) {
+  if (n > kMaxTop) {
     uint64_t least;
-    select_k(sh, n, k, least);
+    select_k<T, NT>(sh, n, k, least);
   } else {
-    for (int i = tid; i < n; i += kThreads) sh.win[i] = sh.buf[i];
+    for (int i = tid; i < n; i += NT) sh.win[i] = buf[i];
     if (tid == 0) sh.nwin = n;
     __syncthreads();
   }
 }
 
 // Block-wide (m, s); all threads get it.
-__device__ void block_stat(Shared& sh, Stat& st, float c) {
+template <typename T, int NT>
+__device__ void block_stat(Shared<T, NT>& sh, Stat& st, float c) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const float m2 = __shfl_xor_sync(0xffffffffu, st.m, o), s2 = __shfl_xor_sync(0xffffffffu, st.s, o);
@@ -267,14 +376,21 @@ __device__ void block_stat(Shared& sh, Stat& st, float c) {
     sh.ws[threadIdx.x >> 5] = st.s;
   }
   __syncthreads();
-  Stat all;
-  for (int w = 0; w < kWarps; ++w) stat_merge(all.m, all.s, sh.wm[w], sh.ws[w], c);
-  st = all;
+  // each warp merges the warps' pairs, in the same order
+  const int lane = threadIdx.x & 31;
+  st.m = lane < NT / 32 ? sh.wm[lane] : -INFINITY;
+  st.s = lane < NT / 32 ? sh.ws[lane] : 0.f;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, st.m, o), s2 = __shfl_xor_sync(0xffffffffu, st.s, o);
+    stat_merge(st.m, st.s, m2, s2, c);
+  }
 }
 
 // The row's k largest from the parts' lists: part 0 gets them in sh.win in rank order (sh.nwin of them); every part
 // gets the row's statistics.
-__device__ void join_parts(Shared& sh, int k, float c, Stat& st) {
+template <typename T, int NT>
+__device__ void join_parts(Shared<T, NT>& sh, int k, float c, Stat& st) {
   const int tid = threadIdx.x;
   cg::cluster_group cl = cg::this_cluster();
   const int parts = (int)cl.num_blocks();
@@ -285,27 +401,35 @@ __device__ void join_parts(Shared& sh, int k, float c, Stat& st) {
     }
     cl.sync();
     Stat row;
-    for (int r = 0; r < parts; ++r) {
-      Shared* o = cl.map_shared_rank(&sh, r);
-      stat_merge(row.m, row.s, o->pm[0], o->ps[0], c);
+    int off[kMaxParts], n = 0;
+#pragma unroll
+    for (int r = 0; r < kMaxParts; ++r) {
+      if (r < parts) {
+        Shared<T, NT>* o = cl.map_shared_rank(&sh, r);
+        stat_merge(row.m, row.s, o->pm[0], o->ps[0], c);
+        off[r] = n;
+        n += o->nwin;
+      }
     }
     st = row;
-    int n = 0;
-    if (cl.block_rank() == 0) {
-      for (int r = 0; r < parts; ++r) {
-        Shared* o = cl.map_shared_rank(&sh, r);
-        const int cnt = o->nwin;
-        for (int i = tid; i < cnt; i += kThreads) sh.buf[n + i] = o->win[i];
-        n += cnt;
+    const bool first = cl.block_rank() == 0;
+    if (first) {
+#pragma unroll
+      for (int r = 0; r < kMaxParts; ++r) {
+        if (r < parts) {
+          Shared<T, NT>* o = cl.map_shared_rank(&sh, r);
+          const int cnt = (r + 1 < parts ? off[r + 1 < kMaxParts ? r + 1 : r] : n) - off[r];
+          if (tid < cnt) sh.buf()[off[r] + tid] = o->win[tid];
+        }
       }
     }
     cl.sync();
-    if (cl.block_rank() == 0) {
-      uint64_t least;
-      if (n > k) {
-        select_k(sh, n, k, least);
+    if (first) {
+      if (n > kMaxTop) {
+        uint64_t least;
+        select_k<T, NT>(sh, n, k, least);
       } else {
-        for (int i = tid; i < n; i += kThreads) sh.win[i] = sh.buf[i];
+        if (tid < n) sh.win[tid] = sh.buf()[tid];
         if (tid == 0) sh.nwin = n;
         __syncthreads();
       }
@@ -321,30 +445,31 @@ __device__ void join_parts(Shared& sh, int k, float c, Stat& st) {
       for (int j = 0; j < n; ++j) at += sh.win[j] > mine;
     }
     __syncthreads();
-    if (tid < n) sh.win[at] = mine;
+    if (tid < n && at < k) sh.win[at] = mine;
+    if (tid == 0) sh.nwin = min(n, k);
     __syncthreads();
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) topk_kernel(const T* __restrict__ logits, long long stride, int v, int k,
-                                                        float temperature, int64_t* __restrict__ ids,
-                                                        float* __restrict__ logprobs) {
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT) topk_kernel(const T* __restrict__ logits, long long stride, int v, int k,
+                                                  float temperature, int64_t* __restrict__ ids,
+                                                  float* __restrict__ logprobs) {
   extern __shared__ __align__(16) uint8_t raw[];
-  Shared& sh = *reinterpret_cast<Shared*>(raw);
+  Shared<T, NT>& sh = *reinterpret_cast<Shared<T, NT>*>(raw);
   cg::cluster_group cl = cg::this_cluster();
   const int parts = (int)cl.num_blocks();
   const int row = blockIdx.x / parts;
   const float c = kLog2e / temperature;
   Slice<T> sl(logits + row * stride, v, (int)cl.block_rank(), parts);
   Stat st;
-  scan_slice<T>(sh, sl, k, c, st);
+  scan_slice<T, NT>(sh, sl, k, c, st);
   block_stat(sh, st, c);
   join_parts(sh, k, c, st);
   if (cl.block_rank() == 0) {
     const float m = st.m == -INFINITY ? 0.f : st.m;
     const float ls = st.s == 0.f ? 0.f : logf(st.s);  // a row of -inf alone: its log-probs are -inf
-    for (int i = threadIdx.x; i < k; i += kThreads) {
+    for (int i = threadIdx.x; i < k; i += NT) {
       const uint64_t x = sh.win[i];
       ids[(long long)row * k + i] = rank_id(x);
       logprobs[(long long)row * k + i] = (rank_value(x) - m) / temperature - ls;
@@ -352,99 +477,223 @@ __global__ void __launch_bounds__(kThreads) topk_kernel(const T* __restrict__ lo
   }
 }
 
-constexpr float kColdest = 1e-6f;  // colder rows are greedy
-
-// One pass over the slice for the token search of rows whose kept set is not known: of the tokens ranked before
-// `bound` (all, where it is ~0) the number and mass before `bound`, and the best key w/e among those with w >= min_p.
-template <typename T>
-__device__ void scan_keys(const Slice<T>& sl, const float* __restrict__ noise, float m, float temperature,
-                          float min_p, uint64_t bound, int& count, float& mass, uint64_t& best) {
-  constexpr int VEC = Slice<T>::kVec;
-  const int tid = threadIdx.x;
-  auto one = [&](float z, float e, int id) {
-    if (bound != 0 && rank_key(z, id) <= bound) return;
-    const float w = expf((z - m) / temperature);
-    ++count;
-    mass += w;
-    if (w >= min_p) {
-      const float key = w / e;
-      if (key >= 0.f) {
-        const uint64_t x = ((uint64_t)__float_as_uint(key) << 32) | (uint32_t)~(uint32_t)id;
-        if (x > best) best = x;
-      }
-    }
-  };
-  for (int i = tid; i < sl.head; i += kThreads) one(to_f(sl.p[i]), noise[i], sl.lo + i);
-  const T* body = sl.body();
-  const float* nb = noise + sl.head;
-  const bool wide = (reinterpret_cast<uintptr_t>(nb) & 15) == 0;
-  for (int i = tid; i < sl.nvec; i += kThreads) {
-    float z[VEC], e[VEC];
-    unpack<T>(load_stream(body + (long long)i * VEC), z);
-    if (wide) {
-#pragma unroll
-      for (int q = 0; q < VEC; q += 4) unpack<float>(load_stream(nb + (long long)i * VEC + q), e + q);
-    } else {
-#pragma unroll
-      for (int q = 0; q < VEC; ++q) e[q] = nb[(long long)i * VEC + q];
-    }
-#pragma unroll
-    for (int q = 0; q < VEC; ++q) one(z[q], e[q], sl.lo + sl.head + i * VEC + q);
-  }
-  const int t0 = sl.head + sl.nvec * VEC;
-  for (int i = tid; i < sl.tail; i += kThreads) one(to_f(sl.p[t0 + i]), noise[t0 + i], sl.lo + t0 + i);
+// ------------------------------------------------------------------ sampling
+TS_DEVICE float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
-// Row-wide (cluster-wide) sums and best of scan_keys; all threads of all parts get them. `turn` alternates.
-__device__ void join_keys(Shared& sh, int turn, int& count, float& mass, uint64_t& best) {
-  cg::cluster_group cl = cg::this_cluster();
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    count += __shfl_xor_sync(0xffffffffu, count, o);
-    mass += __shfl_xor_sync(0xffffffffu, mass, o);
-    const uint64_t b = __shfl_xor_sync(0xffffffffu, best, o);
-    best = b > best ? b : best;
+// The race's winner so far among this thread's tokens, by y = z·c - log2 e (log2 of the key, up to the row's
+// constant). y is off by less than margin(y), so what counts in the end is the exact key w / e of the few tokens
+// within the margin of the best. A thread keeps one token: `tie` says that another one came as near, and then the
+// tokens are gone over again with exact keys.
+struct Race {
+  float y = -INFINITY, z = 0.f, e = 1.f;
+  int id = -1;
+  bool tie = false;
+
+  // c's and the difference's roundings, 2^-24 each of values up to |y| and log2 e; lg2.approx; the key's own
+  static TS_DEVICE float margin(float y) { return 1e-4f + 1e-6f * fabsf(y); }
+  TS_DEVICE void take(float y2, float z2, float e2, int id2) {
+    if (!(y2 > y - margin(y)) && y != -INFINITY) return;
+    if (!(y2 > -INFINITY)) return;
+    const bool near = y != -INFINITY && !(y2 > y + margin(y));
+    tie = near || y2 == INFINITY;
+    if (y2 > y) {
+      y = y2;
+      z = z2;
+      e = e2;
+      id = id2;
+    }
   }
-  __syncthreads();
-  const int warp = threadIdx.x >> 5;
-  if ((threadIdx.x & 31) == 0) {
+};
+
+TS_DEVICE float weight(float z, float m, float temperature) { return expf((z - m) / temperature); }
+// (key, token) in one word: the greater key first, then the lower token; 0 is nothing
+TS_DEVICE uint64_t race_key(float w, float e, int id) {
+  const float key = w / e;
+  return key >= 0.f ? ((uint64_t)__float_as_uint(key) << 32) | (uint32_t)~(uint32_t)id : 0;
+}
+
+// One pass over logits and random numbers together: statistics and the race among all tokens.
+template <typename T, int NT>
+__device__ void scan_free(Shared<T, NT>& sh, const Slice<T>& sl, const float* __restrict__ noise, float c, Stat& st,
+                          Race& race) {
+  constexpr int VEC = Slice<T>::kVec;
+  constexpr int Q = VEC / 4;  // 16-byte pieces of a vector's random numbers
+  constexpr int R = work_bytes<T, NT>() / (NT * 16 * (1 + Q)) < 6 ? work_bytes<T, NT>() / (NT * 16 * (1 + Q)) : 6;
+  static_assert(R >= 3, "a ring of three");
+  const int tid = threadIdx.x;
+  const T* body = sl.body();
+  const float* nb = noise + sl.head;
+  uint4* ring = reinterpret_cast<uint4*>(sh.work) + tid;
+  const bool wide = (reinterpret_cast<uintptr_t>(nb) & 15) == 0;
+  const int mine = tid < sl.nvec ? (sl.nvec - tid + NT - 1) / NT : 0;
+  auto fetch = [&](int j) {
+    if (j < mine) {
+      uint4* slot = ring + (j % R) * (1 + Q) * NT;
+      const long long i = (long long)(j * NT + tid) * VEC;
+      copy16(slot, body + i);
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        uint4* to = slot + (1 + q) * NT;
+        if (wide) {
+          copy16(to, nb + i + 4 * q);
+        } else {
+#pragma unroll
+          for (int w = 0; w < 4; ++w) copy4(reinterpret_cast<float*>(to) + w, nb + i + 4 * q + w);
+        }
+      }
+    }
+    copy_commit();
+  };
+#pragma unroll
+  for (int j = 0; j < R; ++j) fetch(j);
+  if (tid < sl.head + sl.tail) {
+    const int i = tid < sl.head ? tid : sl.nvec * VEC + tid;
+    const float z = to_f(sl.p[i]), e = noise[i];
+    stat_raise(st.m, st.s, fmaxf(z, -INFINITY), c);
+    st.s += sum_exp<1>(&z, st.m, c);
+    race.take(fmaf(z, c, -lg2(e)), z, e, sl.lo + i);
+  }
+  float least = race.y - Race::margin(race.y);
+  if (race.y == -INFINITY) least = -INFINITY;
+  for (int j = 0; j < mine; ++j) {
+    copy_wait<R - 1>();
+    const uint4* slot = ring + (j % R) * (1 + Q) * NT;
+    float z[VEC], e[VEC], y[VEC];
+    unpack<T>(slot[0], z);
+#pragma unroll
+    for (int q = 0; q < Q; ++q) unpack<float>(slot[(1 + q) * NT], e + 4 * q);
+    fetch(j + R);
+    stat_raise(st.m, st.s, vec_max<VEC>(z), c);
+    st.s += sum_exp<VEC>(z, st.m, c);
+#pragma unroll
+    for (int q = 0; q < VEC; ++q) y[q] = fmaf(z[q], c, -lg2(e[q]));
+    if (vec_max<VEC>(y) > least) {
+#pragma unroll
+      for (int q = 0; q < VEC; ++q) race.take(y[q], z[q], e[q], sl.lo + sl.head + (j * NT + tid) * VEC + q);
+      least = race.y - Race::margin(race.y);
+    }
+  }
+  copy_wait<0>();
+}
+
+struct Bound {  // tokens ranked before (z, id); `none`: all tokens
+  bool none = true;
+  float z = 0.f;
+  int id = 0;
+  TS_DEVICE bool before(float x, int i) const { return none || x > z || (x == z && i < id); }
+};
+
+// Over the tokens before `bound`: how many, their mass, and the race among those with weight min_p at least (none is
+// below zmin). EXACT: by the keys themselves, in `best`.
+template <typename T, int NT, bool EXACT>
+__device__ void scan_before(const Slice<T>& sl, const float* __restrict__ noise, float m, float temperature, float c,
+                            float min_p, float zmin, const Bound& bound, int& count, float& mass, Race& race,
+                            uint64_t& best) {
+  constexpr int VEC = Slice<T>::kVec;
+  const int tid = threadIdx.x;
+  auto one = [&](float z, const float* e, int id) {
+    if (!bound.before(z, id)) return;
+    ++count;
+    mass += rel_exp(z, m, c);
+    if (!(z >= zmin)) return;
+    const float x = *e;
+    if (EXACT) {
+      const float w = weight(z, m, temperature);
+      const uint64_t key = w >= min_p ? race_key(w, x, id) : 0;
+      best = key > best ? key : best;
+    } else {
+      const float y = fmaf(z, c, -lg2(x));
+      if ((race.id < 0 || y > race.y - Race::margin(race.y)) && weight(z, m, temperature) >= min_p)
+        race.take(y, z, x, id);
+    }
+  };
+  if (tid < sl.head + sl.tail) {
+    const int i = tid < sl.head ? tid : sl.nvec * VEC + tid;
+    one(to_f(sl.p[i]), noise + i, sl.lo + i);
+  }
+  const T* body = sl.body();
+  const float* nb = noise + sl.head;
+  constexpr int U = 4;
+  for (int i0 = tid; i0 < sl.nvec; i0 += U * NT) {
+    uint4 raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i0 + u * NT < sl.nvec) raw[u] = load_stream(body + (long long)(i0 + u * NT) * VEC);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * NT;
+      if (i < sl.nvec) {
+        float z[VEC];
+        unpack<T>(raw[u], z);
+        if (bound.none || vec_max<VEC>(z) >= bound.z) {
+#pragma unroll
+          for (int q = 0; q < VEC; ++q) one(z[q], nb + (long long)i * VEC + q, sl.lo + sl.head + i * VEC + q);
+        }
+      }
+    }
+  }
+}
+
+// Cluster-wide sums and bests; all threads of all parts get them. `turn` alternates between calls.
+template <typename T, int NT>
+__device__ void join_keys(Shared<T, NT>& sh, int& turn, int& count, float& mass, uint64_t& best, int& flag) {
+  cg::cluster_group cl = cg::this_cluster();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto fold = [&]() {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      count += __shfl_xor_sync(0xffffffffu, count, o);
+      mass += __shfl_xor_sync(0xffffffffu, mass, o);
+      const uint64_t b = __shfl_xor_sync(0xffffffffu, best, o);
+      best = b > best ? b : best;
+    }
+  };
+  flag = __syncthreads_or(flag);
+  fold();
+  if (lane == 0) {
     sh.wm[warp] = mass;
-    sh.hist[warp] = count;
+    sh.wc[warp] = count;
     sh.wbest[warp] = best;
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    count = 0;
-    mass = 0.f;
-    best = 0;
-    for (int w = 0; w < kWarps; ++w) {
-      mass += sh.wm[w];
-      count += (int)sh.hist[w];
-      best = sh.wbest[w] > best ? sh.wbest[w] : best;
+  if (warp == 0) {
+    mass = lane < NT / 32 ? sh.wm[lane] : 0.f;
+    count = lane < NT / 32 ? sh.wc[lane] : 0;
+    best = lane < NT / 32 ? sh.wbest[lane] : 0;
+    fold();
+    if (lane == 0) {
+      sh.ps[turn] = mass;
+      sh.pcount[turn] = count;
+      sh.pbest[turn] = best;
+      sh.pflag[turn] = flag;
     }
-    sh.ps[turn] = mass;
-    sh.pcount[turn] = count;
-    sh.pbest[turn] = best;
   }
   cl.sync();
   count = 0;
   mass = 0.f;
   best = 0;
+  flag = 0;
   for (int r = 0; r < (int)cl.num_blocks(); ++r) {
-    Shared* o = cl.map_shared_rank(&sh, r);
+    Shared<T, NT>* o = cl.map_shared_rank(&sh, r);
     mass += o->ps[turn];
     count += o->pcount[turn];
     best = o->pbest[turn] > best ? o->pbest[turn] : best;
+    flag |= o->pflag[turn];
   }
+  turn ^= 1;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const T* __restrict__ logits, long long stride,
-                                                          const float* __restrict__ noise, long long nstride, int v,
-                                                          SampleArgs a, int64_t* __restrict__ tokens,
-                                                          float* __restrict__ logprobs) {
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT) sample_kernel(const T* __restrict__ logits, long long stride,
+                                                    const float* __restrict__ noise, long long nstride, int v,
+                                                    SampleArgs a, int64_t* __restrict__ tokens,
+                                                    float* __restrict__ logprobs) {
   extern __shared__ __align__(16) uint8_t raw[];
-  Shared& sh = *reinterpret_cast<Shared*>(raw);
+  Shared<T, NT>& sh = *reinterpret_cast<Shared<T, NT>*>(raw);
   cg::cluster_group cl = cg::this_cluster();
   const int parts = (int)cl.num_blocks(), part = (int)cl.block_rank();
   const int row = blockIdx.x / parts;
@@ -456,16 +705,38 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const T* __restrict__ 
   const bool greedy = !(temperature >= kColdest);
   if (greedy) temperature = 1.f;
   const float c = kLog2e / temperature;
-  const bool by_k = top_k > 0 && top_k < v, by_p = top_p < 1.f;
-  const bool free_row = !greedy && !by_k && !by_p && !(min_p > 0.f);
-  const int k = greedy || free_row ? 1 : by_k && top_k < kMaxTop ? (int)top_k : min(v, kMaxTop);
+  const bool by_k = top_k > 0 && top_k < v, by_p = top_p < 1.f, by_m = min_p > 0.f;
+  const bool race_first = !greedy && !by_p && !by_m && (!by_k || top_k > kMaxTop);  // the list could not be enough
+  const int k = greedy ? 1 : by_k && top_k < kMaxTop ? (int)top_k : min(v, kMaxTop);
   const T* lrow = logits + row * stride;
   const float* nrow = noise ? noise + row * nstride : nullptr;
   Slice<T> sl(lrow, v, part, parts);
+  const float* ns = nrow ? nrow + sl.lo : nullptr;
   Stat st;
-  scan_slice<T>(sh, sl, k, c, st);
-  block_stat(sh, st, c);
-  join_parts(sh, k, c, st);
+  Race race;
+  int turn = 0;
+  if (race_first) {
+    scan_free<T, NT>(sh, sl, ns, c, st, race);
+    block_stat(sh, st, c);
+    if (parts > 1) {  // the row's statistics
+      if (tid == 0) {
+        sh.pm[0] = st.m;
+        sh.ps[0] = st.s;
+      }
+      cl.sync();
+      Stat all;
+      for (int r = 0; r < parts; ++r) {
+        Shared<T, NT>* o = cl.map_shared_rank(&sh, r);
+        stat_merge(all.m, all.s, o->pm[0], o->ps[0], c);
+      }
+      st = all;
+      turn = 1;
+    }
+  } else {
+    scan_slice<T, NT>(sh, sl, k, c, st);
+    block_stat(sh, st, c);
+    join_parts(sh, k, c, st);
+  }
   const float m = st.m, total = st.s;
   auto result = [&](int id) {
     tokens[row] = id;
@@ -473,21 +744,20 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const T* __restrict__ 
   };
   if (!(total > 0.f && total < INFINITY)) {  // the same in every part: no distribution
     if (part == 0 && tid == 0) result(-1);
+    cl.sync();
     return;
   }
-  if (part == 0) {
+  if (part == 0 && !race_first) {
     if (greedy) {
       if (tid == 0) {
         result(rank_id(sh.win[0]));
         sh.verdict = 0;
       }
-    } else if (free_row) {
-      if (tid == 0) sh.verdict = 1;
     } else {
       // the list in rank order: weights, the mass before each, and whether the list holds all that is kept
       const int n = sh.nwin;
       const uint64_t x = tid < n ? sh.win[tid] : 0;
-      const float w = tid < n ? expf((rank_value(x) - m) / temperature) : 0.f;
+      const float w = tid < n ? weight(rank_value(x), m, temperature) : 0.f;
       float incl = w;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -497,16 +767,13 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const T* __restrict__ 
       if ((tid & 31) == 31) sh.wm[tid >> 5] = incl;
       __syncthreads();
       float before = incl - w;
-      for (int q = 0; q < (tid >> 5); ++q) before += sh.wm[q];
+      if (tid < n)
+        for (int q = 0; q < (tid >> 5); ++q) before += sh.wm[q];
       const bool kept = tid < n && (tid == 0 || ((!by_p || before < top_p * total) && w >= min_p));
       const bool open = kept && tid == n - 1 && n < v && !(by_k && top_k <= n);
       const int more = __syncthreads_or(open);
       if (!more) {
-        uint64_t best = 0;
-        if (kept) {
-          const float key = w / nrow[rank_id(x)];
-          if (key >= 0.f) best = ((uint64_t)__float_as_uint(key) << 32) | (uint32_t)x;
-        }
+        uint64_t best = kept ? race_key(w, nrow[rank_id(x)], rank_id(x)) : 0;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
           const uint64_t b = __shfl_xor_sync(0xffffffffu, best, o);
@@ -515,56 +782,91 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const T* __restrict__ 
         if ((tid & 31) == 0) sh.wbest[tid >> 5] = best;
         __syncthreads();
         if (tid == 0) {
-          for (int q = 0; q < kWarps; ++q) best = sh.wbest[q] > best ? sh.wbest[q] : best;
+          for (int q = 0; q < kMaxTop / 32; ++q) best = sh.wbest[q] > best ? sh.wbest[q] : best;
           result(rank_id(best ? best : sh.win[0]));
         }
       }
       if (tid == 0) sh.verdict = more ? 1 : 0;
     }
   }
-  cl.sync();
-  const int verdict = cl.map_shared_rank(&sh, 0)->verdict;
-  if (verdict) {
-    // General search. The best key over all tokens is the sample if it is kept. If it is not, no token ranked after
-    // it is kept either (the filters keep a prefix of the rank order), and the best key of those before it is next.
-    const float* ns = nrow + sl.lo;
-    uint64_t bound = 0;  // 0: all tokens
-    int id = -1;
-    for (int turn = 0;; turn ^= 1) {
-      int count = 0;
-      float mass = 0.f;
-      uint64_t best = 0;
-      scan_keys<T>(sl, ns, m, temperature, min_p, bound, count, mass, best);
-      join_keys(sh, turn, count, mass, best);
-      if (bound != 0) {
-        const bool kept = count == 0 || ((!by_k || count < top_k) && (!by_p || mass < top_p * total));
-        if (kept || best == 0) break;
-      }
-      if (best == 0) break;
-      id = rank_id(best);
-      if (free_row) break;
-      bound = rank_key(to_f(lrow[id]), id);
+  if (!race_first) {
+    cl.sync();
+    if (cl.map_shared_rank(&sh, 0)->verdict == 0) {
+      cl.sync();
+      return;
     }
-    if (part == 0 && tid == 0) result(id >= 0 ? id : rank_id(sh.win[0]));
   }
+  // Search over all tokens. The best key of all is the sample if it is kept. If it is not, no token ranked after it
+  // is kept either (the filters keep a prefix of the rank order), and the best key of those before it is next.
+  // no token below zmin has weight min_p (the weight itself decides about those above)
+  const float zmin = by_m ? m + temperature * (logf(min_p) - 1e-4f) - 1e-5f * fabsf(m) : -INFINITY;
+  Bound bound;
+  int id = -1;
+  bool scanned = race_first;
+  for (;;) {
+    int count = 0, tie = 0;
+    float mass = 0.f;
+    uint64_t best = 0;
+    if (!scanned) {
+      race = Race();
+      scan_before<T, NT, false>(sl, ns, m, temperature, c, min_p, zmin, bound, count, mass, race, best);
+    }
+    scanned = false;
+    // the best of y, and then of the exact keys of the tokens within its margin
+    int c0 = 0, f0 = 0;
+    float m0 = 0.f;
+    uint64_t top = race.id >= 0 ? (uint64_t)order_key(race.y) << 32 : 0;
+    join_keys(sh, turn, c0, m0, top, f0);
+    const float ybest = key_value((uint32_t)(top >> 32));
+    if (race.id >= 0 && race.y >= ybest - Race::margin(ybest)) {
+      best = race_key(weight(race.z, m, temperature), race.e, race.id);
+      tie = race.tie;
+    }
+    join_keys(sh, turn, count, mass, best, tie);
+    if (!bound.none) {
+      const bool kept = count == 0 || ((!by_k || count < top_k) && (!by_p || mass < top_p * total));
+      if (kept) break;
+    }
+    if (tie || (best >> 32) == 0) {  // no single winner by y (or a key that vanished): by exact keys
+      best = 0;
+      int c1 = 0;
+      float m1 = 0.f;
+      scan_before<T, NT, true>(sl, ns, m, temperature, c, min_p, zmin, bound, c1, m1, race, best);
+      c1 = 0;
+      m1 = 0.f;
+      int f1 = 0;
+      join_keys(sh, turn, c1, m1, best, f1);
+    }
+    if (best == 0) break;  // random numbers that are none
+    id = rank_id(best);
+    if (race_first && !by_k) break;
+    bound.none = false;
+    bound.id = id;
+    bound.z = to_f(lrow[id]);
+    if (!race_first && rank_key(bound.z, id) >= cl.map_shared_rank(&sh, 0)->win[k - 1]) break;  // in the list: kept
+  }
+  if (part == 0 && tid == 0) result(id);
   cl.sync();  // no part leaves while another may still read its shared memory
 }
 
-// Parts (CTAs) of a row: one where the rows alone fill the SMs, up to a cluster of eight where there are few.
+// Parts (CTAs) of a row and threads of a part: one part where the rows alone fill the SMs, up to a cluster of eight
+// where there are few, and then with all the threads of an SM.
 int row_parts(int64_t rows, int v, int sms) {
   int parts = 1;
-  while (parts < kMaxParts && rows * parts < 2 * sms && v / (2 * parts) >= kTile) parts *= 2;
+  while (parts < kMaxParts && rows * parts < 4 * sms && v / (2 * parts) >= 4096) parts *= 2;
   return parts;
 }
+bool few_rows(int64_t rows, int parts, int sms) { return rows * parts <= sms && parts == kMaxParts; }
 
-template <typename... KArgs, typename... Args>
+template <typename T, int NT, typename... KArgs, typename... Args>
 cudaError_t launch_rows(const VocabLaunch& l, void (*kernel)(KArgs...), int64_t rows, int parts, Args&&... args) {
-  const cudaError_t e = l.set_smem((const void*)kernel, (int)sizeof(Shared));
+  const int bytes = (int)sizeof(Shared<T, NT>);
+  const cudaError_t e = l.set_smem((const void*)kernel, bytes);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * parts));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = sizeof(Shared);
+  cfg.blockDim = dim3(NT);
+  cfg.dynamicSmemBytes = bytes;
   cfg.stream = l.stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -578,14 +880,22 @@ cudaError_t launch_rows(const VocabLaunch& l, void (*kernel)(KArgs...), int64_t 
 
 template <typename T>
 cudaError_t topk_of(const VocabLaunch& l, const VocabRows& x, int k, float temperature, int64_t* ids, float* lp) {
-  return launch_rows(l, topk_kernel<T>, x.n, row_parts(x.n, x.v, l.sms), (const T*)x.logits, x.stride, x.v, k,
-                     temperature, ids, lp);
+  const int parts = row_parts(x.n, x.v, l.sms);
+  if (few_rows(x.n, parts, l.sms))
+    return launch_rows<T, 1024>(l, topk_kernel<T, 1024>, x.n, parts, (const T*)x.logits, x.stride, x.v, k, temperature,
+                                ids, lp);
+  return launch_rows<T, 256>(l, topk_kernel<T, 256>, x.n, parts, (const T*)x.logits, x.stride, x.v, k, temperature, ids,
+                             lp);
 }
 template <typename T>
 cudaError_t sample_of(const VocabLaunch& l, const VocabRows& x, const float* noise, long long nstride,
                       const SampleArgs& a, int64_t* tokens, float* lp) {
-  return launch_rows(l, sample_kernel<T>, x.n, row_parts(x.n, x.v, l.sms), (const T*)x.logits, x.stride, noise, nstride,
-                     x.v, a, tokens, lp);
+  const int parts = row_parts(x.n, x.v, l.sms);
+  if (few_rows(x.n, parts, l.sms))
+    return launch_rows<T, 1024>(l, sample_kernel<T, 1024>, x.n, parts, (const T*)x.logits, x.stride, noise, nstride,
+                                x.v, a, tokens, lp);
+  return launch_rows<T, 256>(l, sample_kernel<T, 256>, x.n, parts, (const T*)x.logits, x.stride, noise, nstride, x.v, a,
+                             tokens, lp);
 }
 
 }  // namespace
