@@ -27,14 +27,12 @@ using namespace vocab;
 constexpr int kMaxTop = 256;
 constexpr int kMaxParts = 8;
 constexpr int kLimit = 768;                  // entries at which the buffer is cut back, at most
-constexpr int kStep = 4;                     // vectors of a thread between two looks at the buffer
-constexpr int kRing = 6;                     // vectors of a thread in flight
+constexpr int kRing = 8;                     // vectors of a thread in its ring
 constexpr float kColdest = 1e-6f;            // colder rows are greedy
 
-// The buffer holds the limit and one vector of each thread (the step of the careful path), and the parts' lists.
+// The buffer holds the limit and four elements of each thread (the step of the careful path), and the parts' lists.
 template <typename T, int NT> constexpr int buf_cap() {
-  return kLimit + NT * Slice<T>::kVec + 32 > kMaxParts * kMaxTop ? kLimit + NT * Slice<T>::kVec + 32
-                                                                 : kMaxParts * kMaxTop;
+  return kLimit + NT * 4 + 32 > kMaxParts * kMaxTop ? kLimit + NT * 4 + 32 : kMaxParts * kMaxTop;
 }
 template <typename T, int NT> constexpr int work_bytes() { return buf_cap<T, NT>() * 8 + kRing * NT * 16; }
 
@@ -45,13 +43,12 @@ struct Shared {
   uint64_t pbest[2];  // this CTA's partial results, read by its cluster (two sets, used in turn)
   float wm[NT / 32], ws[NT / 32];
   int wc[NT / 32];
-  uint32_t group[kMaxTop], hist[256];
+  uint32_t group[kMaxTop], hist[2][256], sel_min, sel_max;
   float pm[2], ps[2];
   int pcount[2], pflag[2];
   int count;          // entries appended to the buffer (may pass its capacity: then they were not stored)
   int nwin;           // entries in win
   int sel_need, sel_bin, sel_done;
-  int verdict;        // of part 0: 0 done, else the search over all tokens follows
   __align__(16) uint8_t work[work_bytes<T, NT>()];
 
   __device__ uint64_t* buf() { return reinterpret_cast<uint64_t*>(work); }
@@ -69,31 +66,108 @@ TS_DEVICE void copy4(void* dst, const void* src) {
 TS_DEVICE void copy_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
 template <int N> TS_DEVICE void copy_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
 
+// This thread's vectors of a slice through its private ring, a step of 16 elements (four vectors, or two of 16-bit
+// types) at a time: vectors t·kVecs + q, q < kVecs, of every thread. Places past the end read as -inf.
+template <typename T, int NT>
+struct Steps {
+  static constexpr int VEC = Slice<T>::kVec;
+  static constexpr int kVecs = 16 / VEC;
+  static constexpr int kAhead = kRing / kVecs;  // steps in flight
+  const T* src;
+  uint4* ring;
+  int nvec, count;
+
+  __device__ Steps(const Slice<T>& sl, void* work)
+      : src(sl.body() + threadIdx.x * VEC), ring(reinterpret_cast<uint4*>(work) + threadIdx.x), nvec(sl.nvec),
+        count((sl.nvec + kVecs * NT - 1) / (kVecs * NT)) {
+#pragma unroll
+    for (int t = 0; t < kAhead; ++t) fetch(t);
+  }
+  TS_DEVICE bool has(int t, int q) const { return (t * kVecs + q) * NT + (int)threadIdx.x < nvec; }
+  TS_DEVICE void fetch(int t) {
+    uint4* to = ring + (t % kAhead) * (kVecs * NT);
+    const T* from = src + (long long)t * (kVecs * NT * VEC);
+    if ((t + 1) * kVecs * NT <= nvec) {
+#pragma unroll
+      for (int q = 0; q < kVecs; ++q) copy16(to + q * NT, from + q * NT * VEC);
+    } else {
+#pragma unroll
+      for (int q = 0; q < kVecs; ++q)
+        if (has(t, q)) copy16(to + q * NT, from + q * NT * VEC);
+    }
+    copy_commit();
+  }
+  // step t (in order), and the fetch of the one that takes its place
+  TS_DEVICE void read(int t, float (&z)[kVecs][VEC]) {
+    copy_wait<kAhead - 1>();
+    const uint4* at = ring + (t % kAhead) * (kVecs * NT);
+#pragma unroll
+    for (int q = 0; q < kVecs; ++q) unpack<T>(at[q * NT], z[q]);
+    if ((t + 1) * kVecs * NT > nvec) {
+#pragma unroll
+      for (int q = 0; q < kVecs; ++q) {
+        if (!has(t, q)) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) z[q][e] = -INFINITY;
+        }
+      }
+    }
+    fetch(t + kAhead);
+  }
+};
+
 struct Stat {
   float m = -INFINITY, s = 0.f;
 };
 
 // Moves the `k` largest of buf[0, n) to sh.win (in no order); `least` is a lower bound of them above which no other
-// entry is. n >= k. All threads call it after a barrier that follows the last write to buf.
+// entry is. n >= k. All threads call it after a barrier that follows the last write to buf. Digits of eight bits from
+// the first bit in which the entries' logits differ.
 template <typename T, int NT>
-__device__ void select_k(Shared<T, NT>& sh, int n, int k, uint64_t& least) {
-  uint64_t prefix = 0;  // decided digits of the k-th largest
-  int need = k;
+__device__ __noinline__ void select_k(Shared<T, NT>& sh, int n, int k, uint64_t& least) {
   const int tid = threadIdx.x;
   const uint64_t* buf = sh.buf();
-  for (int shift = 56;; shift -= 8) {
-    if (tid < 256) sh.hist[tid] = 0;
-    __syncthreads();
+  if (tid < 256) {
+    sh.hist[0][tid] = 0;
+    sh.hist[1][tid] = 0;
+  }
+  if (tid == 0) {
+    sh.sel_min = 0xffffffffu;
+    sh.sel_max = 0;
+    sh.nwin = 0;
+  }
+  __syncthreads();
+  uint32_t mn = 0xffffffffu, mx = 0;
+  for (int i = tid; i < n; i += NT) {
+    const uint32_t x = (uint32_t)(buf[i] >> 32);
+    mn = min(mn, x);
+    mx = max(mx, x);
+  }
+  mn = __reduce_min_sync(0xffffffffu, mn);
+  mx = __reduce_max_sync(0xffffffffu, mx);
+  if ((tid & 31) == 0 && mn <= mx) {
+    atomicMin(&sh.sel_min, mn);
+    atomicMax(&sh.sel_max, mx);
+  }
+  __syncthreads();
+  mn = sh.sel_min;
+  mx = sh.sel_max;
+  int prev = mn == mx ? 32 : 64 - __clz(mn ^ mx);  // the bits from here on are decided
+  uint64_t prefix = prev == 64 ? 0 : ((uint64_t)mx << 32) >> prev << prev;
+  int need = k;
+  for (int turn = 0;; turn ^= 1) {
+    const int width = min(8, prev), shift = prev - width;
+    const uint32_t mask = (1u << width) - 1;
     for (int i = tid; i < n; i += NT) {
       const uint64_t x = buf[i];
-      if (shift == 56 || (x >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&sh.hist[(x >> shift) & 255], 1u);
+      if (prev == 64 || (x >> prev) == (prefix >> prev)) atomicAdd(&sh.hist[turn][(uint32_t)(x >> shift) & mask], 1u);
     }
     __syncthreads();
     if (tid < 32) {
       // lane l sums the 8 bins from 255 - 8l downwards
       uint32_t h[8], sum = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sum += h[j] = sh.hist[255 - 8 * tid - j];
+      for (int j = 0; j < 8; ++j) sum += h[j] = sh.hist[turn][255 - 8 * tid - j];
       uint32_t incl = sum;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -113,15 +187,17 @@ __device__ void select_k(Shared<T, NT>& sh, int n, int k, uint64_t& least) {
           above += h[j];
         }
       }
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sh.hist[turn][255 - 8 * tid - j] = 0;
     }
     __syncthreads();
     prefix |= (uint64_t)sh.sel_bin << shift;
     need = sh.sel_need;
+    prev = shift;
     if (sh.sel_done || shift == 0) break;  // every entry of the bin belongs to the k
   }
   least = prefix;
-  if (tid == 0) sh.nwin = 0;
-  __syncthreads();
   for (int i = tid; i < n; i += NT) {
     const uint64_t x = buf[i];
     if (x >= prefix) {
@@ -187,57 +263,47 @@ TS_DEVICE float vec_max(const float* z) {
 // Leaves the slice's k largest (all of it where it is shorter) in sh.win, sh.nwin entries of which some may be
 // smaller, in no order; and this thread's part of the statistics.
 template <typename T, int NT>
-__device__ void scan_slice(Shared<T, NT>& sh, const Slice<T>& sl, int k, float c, Stat& st) {
-  constexpr int VEC = Slice<T>::kVec;
+__device__ __noinline__ Stat scan_slice(Shared<T, NT>& sh, const Slice<T> sl, int k, float c) {
+  using S = Steps<T, NT>;
+  constexpr int VEC = S::VEC, Q = S::kVecs;
   const int tid = threadIdx.x;
-  const T* body = sl.body();
   uint64_t* buf = sh.buf();
-  uint4* ring = sh.ring() + tid;
   const int limit = min(kLimit, max(4 * k, 128));
+  Stat st;
   if (tid == 0) sh.count = 0;
+  S steps(sl, sh.ring());
+  __syncthreads();
 
+  bool slow = true;     // look at the order of every element: no threshold yet, or one below -inf
   bool open = true;     // no threshold yet: every element is appended
   uint32_t tkey = 0;    // else elements whose order is above it (strictly: at equal logits the lower token is in)
-  float tval = 0.f;     // the same as a logit, for a first look at a vector's maximum
-  bool low = false;     // the threshold is below -inf: look at every vector
+  float tval = 0.f;     // the same as a logit
+  int seen = 0;         // entries of the buffer as far as this thread knows
   auto set_threshold = [&](uint32_t key) {
     open = false;
     tkey = key;
-    low = key < 0x007fffffu;  // -inf's order
+    slow = key < 0x007fffffu;  // -inf's order
     // -0 has the order of +0: below that, the next logit down
     tval = key == 0x7fffffffu ? __uint_as_float(0x80000001u) : key_value(key);
   };
   auto push = [&](float z, int id) {
-    if (open || order_key(z) > tkey) {
+    if (slow ? open || order_key(z) > tkey : z > tval) {
       const int at = atomicAdd(&sh.count, 1);
+      seen = at + 1;
       if (at < buf_cap<T, NT>()) buf[at] = rank_key(z, id);
     }
   };
-  auto push_vec = [&](const float* z, int i) {
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) push(z[e], sl.lo + sl.head + i * VEC + e);
-  };
+  auto id_of = [&](int t, int q) { return sl.lo + sl.head + ((t * Q + q) * NT + tid) * VEC; };
   auto cut = [&](int n) {  // all threads; the buffer is complete
     if (n < k) return;
     uint64_t least;
     select_k<T, NT>(sh, n, k, least);
     for (int i = tid; i < k; i += NT) buf[i] = sh.win[i];
     if (tid == 0) sh.count = k;
+    seen = k;
     set_threshold((uint32_t)(least >> 32));
     __syncthreads();
   };
-
-  const int nvec = sl.nvec;
-  const int mine = tid < nvec ? (nvec - tid + NT - 1) / NT : 0;  // vectors of this thread
-  const int most = (nvec + NT - 1) / NT;                         // of the first thread
-  auto fetch = [&](int j) {
-    if (j < mine) copy16(&ring[(j % kRing) * NT], body + (long long)(j * NT + tid) * VEC);
-    copy_commit();
-  };
-#pragma unroll
-  for (int j = 0; j < kRing; ++j) fetch(j);
-  __syncthreads();
-
   auto edge = [&](int first, int cnt) {  // the unaligned ends: less than a vector
     if (tid < cnt) {
       const int i = first + tid;
@@ -249,103 +315,82 @@ __device__ void scan_slice(Shared<T, NT>& sh, const Slice<T>& sl, int k, float c
   };
   edge(0, sl.head);
 
-  // the first vectors stay in registers until there is a threshold for them
-  int j = 0;
-  if (most > 0) {
-    constexpr int F = VEC == 4 ? 4 : 2;
-    float z[F][VEC];
-    float zmax = -INFINITY;
-    copy_wait<kRing - F>();
+  int from = 0, t0 = 0;  // `from` entries were in the buffer before step t0
+  bool head_too = true;
+  for (int t = 0;; ++t) {
+    // the threads look whether the buffer has filled
+    if (__syncthreads_or(seen > limit)) {
+      const int n = sh.count;
+      __syncthreads();
+      if (n > buf_cap<T, NT>()) {
+        // more came than fits (very many equal logits, or rising ones): again from t0, four elements of each thread
+        // at a time
+        if (tid == 0) sh.count = from;
+        __syncthreads();
+        if (head_too && tid < sl.head) push(to_f(sl.p[tid]), sl.lo + tid);
+        for (int v = t0 * Q; v < t * Q && v * NT < sl.nvec; ++v) {
+          float z[VEC];
+          const int i = v * NT + tid;
+          if (i < sl.nvec) unpack<T>(load_stream(sl.body() + (long long)i * VEC), z);
 #pragma unroll
-    for (int q = 0; q < F; ++q) {
-      if (q < mine) {
-        unpack<T>(ring[q * NT], z[q]);
-        zmax = fmaxf(zmax, vec_max<VEC>(z[q]));
+          for (int h = 0; h < VEC; h += 4) {
+            if (i < sl.nvec) {
+#pragma unroll
+              for (int e = h; e < h + 4; ++e) push(z[e], sl.lo + sl.head + i * VEC + e);
+            }
+            __syncthreads();
+            const int now = sh.count;
+            __syncthreads();
+            if (now > limit) cut(now);
+          }
+        }
+        __syncthreads();
+        from = sh.count;
+        __syncthreads();
+      } else {
+        cut(n);
+        from = k;
       }
+      seen = from;
+      t0 = t;
+      head_too = false;
+    }
+    if (t >= steps.count) break;
+    float z[Q][VEC], top[Q];
+    steps.read(t, z);
+    float zmax = -INFINITY;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      top[q] = vec_max<VEC>(z[q]);
+      zmax = fmaxf(zmax, top[q]);
     }
     stat_raise(st.m, st.s, zmax, c);
-    uint32_t best = 0;
-    if (zmax > -INFINITY) best = order_key(zmax);
+    st.s += sum_exp<16>(&z[0][0], st.m, c);
+    if (t == 0) {
+      // the first threshold, from the threads' largest elements so far
+      uint32_t best = 0;
+      if (zmax > -INFINITY) {
+        best = order_key(zmax);
+      } else {  // nothing but -inf and NaN, which zmax leaves out
 #pragma unroll
-    for (int q = 0; q < F; ++q) {
-      if (q < mine) {
-        st.s += sum_exp<VEC>(z[q], st.m, c);
-        if (!(zmax > -INFINITY)) {  // nothing but -inf and NaN, which zmax leaves out
+        for (int q = 0; q < Q; ++q) {
+          if (steps.has(t, q)) {
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) best = max(best, order_key(z[q][e]));
+            for (int e = 0; e < VEC; ++e) best = max(best, order_key(z[q][e]));
+          }
         }
       }
+      const uint32_t key = group_threshold<T, NT>(sh, best, k);
+      if (key > 0) set_threshold(key - 1);
     }
+    if (slow || zmax > tval) {
 #pragma unroll
-    for (int q = 0; q < F; ++q) fetch(kRing + q);
-    const uint32_t t0 = group_threshold<T, NT>(sh, best, k);
-    if (t0 > 0) set_threshold(t0 - 1);
+      for (int q = 0; q < Q; ++q) {
+        if (slow ? steps.has(t, q) : top[q] > tval) {
 #pragma unroll
-    for (int q = 0; q < F; ++q)
-      if (q < mine && (open || low || vec_max<VEC>(z[q]) > tval)) push_vec(z[q], q * NT + tid);
-    j = F;
-    __syncthreads();
-    const int n = sh.count;
-    __syncthreads();
-    if (n > buf_cap<T, NT>()) {
-      // more than fit (very many equal logits): once more, a vector of each thread at a time
-      if (tid == 0) sh.count = 0;
-      __syncthreads();
-      if (tid < sl.head) push(to_f(sl.p[tid]), sl.lo + tid);
-      for (int q = 0; q < F; ++q) {
-        if (q < mine) {
-          float x[VEC];
-          unpack<T>(load_stream(body + (long long)(q * NT + tid) * VEC), x);
-          push_vec(x, q * NT + tid);
+          for (int e = 0; e < VEC; ++e) push(z[q][e], id_of(t, q) + e);
         }
-        __syncthreads();
-        const int now = sh.count;
-        __syncthreads();
-        if (now > limit) cut(now);
       }
-    } else if (n > limit) {
-      cut(n);
-    }
-  }
-  while (j < most) {
-    const int from = sh.count;  // uniform: a barrier has passed since the last append
-    __syncthreads();
-    const int j0 = j;
-#pragma unroll
-    for (int q = 0; q < kStep; ++q, ++j) {
-      copy_wait<kRing - 1>();
-      if (j < mine) {
-        float z[VEC];
-        unpack<T>(ring[(j % kRing) * NT], z);
-        fetch(j + kRing);
-        const float zmax = vec_max<VEC>(z);
-        stat_raise(st.m, st.s, zmax, c);
-        st.s += sum_exp<VEC>(z, st.m, c);
-        if (open || low || zmax > tval) push_vec(z, j * NT + tid);
-      } else {
-        copy_commit();
-      }
-    }
-    __syncthreads();
-    const int n = sh.count;
-    __syncthreads();
-    if (n > buf_cap<T, NT>()) {
-      // these vectors brought more than fits: once more from `from`, one vector of each thread at a time
-      if (tid == 0) sh.count = from;
-      __syncthreads();
-      for (int q = j0; q < j0 + kStep && q < most; ++q) {
-        if (q < mine) {
-          float z[VEC];
-          unpack<T>(load_stream(body + (long long)(q * NT + tid) * VEC), z);
-          push_vec(z, q * NT + tid);
-        }
-        __syncthreads();
-        const int now = sh.count;
-        __syncthreads();
-        if (now > limit) cut(now);
-      }
-    } else if (n > limit) {
-      cut(n);
     }
   }
   copy_wait<0>();
@@ -360,6 +405,7 @@ __device__ void scan_slice(Shared<T, NT>& sh, const Slice<T>& sl, int k, float c
     if (tid == 0) sh.nwin = n;
     __syncthreads();
   }
+  return st;
 }
 
 // Block-wide (m, s); all threads get it.
@@ -462,8 +508,7 @@ __global__ void __launch_bounds__(NT) topk_kernel(const T* __restrict__ logits, 
   const int row = blockIdx.x / parts;
   const float c = kLog2e / temperature;
   Slice<T> sl(logits + row * stride, v, (int)cl.block_rank(), parts);
-  Stat st;
-  scan_slice<T, NT>(sh, sl, k, c, st);
+  Stat st = scan_slice<T, NT>(sh, sl, k, c);
   block_stat(sh, st, c);
   join_parts(sh, k, c, st);
   if (cl.block_rank() == 0) {
@@ -518,8 +563,10 @@ TS_DEVICE uint64_t race_key(float w, float e, int id) {
 
 // One pass over logits and random numbers together: statistics and the race among all tokens.
 template <typename T, int NT>
-__device__ void scan_free(Shared<T, NT>& sh, const Slice<T>& sl, const float* __restrict__ noise, float c, Stat& st,
-                          Race& race) {
+__device__ __noinline__ void scan_free(Shared<T, NT>& sh, const Slice<T> sl, const float* __restrict__ noise, float c,
+                                       Stat& st_out, Race& race_out) {
+  Stat st;
+  Race race;
   constexpr int VEC = Slice<T>::kVec;
   constexpr int Q = VEC / 4;  // 16-byte pieces of a vector's random numbers
   constexpr int R = work_bytes<T, NT>() / (NT * 16 * (1 + Q)) < 6 ? work_bytes<T, NT>() / (NT * 16 * (1 + Q)) : 6;
@@ -578,6 +625,8 @@ __device__ void scan_free(Shared<T, NT>& sh, const Slice<T>& sl, const float* __
     }
   }
   copy_wait<0>();
+  st_out = st;
+  race_out = race;
 }
 
 struct Bound {  // tokens ranked before (z, id); `none`: all tokens
@@ -587,55 +636,146 @@ struct Bound {  // tokens ranked before (z, id); `none`: all tokens
   TS_DEVICE bool before(float x, int i) const { return none || x > z || (x == z && i < id); }
 };
 
-// Over the tokens before `bound`: how many, their mass, and the race among those with weight min_p at least (none is
-// below zmin). EXACT: by the keys themselves, in `best`.
-template <typename T, int NT, bool EXACT>
-__device__ void scan_before(const Slice<T>& sl, const float* __restrict__ noise, float m, float temperature, float c,
-                            float min_p, float zmin, const Bound& bound, int& count, float& mass, Race& race,
-                            uint64_t& best) {
-  constexpr int VEC = Slice<T>::kVec;
+// How many tokens rank before `bound`, and their mass.
+template <typename T, int NT>
+__device__ __noinline__ void count_before(Shared<T, NT>& sh, const Slice<T> sl, float m, float c, const Bound& bound,
+                                          int& count, float& mass) {
+  constexpr int VEC = Slice<T>::kVec, Q = 16 / VEC;
   const int tid = threadIdx.x;
-  auto one = [&](float z, const float* e, int id) {
-    if (!bound.before(z, id)) return;
-    ++count;
-    mass += rel_exp(z, m, c);
-    if (!(z >= zmin)) return;
-    const float x = *e;
-    if (EXACT) {
-      const float w = weight(z, m, temperature);
-      const uint64_t key = w >= min_p ? race_key(w, x, id) : 0;
-      best = key > best ? key : best;
-    } else {
-      const float y = fmaf(z, c, -lg2(x));
-      if ((race.id < 0 || y > race.y - Race::margin(race.y)) && weight(z, m, temperature) >= min_p)
-        race.take(y, z, x, id);
+  Steps<T, NT> steps(sl, sh.ring());
+  const float bz = bound.z;
+  const int bi = bound.id;
+  const bool plain = m > -1e30f;  // as in sum_exp
+  const float r = m * c;
+  int n = 0;
+  float s0 = 0.f, s1 = 0.f;
+  if (tid < sl.head + sl.tail) {
+    const int i = tid < sl.head ? tid : sl.nvec * VEC + tid;
+    const float a = to_f(sl.p[i]);
+    if (bound.before(a, sl.lo + i)) {
+      ++n;
+      s0 += rel_exp(a, m, c);
+    }
+  }
+  for (int t = 0; t < steps.count; ++t) {
+    float z[Q][VEC];
+    steps.read(t, z);
+    bool even = false;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+#pragma unroll
+      for (int e = 0; e < VEC; e += 2) {
+        const float a = z[q][e], b = z[q][e + 1];
+        const float ea = plain ? ex2(fmaf(a, c, -r)) : rel_exp(a, m, c);
+        const float eb = plain ? ex2(fmaf(b, c, -r)) : rel_exp(b, m, c);
+        n += (a > bz) + (b > bz);
+        s0 += a > bz ? ea : 0.f;
+        s1 += b > bz ? eb : 0.f;
+        even |= a == bz || b == bz;
+      }
+    }
+    if (even) {
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        const int id = sl.lo + sl.head + ((t * Q + q) * NT + tid) * VEC;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          if (z[q][e] == bz && id + e < bi && steps.has(t, q)) {
+            ++n;
+            s0 += rel_exp(bz, m, c);
+          }
+        }
+      }
+    }
+  }
+  copy_wait<0>();
+  count = n;
+  mass = s0 + s1;
+}
+
+// The race among the tokens before `bound` with weight min_p at least (none is below zmin). Random numbers are read
+// where a vector holds such a token.
+template <typename T, int NT>
+__device__ __noinline__ void race_before(const Slice<T> sl, const float* __restrict__ noise, float m,
+                                         float temperature, float c, float min_p, float zmin, const Bound& bound,
+                                         Race& race) {
+  constexpr int VEC = Slice<T>::kVec;
+  constexpr int U = VEC == 4 ? 4 : 2;
+  const int tid = threadIdx.x;
+  const float bz = bound.z;
+  const int bi = bound.id;
+  const float floor = fmaxf(bz, zmin);
+  const bool all = !(min_p > 0.f);
+  Race r;
+  float least = -INFINITY;
+  auto one = [&](float z, float e, int id) {
+    const float y = fmaf(z, c, -lg2(e));
+    if (y > least && (z > bz || (z == bz && id < bi)) && z >= zmin &&
+        (all || weight(z, m, temperature) >= min_p || z == m)) {
+      r.take(y, z, e, id);
+      least = r.y - Race::margin(r.y);
     }
   };
   if (tid < sl.head + sl.tail) {
     const int i = tid < sl.head ? tid : sl.nvec * VEC + tid;
-    one(to_f(sl.p[i]), noise + i, sl.lo + i);
+    one(to_f(sl.p[i]), noise[i], sl.lo + i);
   }
   const T* body = sl.body();
   const float* nb = noise + sl.head;
-  constexpr int U = 4;
+  const bool wide = (reinterpret_cast<uintptr_t>(nb) & 15) == 0;
   for (int i0 = tid; i0 < sl.nvec; i0 += U * NT) {
     uint4 raw[U];
+    float e[U][VEC];
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (i0 + u * NT < sl.nvec) raw[u] = load_stream(body + (long long)(i0 + u * NT) * VEC);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * NT;
-      if (i < sl.nvec) {
-        float z[VEC];
-        unpack<T>(raw[u], z);
-        if (bound.none || vec_max<VEC>(z) >= bound.z) {
+      const long long i = (long long)(i0 + u * NT) * VEC;
+      float z[VEC];
+      unpack<T>(raw[u], z);
+      if (i0 + u * NT < sl.nvec && vec_max<VEC>(z) >= floor) {
+        if (wide) {
 #pragma unroll
-          for (int q = 0; q < VEC; ++q) one(z[q], nb + (long long)i * VEC + q, sl.lo + sl.head + i * VEC + q);
+          for (int q = 0; q < VEC; q += 4) unpack<float>(load_stream(nb + i + q), e[u] + q);
+        } else {
+#pragma unroll
+          for (int q = 0; q < VEC; ++q) e[u][q] = nb[i + q];
         }
+      } else {
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) e[u][q] = INFINITY;  // (never wins)
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = sl.head + (i0 + u * NT) * VEC;
+      float z[VEC];
+      unpack<T>(raw[u], z);
+#pragma unroll
+      for (int q = 0; q < VEC; ++q) one(z[q], e[u][q], sl.lo + i + q);
+    }
+  }
+  race = r;
+}
+
+// The best exact key of those tokens (of all tokens, where there is no bound).
+template <typename T, int NT>
+__device__ __noinline__ uint64_t scan_exact(const Slice<T> sl, const float* __restrict__ noise, float m,
+                                            float temperature, float min_p, float zmin, const Bound& bound) {
+  uint64_t best = 0;
+  for (int i = threadIdx.x; i < sl.n; i += NT) {
+    const float z = to_f(sl.p[i]);
+    const int id = sl.lo + i;
+    if (bound.none || (bound.before(z, id) && z >= zmin)) {
+      const float w = weight(z, m, temperature);
+      if (w >= min_p || z == m) {
+        const uint64_t key = race_key(w, noise[i], id);
+        best = key > best ? key : best;
       }
     }
   }
+  return best;
 }
 
 // Cluster-wide sums and bests; all threads of all parts get them. `turn` alternates between calls.
@@ -687,8 +827,22 @@ __device__ void join_keys(Shared<T, NT>& sh, int& turn, int& count, float& mass,
   turn ^= 1;
 }
 
+// The first-ranked token.
 template <typename T, int NT>
-__global__ void __launch_bounds__(NT) sample_kernel(const T* __restrict__ logits, long long stride,
+__device__ __noinline__ int first_rank(Shared<T, NT>& sh, const Slice<T>& sl, int& turn) {
+  uint64_t best = 0;
+  for (int i = threadIdx.x; i < sl.n; i += NT) {
+    const uint64_t x = rank_key(to_f(sl.p[i]), sl.lo + i);
+    best = x > best ? x : best;
+  }
+  int count = 0, flag = 0;
+  float mass = 0.f;
+  join_keys(sh, turn, count, mass, best, flag);
+  return rank_id(best);
+}
+
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) sample_kernel(const T* __restrict__ logits, long long stride,
                                                     const float* __restrict__ noise, long long nstride, int v,
                                                     SampleArgs a, int64_t* __restrict__ tokens,
                                                     float* __restrict__ logprobs) {
@@ -706,8 +860,8 @@ __global__ void __launch_bounds__(NT) sample_kernel(const T* __restrict__ logits
   if (greedy) temperature = 1.f;
   const float c = kLog2e / temperature;
   const bool by_k = top_k > 0 && top_k < v, by_p = top_p < 1.f, by_m = min_p > 0.f;
-  const bool race_first = !greedy && !by_p && !by_m && (!by_k || top_k > kMaxTop);  // the list could not be enough
-  const int k = greedy ? 1 : by_k && top_k < kMaxTop ? (int)top_k : min(v, kMaxTop);
+  const bool race_first = !greedy && !(by_k && top_k <= kMaxTop);
+  const int k = greedy ? 1 : (int)top_k;  // of the list
   const T* lrow = logits + row * stride;
   const float* nrow = noise ? noise + row * nstride : nullptr;
   Slice<T> sl(lrow, v, part, parts);
@@ -733,7 +887,7 @@ __global__ void __launch_bounds__(NT) sample_kernel(const T* __restrict__ logits
       turn = 1;
     }
   } else {
-    scan_slice<T, NT>(sh, sl, k, c, st);
+    st = scan_slice<T, NT>(sh, sl, k, c);
     block_stat(sh, st, c);
     join_parts(sh, k, c, st);
   }
@@ -749,12 +903,9 @@ __global__ void __launch_bounds__(NT) sample_kernel(const T* __restrict__ logits
   }
   if (part == 0 && !race_first) {
     if (greedy) {
-      if (tid == 0) {
-        result(rank_id(sh.win[0]));
-        sh.verdict = 0;
-      }
+      if (tid == 0) result(rank_id(sh.win[0]));
     } else {
-      // the list in rank order: weights, the mass before each, and whether the list holds all that is kept
+      // the list in rank order: weights, the mass before each, and the race among the kept
       const int n = sh.nwin;
       const uint64_t x = tid < n ? sh.win[tid] : 0;
       const float w = tid < n ? weight(rank_value(x), m, temperature) : 0.f;
@@ -770,80 +921,68 @@ __global__ void __launch_bounds__(NT) sample_kernel(const T* __restrict__ logits
       if (tid < n)
         for (int q = 0; q < (tid >> 5); ++q) before += sh.wm[q];
       const bool kept = tid < n && (tid == 0 || ((!by_p || before < top_p * total) && w >= min_p));
-      const bool open = kept && tid == n - 1 && n < v && !(by_k && top_k <= n);
-      const int more = __syncthreads_or(open);
-      if (!more) {
-        uint64_t best = kept ? race_key(w, nrow[rank_id(x)], rank_id(x)) : 0;
+      uint64_t best = kept ? race_key(w, nrow[rank_id(x)], rank_id(x)) : 0;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-          const uint64_t b = __shfl_xor_sync(0xffffffffu, best, o);
-          best = b > best ? b : best;
-        }
-        if ((tid & 31) == 0) sh.wbest[tid >> 5] = best;
-        __syncthreads();
-        if (tid == 0) {
-          for (int q = 0; q < kMaxTop / 32; ++q) best = sh.wbest[q] > best ? sh.wbest[q] : best;
-          result(rank_id(best ? best : sh.win[0]));
-        }
+      for (int o = 16; o > 0; o >>= 1) {
+        const uint64_t b = __shfl_xor_sync(0xffffffffu, best, o);
+        best = b > best ? b : best;
       }
-      if (tid == 0) sh.verdict = more ? 1 : 0;
+      if ((tid & 31) == 0) sh.wbest[tid >> 5] = best;
+      __syncthreads();
+      if (tid == 0) {
+        for (int q = 0; q < kMaxTop / 32; ++q) best = sh.wbest[q] > best ? sh.wbest[q] : best;
+        result(rank_id(best ? best : sh.win[0]));
+      }
     }
   }
   if (!race_first) {
-    cl.sync();
-    if (cl.map_shared_rank(&sh, 0)->verdict == 0) {
-      cl.sync();
-      return;
-    }
+    cl.sync();  // no part leaves while another may still read its shared memory
+    return;
   }
-  // Search over all tokens. The best key of all is the sample if it is kept. If it is not, no token ranked after it
-  // is kept either (the filters keep a prefix of the rank order), and the best key of those before it is next.
-  // no token below zmin has weight min_p (the weight itself decides about those above)
+  // The best key of all tokens is the sample if it is kept: two passes over the logits alone where there is a top-k
+  // or top-p (the race, and what ranks before the winner), else one. If it is not kept, no token ranked after it is
+  // (the filters keep a prefix of the rank order), and the best key of those before it is next.
+  // No token below zmin has weight min_p (the weight itself decides about those above).
   const float zmin = by_m ? m + temperature * (logf(min_p) - 1e-4f) - 1e-5f * fabsf(m) : -INFINITY;
   Bound bound;
   int id = -1;
-  bool scanned = race_first;
   for (;;) {
-    int count = 0, tie = 0;
-    float mass = 0.f;
-    uint64_t best = 0;
-    if (!scanned) {
-      race = Race();
-      scan_before<T, NT, false>(sl, ns, m, temperature, c, min_p, zmin, bound, count, mass, race, best);
-    }
-    scanned = false;
     // the best of y, and then of the exact keys of the tokens within its margin
-    int c0 = 0, f0 = 0;
+    int c0 = 0, f0 = 0, tie = 0;
     float m0 = 0.f;
-    uint64_t top = race.id >= 0 ? (uint64_t)order_key(race.y) << 32 : 0;
-    join_keys(sh, turn, c0, m0, top, f0);
-    const float ybest = key_value((uint32_t)(top >> 32));
+    uint64_t best = race.id >= 0 ? (uint64_t)order_key(race.y) << 32 : 0;
+    join_keys(sh, turn, c0, m0, best, f0);
+    const float ybest = key_value((uint32_t)(best >> 32));
+    best = 0;
     if (race.id >= 0 && race.y >= ybest - Race::margin(ybest)) {
       best = race_key(weight(race.z, m, temperature), race.e, race.id);
       tie = race.tie;
     }
-    join_keys(sh, turn, count, mass, best, tie);
-    if (!bound.none) {
-      const bool kept = count == 0 || ((!by_k || count < top_k) && (!by_p || mass < top_p * total));
-      if (kept) break;
-    }
+    join_keys(sh, turn, c0, m0, best, tie);
     if (tie || (best >> 32) == 0) {  // no single winner by y (or a key that vanished): by exact keys
-      best = 0;
-      int c1 = 0;
-      float m1 = 0.f;
-      scan_before<T, NT, true>(sl, ns, m, temperature, c, min_p, zmin, bound, c1, m1, race, best);
-      c1 = 0;
-      m1 = 0.f;
-      int f1 = 0;
-      join_keys(sh, turn, c1, m1, best, f1);
+      best = scan_exact<T, NT>(sl, ns, m, temperature, bound.none ? 0.f : min_p, zmin, bound);
+      join_keys(sh, turn, c0, m0, best, f0);
     }
-    if (best == 0) break;  // random numbers that are none
+    if (best == 0) {  // random numbers that are none: the first of the ranks
+      if (id < 0) id = first_rank<T, NT>(sh, sl, turn);
+      break;
+    }
     id = rank_id(best);
-    if (race_first && !by_k) break;
+    const float z = to_f(lrow[id]);
     bound.none = false;
     bound.id = id;
-    bound.z = to_f(lrow[id]);
-    if (!race_first && rank_key(bound.z, id) >= cl.map_shared_rank(&sh, 0)->win[k - 1]) break;  // in the list: kept
+    bound.z = z;
+    if (weight(z, m, temperature) >= min_p || z == m) {
+      if (!by_k && !by_p) break;
+      int count = 0;
+      float mass = 0.f;
+      count_before<T, NT>(sh, sl, m, c, bound, count, mass);
+      best = 0;
+      join_keys(sh, turn, count, mass, best, f0);
+      if (count == 0 || ((!by_k || count < top_k) && (!by_p || mass < top_p * total))) break;
+    }
+    race = Race();
+    race_before<T, NT>(sl, ns, m, temperature, c, min_p, zmin, bound, race);
   }
   if (part == 0 && tid == 0) result(id);
   cl.sync();  // no part leaves while another may still read its shared memory
