@@ -7,10 +7,11 @@
 //   order (greater logit first, then lower token), which is what the kernels use.
 //
 // Both are bound by reading the logits once. A thread copies its own vectors through a private ring in shared memory
-// (cp.async, no barriers), so many loads are in flight without registers. Selection: elements above a threshold that
-// at least k elements reach go to a buffer; when that fills, it is cut back to the k best (radix select on 64-bit
-// words of logit order and token, so that there are no ties) and the threshold rises. The first threshold comes from
-// the threads' maxima over their first vectors.
+// (cp.async, no barriers), so many loads are in flight without registers. Selection needs no buffer along the way: the
+// pass keeps the largest logit of each group (a thread's elements over a few steps, 4096 groups in a slice). The k-th
+// largest of the groups' maxima is a threshold that at least k elements reach, and only groups whose maximum reaches
+// it can hold such elements: about k groups are read again (k times 48 elements), and of the elements that reach the
+// threshold, hardly more than k, the k best are taken by 64-bit words of logit order and token (no ties).
 //
 // Which rows read the random numbers: with a small kept set only its tokens' (the list of the 256 best usually holds
 // all that is kept); without any filter all of them, in the same single pass as the logits.
@@ -26,15 +27,10 @@ using namespace vocab;
 
 constexpr int kMaxTop = 256;
 constexpr int kMaxParts = 8;
-constexpr int kLimit = 768;                  // entries at which the buffer is cut back, at most
+constexpr int kGroups = 4096;                // groups of a slice whose maxima are kept
+constexpr int kMaxList = 512;                // groups that are read again, at most
 constexpr int kRing = 8;                     // vectors of a thread in its ring
 constexpr float kColdest = 1e-6f;            // colder rows are greedy
-
-// The buffer holds the limit and four elements of each thread (the step of the careful path), and the parts' lists.
-template <typename T, int NT> constexpr int buf_cap() {
-  return kLimit + NT * 4 + 32 > kMaxParts * kMaxTop ? kLimit + NT * 4 + 32 : kMaxParts * kMaxTop;
-}
-template <typename T, int NT> constexpr int work_bytes() { return buf_cap<T, NT>() * 8 + kRing * NT * 16; }
 
 template <typename T, int NT>
 struct Shared {
@@ -43,16 +39,22 @@ struct Shared {
   uint64_t pbest[2];  // this CTA's partial results, read by its cluster (two sets, used in turn)
   float wm[NT / 32], ws[NT / 32];
   int wc[NT / 32];
-  uint32_t group[kMaxTop], hist[2][256], sel_min, sel_max;
+  uint32_t hist[2][256], sel_min, sel_max;
   float pm[2], ps[2];
   int pcount[2], pflag[2];
-  int count;          // entries appended to the buffer (may pass its capacity: then they were not stored)
+  int count;          // candidates (may pass the room for them: then they were not stored)
   int nwin;           // entries in win
-  int sel_need, sel_bin, sel_done;
-  __align__(16) uint8_t work[work_bytes<T, NT>()];
+  int sel_need, sel_bin, sel_done, sel_have;
+  int nlist;
+  uint16_t list[kMaxList];
+  __align__(16) uint32_t keys[kGroups];          // order of the groups' maxima
+  __align__(16) uint4 ring[kRing * NT];          // the rings; afterwards the candidates
 
-  __device__ uint64_t* buf() { return reinterpret_cast<uint64_t*>(work); }
-  __device__ uint4* ring() { return reinterpret_cast<uint4*>(work + buf_cap<T, NT>() * 8); }
+  static constexpr int kCand = kRing * NT * 2;
+  static constexpr int kWork = sizeof(uint32_t) * kGroups + sizeof(uint4) * kRing * NT;
+  static_assert(kCand >= kMaxParts * kMaxTop && kCand >= kMaxTop + NT * Slice<T>::kVec + 16, "room for the candidates");
+  __device__ uint64_t* cand() { return reinterpret_cast<uint64_t*>(ring); }
+  __device__ uint4* work() { return reinterpret_cast<uint4*>(keys); }  // all of it, for the race's ring
 };
 
 TS_DEVICE void copy16(void* dst, const void* src) {
@@ -77,8 +79,8 @@ struct Steps {
   uint4* ring;
   int nvec, count;
 
-  __device__ Steps(const Slice<T>& sl, void* work)
-      : src(sl.body() + threadIdx.x * VEC), ring(reinterpret_cast<uint4*>(work) + threadIdx.x), nvec(sl.nvec),
+  __device__ Steps(const Slice<T>& sl, uint4* rings)
+      : src(sl.body() + threadIdx.x * VEC), ring(rings + threadIdx.x), nvec(sl.nvec),
         count((sl.nvec + kVecs * NT - 1) / (kVecs * NT)) {
 #pragma unroll
     for (int t = 0; t < kAhead; ++t) fetch(t);
@@ -120,13 +122,14 @@ struct Stat {
   float m = -INFINITY, s = 0.f;
 };
 
-// Moves the `k` largest of buf[0, n) to sh.win (in no order); `least` is a lower bound of them above which no other
-// entry is. n >= k. All threads call it after a barrier that follows the last write to buf. Digits of eight bits from
-// the first bit in which the entries' logits differ.
-template <typename T, int NT>
-__device__ __noinline__ void select_k(Shared<T, NT>& sh, int n, int k, uint64_t& least) {
+// A lower bound of the k-th largest of x[0, n) above or at which exactly `reach` >= k of them are: k, or more where
+// the k-th is one of several equal ones, and then it is the bound itself. Values up to `none` do not count; `reach` is
+// 0 where fewer than k others are. All threads call it, after a barrier that follows the last write to x. Digits of
+// eight bits from the first bit in which the upper 32 differ.
+template <typename X, typename T, int NT>
+__device__ __noinline__ X kth_largest(Shared<T, NT>& sh, const X* x, int n, int k, X none, int& reach) {
+  constexpr int kBits = 8 * sizeof(X);
   const int tid = threadIdx.x;
-  const uint64_t* buf = sh.buf();
   if (tid < 256) {
     sh.hist[0][tid] = 0;
     sh.hist[1][tid] = 0;
@@ -134,33 +137,47 @@ __device__ __noinline__ void select_k(Shared<T, NT>& sh, int n, int k, uint64_t&
   if (tid == 0) {
     sh.sel_min = 0xffffffffu;
     sh.sel_max = 0;
-    sh.nwin = 0;
+    sh.sel_have = 0;
   }
   __syncthreads();
   uint32_t mn = 0xffffffffu, mx = 0;
+  int have = 0;
   for (int i = tid; i < n; i += NT) {
-    const uint32_t x = (uint32_t)(buf[i] >> 32);
-    mn = min(mn, x);
-    mx = max(mx, x);
+    const X full = x[i];
+    if (full <= none) continue;
+    const uint32_t v = (uint32_t)(full >> (kBits - 32));
+    ++have;
+    mn = min(mn, v);
+    mx = max(mx, v);
   }
   mn = __reduce_min_sync(0xffffffffu, mn);
   mx = __reduce_max_sync(0xffffffffu, mx);
-  if ((tid & 31) == 0 && mn <= mx) {
+  have = __reduce_add_sync(0xffffffffu, have);
+  if ((tid & 31) == 0 && have > 0) {
     atomicMin(&sh.sel_min, mn);
     atomicMax(&sh.sel_max, mx);
+    atomicAdd(&sh.sel_have, have);
   }
   __syncthreads();
+  if (sh.sel_have < k) {
+    reach = 0;
+    return none;
+  }
   mn = sh.sel_min;
   mx = sh.sel_max;
-  int prev = mn == mx ? 32 : 64 - __clz(mn ^ mx);  // the bits from here on are decided
-  uint64_t prefix = prev == 64 ? 0 : ((uint64_t)mx << 32) >> prev << prev;
+  int prev = mn == mx ? kBits - 32 : kBits - __clz(mn ^ mx);  // the bits from here on are decided
+  X prefix = prev == kBits ? X(0) : (X)((X)mx << (kBits - 32)) >> prev << prev;
   int need = k;
+  if (prev == 0) {  // (32-bit values that are all equal)
+    reach = sh.sel_have;
+    return prefix;
+  }
   for (int turn = 0;; turn ^= 1) {
     const int width = min(8, prev), shift = prev - width;
     const uint32_t mask = (1u << width) - 1;
     for (int i = tid; i < n; i += NT) {
-      const uint64_t x = buf[i];
-      if (prev == 64 || (x >> prev) == (prefix >> prev)) atomicAdd(&sh.hist[turn][(uint32_t)(x >> shift) & mask], 1u);
+      const X v = x[i];
+      if (v > none && (prev == kBits || (v >> prev) == (prefix >> prev))) atomicAdd(&sh.hist[turn][(uint32_t)(v >> shift) & mask], 1u);
     }
     __syncthreads();
     if (tid < 32) {
@@ -181,7 +198,7 @@ __device__ __noinline__ void select_k(Shared<T, NT>& sh, int n, int k, uint64_t&
           if ((int)above < need && (int)(above + h[j]) >= need) {
             sh.sel_bin = 255 - 8 * tid - j;
             sh.sel_need = need - (int)above;
-            sh.sel_done = (int)h[j] == need - (int)above;
+            sh.sel_done = (int)h[j];
             break;
           }
           above += h[j];
@@ -192,63 +209,31 @@ __device__ __noinline__ void select_k(Shared<T, NT>& sh, int n, int k, uint64_t&
       for (int j = 0; j < 8; ++j) sh.hist[turn][255 - 8 * tid - j] = 0;
     }
     __syncthreads();
-    prefix |= (uint64_t)sh.sel_bin << shift;
+    prefix |= (X)sh.sel_bin << shift;
     need = sh.sel_need;
     prev = shift;
-    if (sh.sel_done || shift == 0) break;  // every entry of the bin belongs to the k
+    if (sh.sel_done == need || shift == 0) break;  // the whole bin belongs to the k, or its entries are equal
   }
-  least = prefix;
-  for (int i = tid; i < n; i += NT) {
-    const uint64_t x = buf[i];
-    if (x >= prefix) {
+  reach = k - need + sh.sel_done;
+  return prefix;
+}
+
+// The k largest of the candidates, all different, to sh.win (in no order); n >= k. `least`: a lower bound of them
+// above which no other candidate is.
+template <typename T, int NT>
+__device__ void select_k(Shared<T, NT>& sh, int n, int k, uint64_t& least) {
+  int reach;
+  least = kth_largest<uint64_t>(sh, sh.cand(), n, k, 0, reach);
+  if (threadIdx.x == 0) sh.nwin = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += NT) {
+    const uint64_t x = sh.cand()[i];
+    if (x >= least) {
       const int at = atomicAdd(&sh.nwin, 1);
       if (at < kMaxTop) sh.win[at] = x;
     }
   }
   __syncthreads();
-}
-
-// A threshold that at least k of the threads' values reach (0: none found), the same in all threads: exact but for
-// the last 12 bits. Values of 32 (k <= 16) or 256 groups of threads; each warp searches them for itself.
-template <typename T, int NT>
-__device__ uint32_t group_threshold(Shared<T, NT>& sh, uint32_t mine, int k) {
-  const int tid = threadIdx.x, lane = tid & 31;
-  constexpr int kSmall = NT / 32 >= 32 ? 16 : 0;  // 32 groups are a warp each
-  const bool few = k <= kSmall;
-  const int width = few ? NT / 32 : NT / 256;  // threads of a group
-  uint32_t x = mine;
-  for (int o = 1; o < width; o <<= 1) x = max(x, __shfl_xor_sync(0xffffffffu, x, o));
-  if (tid % width == 0) sh.group[tid / width] = x;
-  __syncthreads();
-  uint32_t v[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = (j == 0 || !few) ? sh.group[lane + 32 * j] : 0u;
-  uint32_t mx = 0, mn = 0xffffffffu;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    mx = max(mx, v[j]);
-    if (j == 0 || !few) mn = min(mn, v[j]);
-  }
-  mx = __reduce_max_sync(0xffffffffu, mx);
-  mn = __reduce_min_sync(0xffffffffu, mn);
-  if (mn == mx) return mx;
-  const int top = 31 - __clz(mn ^ mx);
-  uint32_t lo = top >= 31 ? 0u : (mx >> (top + 1)) << (top + 1);  // the digits that all have
-  for (int bit = top; bit >= 12; --bit) {
-    const uint32_t cand = lo | (1u << bit);
-    int cnt;
-    if (few) {
-      cnt = __popc(__ballot_sync(0xffffffffu, v[0] >= cand));
-    } else {
-      int c = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) c += v[j] >= cand;
-      cnt = (int)__reduce_add_sync(0xffffffffu, (unsigned)c);
-    }
-    if (cnt >= k) lo = cand;
-    if (cnt == k) break;
-  }
-  return lo;
 }
 
 // Largest of a vector's values; NaN is left out (-inf if there is nothing else).
@@ -265,143 +250,141 @@ TS_DEVICE float vec_max(const float* z) {
 template <typename T, int NT>
 __device__ __noinline__ Stat scan_slice(Shared<T, NT>& sh, const Slice<T> sl, int k, float c) {
   using S = Steps<T, NT>;
-  constexpr int VEC = S::VEC, Q = S::kVecs;
+  constexpr int VEC = S::VEC, Q = S::kVecs, kSegs = kGroups / NT;
+  constexpr uint32_t kMinusInf = 0x007fffffu;  // order of -inf
   const int tid = threadIdx.x;
-  uint64_t* buf = sh.buf();
-  const int limit = min(kLimit, max(4 * k, 128));
   Stat st;
-  if (tid == 0) sh.count = 0;
-  S steps(sl, sh.ring());
-  __syncthreads();
-
-  bool slow = true;     // look at the order of every element: no threshold yet, or one below -inf
-  bool open = true;     // no threshold yet: every element is appended
-  uint32_t tkey = 0;    // else elements whose order is above it (strictly: at equal logits the lower token is in)
-  float tval = 0.f;     // the same as a logit
-  int seen = 0;         // entries of the buffer as far as this thread knows
-  auto set_threshold = [&](uint32_t key) {
-    open = false;
-    tkey = key;
-    slow = key < 0x007fffffu;  // -inf's order
-    // -0 has the order of +0: below that, the next logit down
-    tval = key == 0x7fffffffu ? __uint_as_float(0x80000001u) : key_value(key);
-  };
-  auto push = [&](float z, int id) {
-    if (slow ? open || order_key(z) > tkey : z > tval) {
-      const int at = atomicAdd(&sh.count, 1);
-      seen = at + 1;
-      if (at < buf_cap<T, NT>()) buf[at] = rank_key(z, id);
-    }
-  };
-  auto id_of = [&](int t, int q) { return sl.lo + sl.head + ((t * Q + q) * NT + tid) * VEC; };
-  auto cut = [&](int n) {  // all threads; the buffer is complete
-    if (n < k) return;
-    uint64_t least;
-    select_k<T, NT>(sh, n, k, least);
-    for (int i = tid; i < k; i += NT) buf[i] = sh.win[i];
-    if (tid == 0) sh.count = k;
-    seen = k;
-    set_threshold((uint32_t)(least >> 32));
-    __syncthreads();
-  };
-  auto edge = [&](int first, int cnt) {  // the unaligned ends: less than a vector
-    if (tid < cnt) {
-      const int i = first + tid;
-      const float z = to_f(sl.p[i]);
-      stat_raise(st.m, st.s, fmaxf(z, -INFINITY), c);
-      st.s += sum_exp<1>(&z, st.m, c);
-      push(z, sl.lo + i);
-    }
-  };
-  edge(0, sl.head);
-
-  int from = 0, t0 = 0;  // `from` entries were in the buffer before step t0
-  bool head_too = true;
-  for (int t = 0;; ++t) {
-    // the threads look whether the buffer has filled
-    if (__syncthreads_or(seen > limit)) {
-      const int n = sh.count;
-      __syncthreads();
-      if (n > buf_cap<T, NT>()) {
-        // more came than fits (very many equal logits, or rising ones): again from t0, four elements of each thread
-        // at a time
-        if (tid == 0) sh.count = from;
-        __syncthreads();
-        if (head_too && tid < sl.head) push(to_f(sl.p[tid]), sl.lo + tid);
-        for (int v = t0 * Q; v < t * Q && v * NT < sl.nvec; ++v) {
-          float z[VEC];
-          const int i = v * NT + tid;
-          if (i < sl.nvec) unpack<T>(load_stream(sl.body() + (long long)i * VEC), z);
-#pragma unroll
-          for (int h = 0; h < VEC; h += 4) {
-            if (i < sl.nvec) {
-#pragma unroll
-              for (int e = h; e < h + 4; ++e) push(z[e], sl.lo + sl.head + i * VEC + e);
-            }
-            __syncthreads();
-            const int now = sh.count;
-            __syncthreads();
-            if (now > limit) cut(now);
-          }
-        }
-        __syncthreads();
-        from = sh.count;
-        __syncthreads();
-      } else {
-        cut(n);
-        from = k;
-      }
-      seen = from;
-      t0 = t;
-      head_too = false;
-    }
-    if (t >= steps.count) break;
-    float z[Q][VEC], top[Q];
-    steps.read(t, z);
-    float zmax = -INFINITY;
-#pragma unroll
-    for (int q = 0; q < Q; ++q) {
-      top[q] = vec_max<VEC>(z[q]);
-      zmax = fmaxf(zmax, top[q]);
-    }
-    stat_raise(st.m, st.s, zmax, c);
-    st.s += sum_exp<16>(&z[0][0], st.m, c);
-    if (t == 0) {
-      // the first threshold, from the threads' largest elements so far
-      uint32_t best = 0;
-      if (zmax > -INFINITY) {
-        best = order_key(zmax);
-      } else {  // nothing but -inf and NaN, which zmax leaves out
-#pragma unroll
-        for (int q = 0; q < Q; ++q) {
-          if (steps.has(t, q)) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) best = max(best, order_key(z[q][e]));
-          }
-        }
-      }
-      const uint32_t key = group_threshold<T, NT>(sh, best, k);
-      if (key > 0) set_threshold(key - 1);
-    }
-    if (slow || zmax > tval) {
-#pragma unroll
-      for (int q = 0; q < Q; ++q) {
-        if (slow ? steps.has(t, q) : top[q] > tval) {
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) push(z[q][e], id_of(t, q) + e);
-        }
+  S steps(sl, sh.ring);
+  const int edges = sl.head + sl.tail;
+  float zedge = -INFINITY;  // an element of the unaligned ends
+  const int iedge = tid < sl.head ? tid : sl.nvec * VEC + tid;
+  if (tid < edges) {
+    zedge = to_f(sl.p[iedge]);
+    stat_raise(st.m, st.s, fmaxf(zedge, -INFINITY), c);
+    st.s += sum_exp<1>(&zedge, st.m, c);
+  }
+  const int span = max(1, (steps.count + kSegs - 1) / kSegs);  // steps of a group
+  const int groups = (steps.count + span - 1) / span * NT;
+  {
+    float gmax = -INFINITY;
+    uint32_t* key = sh.keys + tid;
+    for (int t = 0, in = 0; t < steps.count; ++t) {
+      float z[Q][VEC];
+      steps.read(t, z);
+      const float zmax = vec_max<16>(&z[0][0]);
+      stat_raise(st.m, st.s, zmax, c);
+      st.s += sum_exp<16>(&z[0][0], st.m, c);
+      gmax = fmaxf(gmax, zmax);
+      if (++in == span || t + 1 == steps.count) {
+        *key = gmax > -INFINITY ? order_key(gmax) : 0u;
+        key += NT;
+        gmax = -INFINITY;
+        in = 0;
       }
     }
   }
   copy_wait<0>();
-  edge(sl.head + sl.nvec * VEC, sl.tail);
+  if (tid == 0) {
+    sh.count = 0;
+    sh.nlist = 0;
+  }
   __syncthreads();
-  const int n = sh.count;
+
+  // elements whose order is at least `least` are candidates
+  int reach;
+  uint32_t least = kth_largest<uint32_t>(sh, sh.keys, groups, k, kMinusInf, reach);
+  if (reach == 0) ++least;           // fewer than k groups with a logit above -inf: all such logits
+  const uint32_t even = least;       // where very many logits are equal, of these only the first tokens
+  const bool many = reach > kMaxList;
+  if (many) ++least;
+  for (int i = tid; i < groups; i += NT) {
+    if (sh.keys[i] >= least) {
+      const int at = atomicAdd(&sh.nlist, 1);
+      if (at < kMaxList) sh.list[at] = (uint16_t)i;
+    }
+  }
+  uint64_t* cand = sh.cand();
+  auto push = [&](uint64_t x) {
+    const int at = atomicAdd(&sh.count, 1);
+    if (at < Shared<T, NT>::kCand) cand[at] = x;
+  };
+  if (tid < edges && order_key(zedge) >= least) push(rank_key(zedge, sl.lo + iedge));
+  __syncthreads();
+  const int width = span * Q;  // vectors of a group
+  const int tasks = sh.nlist * width;
+  auto vec_of = [&](int i) {
+    const int g = sh.list[i / width];
+    return (g / NT * width + i % width) * NT + g % NT;
+  };
+  constexpr int U = 4;
+  for (int i0 = tid; i0 < tasks; i0 += U * NT) {
+    uint4 raw[U];
+    int v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      v[u] = i0 + u * NT < tasks ? vec_of(i0 + u * NT) : sl.nvec;
+      if (v[u] < sl.nvec) raw[u] = *reinterpret_cast<const uint4*>(sl.body() + (long long)v[u] * VEC);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (v[u] >= sl.nvec) continue;
+      float z[VEC];
+      unpack<T>(raw[u], z);
+      if (order_key(vec_max<VEC>(z)) < least) continue;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        if (order_key(z[e]) >= least) push(rank_key(z[e], sl.lo + sl.head + v[u] * VEC + e));
+    }
+  }
+  __syncthreads();
+  int n = sh.count;
+  __syncthreads();
+  if (n > Shared<T, NT>::kCand) {
+    // groups that hold many such elements: again, a vector of each thread at a time, and only the k best are kept
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    if (tid < edges && order_key(zedge) >= least) push(rank_key(zedge, sl.lo + iedge));
+    uint64_t floor = (uint64_t)least << 32;
+    for (int i0 = 0; i0 < tasks; i0 += NT) {
+      const int v = i0 + tid < tasks ? vec_of(i0 + tid) : sl.nvec;
+      if (v < sl.nvec) {
+        for (int e = 0; e < VEC; ++e) {
+          const int i = sl.head + v * VEC + e;
+          const uint64_t x = rank_key(to_f(sl.p[i]), sl.lo + i);
+          if (x >= floor) push(x);
+        }
+      }
+      __syncthreads();
+      n = sh.count;
+      __syncthreads();
+      if (n > Shared<T, NT>::kCand - NT * VEC) {
+        select_k<T, NT>(sh, n, k, floor);
+        for (int i = tid; i < k; i += NT) cand[i] = sh.win[i];
+        if (tid == 0) sh.count = k;
+        __syncthreads();
+        n = k;
+      }
+    }
+  }
+  // Too few: the first tokens of the next order (the equal ones, or -inf), and after -inf NaN.
+  for (int next = many ? 2 : 0; n < k && next < 3; next = next == 0 ? 1 : 3) {
+    const uint32_t order = next == 2 ? even : next == 0 ? kMinusInf : 0u;
+    for (int i0 = 0; i0 < sl.n && n < k; i0 += NT) {
+      const int i = i0 + tid;
+      if (i < sl.n) {
+        const float z = to_f(sl.p[i]);
+        if (order_key(z) == order) push(rank_key(z, sl.lo + i));
+      }
+      __syncthreads();
+      n = sh.count;
+      __syncthreads();
+    }
+  }
   if (n > kMaxTop) {
-    uint64_t least;
-    select_k<T, NT>(sh, n, k, least);
+    uint64_t floor;
+    select_k<T, NT>(sh, n, k, floor);
   } else {
-    for (int i = tid; i < n; i += NT) sh.win[i] = buf[i];
+    for (int i = tid; i < n; i += NT) sh.win[i] = cand[i];
     if (tid == 0) sh.nwin = n;
     __syncthreads();
   }
@@ -465,7 +448,7 @@ __device__ void join_parts(Shared<T, NT>& sh, int k, float c, Stat& st) {
         if (r < parts) {
           Shared<T, NT>* o = cl.map_shared_rank(&sh, r);
           const int cnt = (r + 1 < parts ? off[r + 1 < kMaxParts ? r + 1 : r] : n) - off[r];
-          if (tid < cnt) sh.buf()[off[r] + tid] = o->win[tid];
+          if (tid < cnt) sh.cand()[off[r] + tid] = o->win[tid];
         }
       }
     }
@@ -475,7 +458,7 @@ __device__ void join_parts(Shared<T, NT>& sh, int k, float c, Stat& st) {
         uint64_t least;
         select_k<T, NT>(sh, n, k, least);
       } else {
-        if (tid < n) sh.win[tid] = sh.buf()[tid];
+        if (tid < n) sh.win[tid] = sh.cand()[tid];
         if (tid == 0) sh.nwin = n;
         __syncthreads();
       }
@@ -569,12 +552,13 @@ __device__ __noinline__ void scan_free(Shared<T, NT>& sh, const Slice<T> sl, con
   Race race;
   constexpr int VEC = Slice<T>::kVec;
   constexpr int Q = VEC / 4;  // 16-byte pieces of a vector's random numbers
-  constexpr int R = work_bytes<T, NT>() / (NT * 16 * (1 + Q)) < 6 ? work_bytes<T, NT>() / (NT * 16 * (1 + Q)) : 6;
+  constexpr int kFit = Shared<T, NT>::kWork / (NT * 16 * (1 + Q));
+  constexpr int R = kFit < 6 ? kFit : 6;
   static_assert(R >= 3, "a ring of three");
   const int tid = threadIdx.x;
   const T* body = sl.body();
   const float* nb = noise + sl.head;
-  uint4* ring = reinterpret_cast<uint4*>(sh.work) + tid;
+  uint4* ring = sh.work() + tid;
   const bool wide = (reinterpret_cast<uintptr_t>(nb) & 15) == 0;
   const int mine = tid < sl.nvec ? (sl.nvec - tid + NT - 1) / NT : 0;
   auto fetch = [&](int j) {
@@ -642,7 +626,7 @@ __device__ __noinline__ void count_before(Shared<T, NT>& sh, const Slice<T> sl, 
                                           int& count, float& mass) {
   constexpr int VEC = Slice<T>::kVec, Q = 16 / VEC;
   const int tid = threadIdx.x;
-  Steps<T, NT> steps(sl, sh.ring());
+  Steps<T, NT> steps(sl, sh.ring);
   const float bz = bound.z;
   const int bi = bound.id;
   const bool plain = m > -1e30f;  // as in sum_exp
