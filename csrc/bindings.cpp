@@ -68,6 +68,12 @@ std::vector<at::Tensor> attn_bwd_packed(const at::Tensor& dout, const at::Tensor
                                         const c10::optional<at::Tensor>& dq_out,
                                         const c10::optional<at::Tensor>& dk_out,
                                         const c10::optional<at::Tensor>& dv_out);
+std::vector<c10::optional<at::Tensor>> distill_head_fwd(const at::Tensor& h, const at::Tensor& w, const at::Tensor& ids,
+                                                        const at::Tensor& lp, double tau, bool reverse, bool tail,
+                                                        bool keep);
+at::Tensor distill_head_logits(const at::Tensor& h, const at::Tensor& w);
+void distill_head_dh(const at::Tensor& dl, const at::Tensor& w, at::Tensor& dh);
+at::Tensor distill_head_dw(const at::Tensor& dl, const at::Tensor& h);
 void register_ipc(pybind11::module& m);
 uint64_t bounds_word_rowops(bool reset);
 uint64_t bounds_word_fold(bool reset);
@@ -235,6 +241,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("sample_tokens", &ts::sample_tokens);
   m.def("distill_rows_fwd", &ts::distill_rows_fwd);
   m.def("distill_rows_bwd", &ts::distill_rows_bwd);
+  m.def("distill_head_fwd", &ts::distill_head_fwd);
+  m.def("distill_head_logits", &ts::distill_head_logits);
+  m.def("distill_head_dh", &ts::distill_head_dh);
+  m.def("distill_head_dw", &ts::distill_head_dw);
   m.def("gdn_bwd", &ts::gdn_bwd);
   m.def("gdn_chunk_fwd", &ts::gdn_chunk_fwd);
   m.def("gdn_chunk_bwd", &ts::gdn_chunk_bwd);

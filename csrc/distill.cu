@@ -331,6 +331,62 @@ __global__ void __launch_bounds__(kThreads) distill_rows_bwd_kernel(const T* __r
   }
 }
 
+// ---- the head's forward: its epilogue wants the entries in order, and leaves sums over pieces of the vocabulary
+__global__ void __launch_bounds__(kThreads) sort_entries_kernel(const int64_t* __restrict__ ids,
+                                                                const float* __restrict__ lp, int k, int v,
+                                                                int* __restrict__ ids_out, float* __restrict__ lp_out) {
+  __shared__ int slots[kMaxTop];
+  const long long row = blockIdx.x;
+  const int tid = threadIdx.x;
+  float t;
+  const int slot = entry_slot(slots, ids, lp, row, k, v, t);
+  __syncthreads();
+  if (tid >= k) return;
+  int at = 0;
+  for (int j = 0; j < k; ++j) {
+    const int o = slots[j];
+    at += slot >= 0 ? (o >= 0 && o < slot) : (o >= 0 || j < tid);
+  }
+  ids_out[row * k + at] = slot >= 0 ? slot : 0x7fffffff;
+  lp_out[row * k + at] = t;
+}
+
+__global__ void __launch_bounds__(kThreads) head_finish_kernel(HeadStats st, const float* __restrict__ lp, float tau,
+                                                               bool reverse, bool tail, DistillOut out) {
+  __shared__ Block2 b;
+  __shared__ float red[kWarps], rs[kWarps];
+  const long long row = blockIdx.x;
+  const int tid = threadIdx.x;
+  const int id = tid < st.k ? st.ids[row * st.k + tid] : 0x7fffffff;
+  const bool have = id != 0x7fffffff;
+  if (tid < st.k) out.slots[row * st.k + tid] = have ? id : -1;
+  if (!__syncthreads_or(have)) {  // a row without entries has no loss
+    if (tid < st.k) out.entry[row * st.k + tid] = 0.f;
+    if (tid == 0) out.loss[row] = out.ref[row] = out.gs[row] = 0.f;
+    return;
+  }
+  float m = -INFINITY, s = 0.f;
+  for (int i = tid; i < st.parts; i += kThreads)
+    stat_merge(m, s, st.pm[row * st.parts + i], st.ps[row * st.parts + i], st.c);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+    stat_merge(m, s, m2, s2, st.c);
+  }
+  if ((tid & 31) == 0) {
+    red[tid >> 5] = m;
+    rs[tid >> 5] = s;
+  }
+  __syncthreads();
+  m = -INFINITY;
+  s = 0.f;
+  for (int w = 0; w < kWarps; ++w) stat_merge(m, s, red[w], rs[w], st.c);
+  __syncthreads();
+  const float z = have ? st.zk[row * st.k + tid] : 0.f;
+  const float t = have ? lp[row * st.k + tid] : 0.f;
+  finish_row(b, red, row, st.k, z, t, have, m, s, st.c, tau, reverse, tail, out);
+}
+
 // Parts of a row: one where the rows alone fill the SMs, up to eight where there are few.
 int row_parts(int64_t rows, int v, int sms) {
   int parts = 1;
@@ -391,6 +447,17 @@ cudaError_t distill_rows_backward(const VocabLaunch& l, const VocabRows& x, cons
   if (otype != x.type) return cudaErrorInvalidValue;
   if (x.type == kRowsBf16) return bwd_of<__nv_bfloat16, __nv_bfloat16>(l, x, a, f, grad, out, ostride);
   return bwd_of<__half, __half>(l, x, a, f, grad, out, ostride);
+}
+
+cudaError_t distill_sort_entries(const VocabLaunch& l, const DistillArgs& a, int64_t n, int v, int* ids, float* lp) {
+  sort_entries_kernel<<<(unsigned)n, kThreads, 0, l.stream>>>(a.ids, a.lp, a.k, v, ids, lp);
+  return cudaGetLastError();
+}
+
+cudaError_t distill_head_finish(const VocabLaunch& l, const HeadStats& st, const float* lp, int64_t n, float tau,
+                                bool reverse, bool tail, const DistillOut& out) {
+  head_finish_kernel<<<(unsigned)n, kThreads, 0, l.stream>>>(st, lp, tau, reverse, tail, out);
+  return cudaGetLastError();
 }
 
 cudaError_t distill_bounds(unsigned long long* word, bool reset) {

@@ -1,0 +1,450 @@
+// tcgen05 products of the distillation head: logits = h Wᵀ with the loss's statistics in the epilogue, dH = d W over
+// slices of the vocabulary, dW = dᵀ h.
+//
+// CTA pairs (cta_group::2): a cluster of two CTAs computes a 256 x 256 tile, each staging 128 rows of A and 128 of B
+// per 64-deep K block through a six-stage TMA ring:
+//   warp 0  TMA producer, warp 1 MMA issuer (one lane each; the even CTA issues for the pair)
+//   warps 2-9  epilogue: two warps for each 32-row slab of tensor memory, half of the tile's columns each
+// The contraction is accumulated in chunks of 512: tensor memory holds one chunk's sum (two buffers, used in turn),
+// and the epilogue warps add the chunks in registers with rounded fp32 additions. The tensor core's own accumulation
+// truncates, which over a contraction of 2048 took the logits 5e-6 of their size towards zero and the loss 2e-5; and
+// a longer chunk hides the epilogue no better.
+//
+// Every wait is bounded (tc::mbar_wait); tensor memory is always freed. Loads have no multicast.
+#include "common.cuh"
+#include "tc.cuh"
+#include "vocab.cuh"
+#include "vocab.h"
+
+#include <algorithm>
+
+namespace ts {
+namespace {
+
+using namespace vocab;
+
+constexpr int kBM = 128, kBN = 256, kBK = 64, kStages = 6;
+constexpr int kChunk = 8;                                  // K blocks of a chunk
+constexpr uint32_t kABytes = kBM * kBK * 2;                // 16 KB of A ...
+constexpr uint32_t kStageBytes = kABytes + 128 * kBK * 2;  // ... and 16 KB of B per CTA and K block
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = 64 + 32 * kEpiWarps;
+constexpr uint32_t kEpiOff = kStages * kStageBytes;        // 4 KB of staging for each epilogue warp
+constexpr uint32_t kBarOff = kEpiOff + kEpiWarps * 4096;
+constexpr uint32_t kSmem = kBarOff + 256 + 1024;
+static_assert(kSmem <= 232448, "shared memory");
+
+enum Out { kNone = 0, kF32 = 1, kBf16 = 2 };
+
+struct Bars {
+  uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2];
+  uint32_t tmem_slot;
+  int abort;
+};
+
+struct Shape {
+  int m, n, k;      // C [m, n] = A [m, k] B [k, n]
+  int splits;       // slices of the contraction, one unit of work each
+  int split_rows;   // rows of C between two slices' outputs
+};
+
+struct Work {
+  int mb, nb, kb0, kb1, row_off;
+};
+
+// Unit u: slices outermost, so that what runs at one time reads the same part of both operands; then groups of eight
+// row blocks, which share B's columns.
+TS_DEVICE Work work_of(const Shape& s, int u) {
+  const int mt = (s.m + 2 * kBM - 1) / (2 * kBM), nt = (s.n + kBN - 1) / kBN, kt = (s.k + kBK - 1) / kBK;
+  const int z = u / (mt * nt), t = u % (mt * nt);
+  const int group = t / (8 * nt), r = t % (8 * nt), first = group * 8, gm = min(8, mt - first);
+  Work w;
+  w.mb = first + r % gm;
+  w.nb = r / gm;
+  const int per = (kt + s.splits - 1) / s.splits;
+  w.kb0 = min(kt, z * per);
+  w.kb1 = min(kt, w.kb0 + per);
+  w.row_off = z * s.split_rows;
+  return w;
+}
+
+TS_DEVICE void store_tile(const CUtensorMap* map, uint32_t src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];\n" ::"l"(map), "r"(src),
+               "r"(x), "r"(y)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
+}
+TS_DEVICE void store_read_wait() { asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory"); }
+TS_DEVICE void store_wait() { asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory"); }
+
+TS_DEVICE uint32_t pack2(float lo, float hi) {
+  __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+
+// This lane's 32 values (row `lane`) of a 32 x 32 chunk at (col, row0), through the warp's staging buffer: rows of 128
+// bytes (fp32) or 64 (bf16) in the output map's swizzle, which keeps the writes of 32 rows apart in the banks.
+template <int OUT>
+TS_DEVICE void store_chunk(uint32_t buf, bool& busy, const CUtensorMap* map, const float* o, int col, int row0) {
+  const int lane = threadIdx.x & 31;
+  if (busy) {  // the store before has read the buffer
+    if (lane == 0) store_read_wait();
+    __syncwarp();
+  }
+  busy = true;
+  if constexpr (OUT == kF32) {
+    const uint32_t rowb = buf + (uint32_t)lane * 128;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};\n" ::"r"(rowb + (uint32_t)((j ^ (lane & 7)) << 4)),
+                   "f"(o[4 * j]), "f"(o[4 * j + 1]), "f"(o[4 * j + 2]), "f"(o[4 * j + 3])
+                   : "memory");
+    }
+  } else {
+    const uint32_t rowb = buf + (uint32_t)lane * 64;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(rowb + (uint32_t)((j ^ ((lane >> 1) & 3)) << 4)),
+                   "r"(pack2(o[8 * j], o[8 * j + 1])), "r"(pack2(o[8 * j + 2], o[8 * j + 3])),
+                   "r"(pack2(o[8 * j + 4], o[8 * j + 5])), "r"(pack2(o[8 * j + 6], o[8 * j + 7]))
+                   : "memory");
+    }
+  }
+  tc::fence_async_smem();
+  __syncwarp();
+  if (lane == 0) store_tile(map, buf, col, row0);
+}
+
+// The row's first entry at or after `col`: the entries are sorted by token, and those that do not count are last with
+// a token past any column.
+TS_DEVICE int first_entry(const int* __restrict__ ids, int k, int col) {
+  int lo = 0, hi = k;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (__ldg(ids + mid) < col) lo = mid + 1;
+    else hi = mid;
+  }
+  return lo;
+}
+
+template <bool A_MN, bool B_MN, int OUT, bool STATS>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    head_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+                     const __grid_constant__ CUtensorMap tm_c, Shape shape, HeadStats st, int* __restrict__ err) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Bars* bars = reinterpret_cast<Bars*>(smem + kBarOff);
+  const uint32_t sbase = tc::smem_addr(smem);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = tc::cluster_rank();
+  const int units = ((shape.m + 2 * kBM - 1) / (2 * kBM)) * ((shape.n + kBN - 1) / kBN) * shape.splits;
+  const int cid = blockIdx.x >> 1, ncl = gridDim.x >> 1;
+  volatile int* abort = &bars->abort;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      tc::mbar_init(&bars->full[s], 1);
+      tc::mbar_init(&bars->empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      tc::mbar_init(&bars->acc_full[b], 1);
+      tc::mbar_init(&bars->acc_empty[b], 2 * kEpiWarps);  // the epilogue warps of both CTAs
+    }
+    bars->abort = 0;
+    tc::fence_barrier_init();
+  }
+  if (warp == 1) tc::tmem_alloc_pair(&bars->tmem_slot, 512);
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::cluster_sync();  // both CTAs' barriers exist before any remote arrive or byte count
+  tc::tc_fence_after();
+  const uint32_t tmem = bars->tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      tc::prefetch_tmap(&tm_a);
+      tc::prefetch_tmap(&tm_b);
+      int it = 0;
+      for (int u = cid; u < units; u += ncl) {
+        const Work w = work_of(shape, u);
+        const int arow = w.mb * 2 * kBM + (int)rank * kBM, bcol = w.nb * kBN + (int)rank * (kBN / 2);
+        for (int kb = w.kb0; kb < w.kb1; ++kb, ++it) {
+          const int s = it % kStages;
+          if (it >= kStages && !tc::mbar_wait(&bars->empty[s], ((it - kStages) / kStages) & 1, abort, err, 301))
+            goto producer_done;
+          if (rank == 0) tc::mbar_expect_tx(&bars->full[s], 2 * kStageBytes);
+          const uint32_t full0 = tc::map_cluster(tc::smem_addr(&bars->full[s]), 0);
+          uint8_t* a = smem + s * kStageBytes;
+          uint8_t* b = a + kABytes;
+          const int kx = kb * kBK;
+          if constexpr (!A_MN) {
+            tc::tma_load_2d_pair(a, &tm_a, kx, arow, full0);  // box 64 (k) x 128 (m)
+          } else {
+            tc::tma_load_2d_pair(a, &tm_a, arow, kx, full0);  // [K][M]: two boxes of 64 m x 64 k
+            tc::tma_load_2d_pair(a + 64 * 128, &tm_a, arow + 64, kx, full0);
+          }
+          if constexpr (!B_MN) {
+            tc::tma_load_2d_pair(b, &tm_b, kx, bcol, full0);  // box 64 (k) x 128 (n)
+          } else {
+            tc::tma_load_2d_pair(b, &tm_b, bcol, kx, full0);  // [K][N]: two boxes of 64 n x 64 k
+            tc::tma_load_2d_pair(b + 64 * 128, &tm_b, bcol + 64, kx, full0);
+          }
+        }
+      }
+    producer_done:;
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      const uint32_t idesc = tc::idesc_bf16(2 * kBM, kBN, A_MN, B_MN);
+      int it = 0, chunk = 0;
+      bool ok = true;
+      for (int u = cid; ok && u < units; u += ncl) {
+        const Work w = work_of(shape, u);
+        for (int kc = w.kb0; ok && kc < w.kb1; kc += kChunk, ++chunk) {
+          const int buf = chunk & 1;
+          if (chunk >= 2 && !tc::mbar_wait(&bars->acc_empty[buf], ((chunk - 2) >> 1) & 1, abort, err, 311)) {
+            ok = false;
+            break;
+          }
+          tc::tc_fence_after();
+          const uint32_t acc = tmem + buf * kBN;
+          const int kend = min(kc + kChunk, w.kb1);
+          for (int kb = kc; kb < kend; ++kb, ++it) {
+            const int s = it % kStages;
+            if (!tc::mbar_wait(&bars->full[s], (it / kStages) & 1, abort, err, 312)) {
+              ok = false;
+              break;
+            }
+            tc::tc_fence_after();
+            const uint32_t a = sbase + s * kStageBytes, b = a + kABytes;
+#pragma unroll
+            for (int kk = 0; kk < kBK / 16; ++kk) {
+              const uint64_t ad = A_MN ? tc::sdesc_sw128(a + kk * 16 * 128, 64 * 128, 1024)
+                                       : tc::sdesc_sw128(a + kk * 32, 16, 1024);
+              const uint64_t bd = B_MN ? tc::sdesc_sw128(b + kk * 16 * 128, 64 * 128, 1024)
+                                       : tc::sdesc_sw128(b + kk * 32, 16, 1024);
+              tc::mma_bf16_pair(acc, ad, bd, idesc, kb > kc || kk > 0);
+            }
+            tc::mma_commit_pair(&bars->empty[s]);
+          }
+          if (ok) tc::mma_commit_pair(&bars->acc_full[buf]);
+        }
+      }
+    }
+  } else {
+    const int sub = warp & 3;            // the 32-row slab of tensor memory that this warp can read
+    const int ew = warp - 2, half = ew >> 2;  // and its half of the tile's columns
+    const uint32_t lane_base = tmem + ((uint32_t)(sub * 32) << 16) + half * (kBN / 2);
+    const uint32_t acc_empty0 = tc::map_cluster(tc::smem_addr(&bars->acc_empty[0]), 0);
+    const uint32_t acc_empty1 = tc::map_cluster(tc::smem_addr(&bars->acc_empty[1]), 0);
+    const uint32_t stage = sbase + kEpiOff + (uint32_t)ew * 4096;
+    bool busy = false, ok = true;
+    int chunk = 0;
+    for (int u = cid; ok && u < units; u += ncl) {
+      const Work w = work_of(shape, u);
+      const int row0 = w.mb * 2 * kBM + (int)rank * kBM + sub * 32, row = row0 + lane;
+      const int col0 = w.nb * kBN + half * (kBN / 2);
+      int at = 0, next = 0x7fffffff;  // the row's next entry
+      const int* ids = nullptr;
+      if constexpr (STATS) {
+        if (row < shape.m) {
+          ids = st.ids + (long long)row * st.k;
+          at = first_entry(ids, st.k, col0);
+          if (at < st.k) next = __ldg(ids + at);
+        }
+      }
+      float acc[kBN / 2];
+#pragma unroll
+      for (int x = 0; x < kBN / 2; ++x) acc[x] = 0.f;
+#pragma unroll 1
+      for (int kc = w.kb0; kc < w.kb1; kc += kChunk, ++chunk) {
+        const int buf = chunk & 1;
+        if (lane == 0) ok = tc::mbar_wait(&bars->acc_full[buf], (chunk >> 1) & 1, abort, err, 321);
+        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+        if (!ok) break;
+        tc::tc_fence_after();
+#pragma unroll
+        for (int g = 0; g < 8; ++g) {
+          float v[16];
+          tc::tmem_ld16(lane_base + buf * kBN + g * 16, v);
+          tc::tmem_ld_wait();
+#pragma unroll
+          for (int x = 0; x < 16; ++x) acc[g * 16 + x] += v[x];
+        }
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive_cluster(buf ? acc_empty1 : acc_empty0);
+      }
+      if (!ok) break;
+      if (row0 >= shape.m) continue;  // the same in the whole warp
+      float m = -INFINITY, s = 0.f;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int col = col0 + g * 32;
+        float* v = acc + g * 32;
+        if (col < shape.n) {
+          if constexpr (OUT != kNone) store_chunk<OUT>(stage, busy, &tm_c, v, col, w.row_off + row0);
+          if constexpr (STATS) {
+            // the entries' logits go to their places and out of the sums
+            uint32_t hit = 0;
+            while (next < col + 32) {
+              const int x = next - col;
+              hit |= 1u << x;
+              float z = v[0];
+#pragma unroll
+              for (int q = 1; q < 32; ++q)
+                if (q == x) z = v[q];
+              st.zk[(long long)row * st.k + at] = z;
+              ++at;
+              next = at < st.k ? __ldg(ids + at) : 0x7fffffff;
+            }
+            if (col + 32 > shape.n) hit |= 0xffffffffu << (shape.n - col);
+            if (__any_sync(0xffffffffu, hit != 0)) {
+#pragma unroll
+              for (int q = 0; q < 32; ++q)
+                if ((hit >> q) & 1) v[q] = -INFINITY;
+            }
+            stat_raise(m, s, [&] {
+              float x = -INFINITY;
+#pragma unroll
+              for (int q = 0; q < 32; ++q) x = fmaxf(x, v[q]);
+              return x;
+            }(), st.c);
+            s += sum_exp<32>(v, m, st.c);
+          }
+        }
+      }
+      if constexpr (STATS) {
+        if (row < shape.m) {
+          const long long o = (long long)row * st.parts + 2 * w.nb + half;
+          st.pm[o] = m;
+          st.ps[o] = s;
+        }
+      }
+    }
+    if (OUT != kNone && lane == 0) store_wait();  // staged stores are done before shared memory goes away
+    __syncwarp();
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::cluster_sync();  // no CTA leaves while its pair may still read its shared memory or arrive on it
+  if (warp == 1) {
+    tc::tc_fence_after();
+    tc::tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+// out bf16 [rows, cols] = the sum of the slices' fp32 products, in order
+__global__ void __launch_bounds__(256) sum_slices_kernel(const float* __restrict__ x, long long slice, int splits,
+                                                         __nv_bfloat16* __restrict__ out, long long n4) {
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n4; i += gridDim.x * 256ll) {
+    float4 a = reinterpret_cast<const float4*>(x)[i];
+    for (int z = 1; z < splits; ++z) {
+      const float4 b = reinterpret_cast<const float4*>(x + z * slice)[i];
+      a.x += b.x;
+      a.y += b.y;
+      a.z += b.z;
+      a.w += b.w;
+    }
+    reinterpret_cast<uint2*>(out)[i] = make_uint2(pack2(a.x, a.y), pack2(a.z, a.w));
+  }
+}
+
+// Pairs of CTAs that the device holds at one time (the persistent grid).
+template <bool A_MN, bool B_MN, int OUT, bool STATS>
+cudaError_t resident_pairs(const VocabLaunch& l, int& pairs) {
+  static int have[16] = {0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  int& n = have[dev & 15];
+  if (n == 0) {
+    const auto kernel = head_gemm_kernel<A_MN, B_MN, OUT, STATS>;
+    e = l.set_smem((const void*)kernel, (int)kSmem);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * l.sms);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kSmem;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 2;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int most = 0;
+    e = cudaOccupancyMaxActiveClusters(&most, kernel, &cfg);
+    if (e != cudaSuccess) return e;
+    n = std::max(1, std::min(most, l.sms / 2));
+  }
+  pairs = n;
+  return cudaSuccess;
+}
+
+template <bool A_MN, bool B_MN, int OUT, bool STATS>
+cudaError_t launch(const VocabLaunch& l, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& c,
+                   const Shape& shape, const HeadStats& st, int* err) {
+  const auto kernel = head_gemm_kernel<A_MN, B_MN, OUT, STATS>;
+  int pairs = 0;
+  const cudaError_t e = resident_pairs<A_MN, B_MN, OUT, STATS>(l, pairs);
+  if (e != cudaSuccess) return e;
+  const int units = ((shape.m + 2 * kBM - 1) / (2 * kBM)) * ((shape.n + kBN - 1) / kBN) * shape.splits;
+  kernel<<<2 * std::min(units, pairs), kThreads, kSmem, l.stream>>>(a, b, c, shape, st, err);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+int head_parts(int v) { return 2 * ((v + kBN - 1) / kBN); }
+
+// Slices of dH's contraction over the vocabulary: the fewest that fill the pairs' rounds to 95%, or the fullest.
+int head_splits(const VocabLaunch& l, int rows, int d, int v) {
+  int pairs = 0;
+  if (resident_pairs<false, true, kF32, false>(l, pairs) != cudaSuccess) return 1;
+  const int tiles = ((rows + 2 * kBM - 1) / (2 * kBM)) * ((d + kBN - 1) / kBN);
+  const int kt = (v + kBK - 1) / kBK;
+  int best = 1;
+  double full = 0.0;
+  for (int s = 1; s <= 16 && kt / s >= 4 * kChunk; ++s) {
+    const int units = tiles * s, rounds = (units + pairs - 1) / pairs;
+    const double f = (double)units / ((double)rounds * pairs);
+    if (f > full + 1e-9) {
+      full = f;
+      best = s;
+    }
+    if (full >= 0.95) break;
+  }
+  return best;
+}
+
+cudaError_t head_logits(const VocabLaunch& l, const CUtensorMap& h, const CUtensorMap& w, const CUtensorMap* out,
+                        int rows, int d, int v, const HeadStats& st, int* err) {
+  const Shape s{rows, v, d, 1, 0};
+  if (out != nullptr) return launch<false, false, kF32, true>(l, h, w, *out, s, st, err);
+  return launch<false, false, kNone, true>(l, h, w, h, s, st, err);
+}
+
+cudaError_t head_logits_again(const VocabLaunch& l, const CUtensorMap& h, const CUtensorMap& w, const CUtensorMap& out,
+                              int rows, int d, int v, int* err) {
+  return launch<false, false, kF32, false>(l, h, w, out, Shape{rows, v, d, 1, 0}, HeadStats{}, err);
+}
+
+cudaError_t head_dh(const VocabLaunch& l, const CUtensorMap& dl, const CUtensorMap& w, const CUtensorMap& out, int rows,
+                    int d, int v, int splits, int split_rows, const float* parts, void* dh, int* err) {
+  const Shape s{rows, d, v, splits, split_rows};
+  if (splits == 1) return launch<false, true, kBf16, false>(l, dl, w, out, s, HeadStats{}, err);
+  const cudaError_t e = launch<false, true, kF32, false>(l, dl, w, out, s, HeadStats{}, err);
+  if (e != cudaSuccess) return e;
+  const long long n4 = (long long)rows * d / 4;
+  const int blocks = (int)std::min<long long>((n4 + 255) / 256, 8ll * l.sms);
+  sum_slices_kernel<<<blocks, 256, 0, l.stream>>>(parts, (long long)split_rows * d, splits, (__nv_bfloat16*)dh, n4);
+  return cudaGetLastError();
+}
+
+cudaError_t head_dw(const VocabLaunch& l, const CUtensorMap& dl, const CUtensorMap& h, const CUtensorMap& out, int rows,
+                    int d, int v, int* err) {
+  return launch<true, true, kBf16, false>(l, dl, h, out, Shape{v, d, rows, 1, 0}, HeadStats{}, err);
+}
+
+}  // namespace ts

@@ -2,6 +2,7 @@
 // pointers, so that the kernel sources compile without torch's headers. Each returns the launch's error.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -48,6 +49,16 @@ struct DistillOut {
   float* entry;  // [n, k] the gradient at the entries
 };
 
+struct HeadStats {      // what the logits' epilogue leaves per row
+  const int* ids = nullptr;  // [rows, k] the entries' tokens in ascending order; 0x7fffffff: none
+  int k = 0;
+  float c = 0.f;        // log2(e) / tau
+  float* pm = nullptr;  // [rows, parts] of the tokens that are no entry: the largest logit of each 128 columns ...
+  float* ps = nullptr;  // ... and their sum of 2^((z - m) c)
+  float* zk = nullptr;  // [rows, k] the entries' logits
+  int parts = 0;
+};
+
 int vocab_max_top();
 cudaError_t vocab_topk(const VocabLaunch& l, const VocabRows& x, int k, float temperature, int64_t* ids, float* lp);
 cudaError_t vocab_sample(const VocabLaunch& l, const VocabRows& x, const float* noise, long long nstride,
@@ -55,6 +66,25 @@ cudaError_t vocab_sample(const VocabLaunch& l, const VocabRows& x, const float* 
 cudaError_t distill_rows_forward(const VocabLaunch& l, const VocabRows& x, const DistillArgs& a, const DistillOut& out);
 cudaError_t distill_rows_backward(const VocabLaunch& l, const VocabRows& x, const DistillArgs& a, const DistillOut& f,
                                   const float* grad, RowType otype, void* out, long long ostride);
+// entries in ascending order of their tokens, those that do not count last (token 0x7fffffff)
+cudaError_t distill_sort_entries(const VocabLaunch& l, const DistillArgs& a, int64_t n, int v, int* ids, float* lp);
+// loss and gradient coefficients from the head's statistics; `lp` sorted as st.ids
+cudaError_t distill_head_finish(const VocabLaunch& l, const HeadStats& st, const float* lp, int64_t n, float tau,
+                                bool reverse, bool tail, const DistillOut& out);
+
+// Products of the head (csrc/head_tc.cu). Operand maps: bf16, boxes of 64 along the contiguous dimension and 128 rows
+// (64 where the contraction is not the contiguous dimension); output maps: boxes of 32 x 32.
+int head_parts(int v);
+int head_splits(const VocabLaunch& l, int rows, int d, int v);
+cudaError_t head_logits(const VocabLaunch& l, const CUtensorMap& h, const CUtensorMap& w, const CUtensorMap* out,
+                        int rows, int d, int v, const HeadStats& st, int* err);
+cudaError_t head_logits_again(const VocabLaunch& l, const CUtensorMap& h, const CUtensorMap& w, const CUtensorMap& out,
+                              int rows, int d, int v, int* err);
+cudaError_t head_dh(const VocabLaunch& l, const CUtensorMap& dl, const CUtensorMap& w, const CUtensorMap& out, int rows,
+                    int d, int v, int splits, int split_rows, const float* parts, void* dh, int* err);
+cudaError_t head_dw(const VocabLaunch& l, const CUtensorMap& dl, const CUtensorMap& h, const CUtensorMap& out, int rows,
+                    int d, int v, int* err);
+
 cudaError_t distill_bounds(unsigned long long* word, bool reset);
 
 }  // namespace ts

@@ -3,6 +3,12 @@
 #include "vocab.h"
 
 namespace ts {
+
+CUtensorMap make_bf16_map(const void* base, uint64_t inner, uint64_t outer, uint64_t row_stride_elems,
+                          uint32_t box_rows);
+CUtensorMap make_out_map(void* base, bool f32, uint64_t cols, uint64_t rows, uint64_t ld);
+at::Tensor& tc_error_flag(const at::Device& dev);
+
 namespace {
 
 void check_rows(const at::Tensor& t, const char* name) {
@@ -130,6 +136,123 @@ void distill_rows_bwd(const at::Tensor& logits, const at::Tensor& slots, const a
                      entry.data_ptr<float>()};
   TS_CUDA_CHECK(distill_rows_backward(launch_on(logits), x, a, f, grad.data_ptr<float>(), row_type(out, "gradient"),
                                       out.data_ptr(), (long long)out.stride(0)));
+}
+
+namespace {
+
+void check_bf16(const at::Tensor& t, const char* name) {
+  check_cuda(t, name);
+  TS_CHECK(t.dim() == 2 && t.scalar_type() == at::kBFloat16 && t.size(1) % 8 == 0 && t.size(0) < (int64_t(1) << 30) &&
+               t.size(1) < (int64_t(1) << 30),
+           name, " must be a bf16 matrix whose rows are a multiple of 8 long");
+}
+void check_head(const at::Tensor& h, const at::Tensor& w) {
+  check_bf16(h, "hidden");
+  check_bf16(w, "weight");
+  TS_CHECK(h.size(1) == w.size(1) && w.size(0) % 8 == 0 && w.size(0) >= 8 && w.size(0) <= 8000000 && h.size(1) >= 8 &&
+               h.device() == w.device(),
+           "hidden [N, D] and weight [V, D] with V a multiple of 8");
+}
+int* error_word(const at::Tensor& t) { return tc_error_flag(t.device()).data_ptr<int>(); }
+CUtensorMap k_rows(const at::Tensor& t) {  // [rows, k], the contraction along the rows
+  return make_bf16_map(t.data_ptr(), t.size(1), t.size(0), t.size(1), 128);
+}
+CUtensorMap k_cols(const at::Tensor& t) {  // [k, cols], the contraction down the columns
+  return make_bf16_map(t.data_ptr(), t.size(1), t.size(0), t.size(1), 64);
+}
+CUtensorMap out_map(const at::Tensor& t) {
+  return make_out_map(t.data_ptr(), t.scalar_type() == at::kFloat, t.size(1), t.size(0), t.size(1));
+}
+
+}  // namespace
+
+// hidden [N, D] and weight [V, D] bf16, teacher entries [N, K]: loss and what the backward reads, as distill_rows_fwd;
+// with `keep` the fp32 logits [N, V] too (else None).
+std::vector<c10::optional<at::Tensor>> distill_head_fwd(const at::Tensor& h, const at::Tensor& w, const at::Tensor& ids,
+                                                        const at::Tensor& lp, double tau, bool reverse, bool tail,
+                                                        bool keep) {
+  check_head(h, w);
+  check_cuda(ids, "teacher_ids");
+  check_cuda(lp, "teacher_logprobs");
+  const int64_t n = h.size(0), d = h.size(1), v = w.size(0);
+  TS_CHECK(ids.dim() == 2 && ids.size(0) == n && ids.scalar_type() == at::kLong && lp.sizes() == ids.sizes() &&
+               lp.scalar_type() == at::kFloat && ids.device() == h.device() && lp.device() == h.device(),
+           "teacher_ids must be int64 [N, K] and teacher_logprobs fp32 [N, K]");
+  const int64_t k = ids.size(1);
+  TS_CHECK(k >= 1 && k <= vocab_max_top(), "teacher entries per row must be in [1, 256]");
+  TS_CHECK(tau > 0, "temperature must be positive");
+  const c10::cuda::CUDAGuard guard(h.device());
+  const auto f32 = h.options().dtype(at::kFloat), i32 = h.options().dtype(at::kInt);
+  auto loss = at::empty({n}, f32), ref = at::empty({n}, f32), gs = at::empty({n}, f32), entry = at::empty({n, k}, f32);
+  auto slots = at::empty({n, k}, i32);
+  c10::optional<at::Tensor> logits;
+  if (keep) logits = at::empty({n, v}, f32);
+  if (n == 0) return {loss, slots, ref, gs, entry, logits};
+  const int parts = head_parts((int)v);
+  auto sorted_ids = at::empty({n, k}, i32);
+  auto sorted_lp = at::empty({n, k}, f32), zk = at::empty({n, k}, f32), sums = at::empty({2, n, parts}, f32);
+  const VocabLaunch l = launch_on(h);
+  const DistillArgs a{ids.data_ptr<int64_t>(), lp.data_ptr<float>(), (int)k, (float)tau, reverse, tail};
+  TS_CUDA_CHECK(distill_sort_entries(l, a, n, (int)v, sorted_ids.data_ptr<int>(), sorted_lp.data_ptr<float>()));
+  HeadStats st;
+  st.ids = sorted_ids.data_ptr<int>();
+  st.k = (int)k;
+  st.c = 1.4426950408889634f / (float)tau;
+  st.pm = sums.data_ptr<float>();
+  st.ps = st.pm + n * parts;
+  st.zk = zk.data_ptr<float>();
+  st.parts = parts;
+  CUtensorMap out{};
+  if (keep) out = out_map(*logits);
+  TS_CUDA_CHECK(head_logits(l, k_rows(h), k_rows(w), keep ? &out : nullptr, (int)n, (int)d, (int)v, st, error_word(h)));
+  const DistillOut o{loss.data_ptr<float>(), slots.data_ptr<int>(), ref.data_ptr<float>(), gs.data_ptr<float>(),
+                     entry.data_ptr<float>()};
+  TS_CUDA_CHECK(distill_head_finish(l, st, sorted_lp.data_ptr<float>(), n, (float)tau, reverse, tail, o));
+  return {loss, slots, ref, gs, entry, logits};
+}
+
+// fp32 logits [N, V] as distill_head_fwd computes them
+at::Tensor distill_head_logits(const at::Tensor& h, const at::Tensor& w) {
+  check_head(h, w);
+  const c10::cuda::CUDAGuard guard(h.device());
+  auto out = at::empty({h.size(0), w.size(0)}, h.options().dtype(at::kFloat));
+  if (h.size(0) == 0) return out;
+  TS_CUDA_CHECK(head_logits_again(launch_on(h), k_rows(h), k_rows(w), out_map(out), (int)h.size(0), (int)h.size(1),
+                                  (int)w.size(0), error_word(h)));
+  return out;
+}
+
+// dH [N, D] = d [N, V] · weight [V, D], bf16
+void distill_head_dh(const at::Tensor& dl, const at::Tensor& w, at::Tensor& dh) {
+  check_bf16(dl, "dlogits");
+  check_bf16(w, "weight");
+  check_bf16(dh, "dhidden");
+  const int64_t n = dl.size(0), v = dl.size(1), d = w.size(1);
+  TS_CHECK(w.size(0) == v && dh.size(0) == n && dh.size(1) == d && dl.device() == w.device() &&
+               dh.device() == w.device(),
+           "distill_head_dh shapes");
+  const c10::cuda::CUDAGuard guard(dl.device());
+  if (n == 0) return;
+  const VocabLaunch l = launch_on(dl);
+  const int splits = head_splits(l, (int)n, (int)d, (int)v);
+  const int split_rows = (int)((n + 255) / 256 * 256);  // whole tiles: a slice's last one writes no row of the next
+  at::Tensor parts;
+  if (splits > 1) parts = at::empty({(int64_t)splits * split_rows, d}, dl.options().dtype(at::kFloat));
+  TS_CUDA_CHECK(head_dh(l, k_rows(dl), k_cols(w), out_map(splits > 1 ? parts : dh), (int)n, (int)d, (int)v, splits,
+                        split_rows, splits > 1 ? parts.data_ptr<float>() : nullptr, dh.data_ptr(), error_word(dl)));
+}
+
+// dW [V, D] = dᵀ [V, N] · hidden [N, D], bf16
+at::Tensor distill_head_dw(const at::Tensor& dl, const at::Tensor& h) {
+  check_bf16(dl, "dlogits");
+  check_bf16(h, "hidden");
+  TS_CHECK(dl.size(0) == h.size(0) && dl.device() == h.device(), "distill_head_dw shapes");
+  const c10::cuda::CUDAGuard guard(dl.device());
+  auto dw = at::empty({dl.size(1), h.size(1)}, dl.options());
+  if (h.size(0) == 0) return dw.zero_();
+  TS_CUDA_CHECK(head_dw(launch_on(dl), k_cols(dl), k_cols(h), out_map(dw), (int)h.size(0), (int)h.size(1),
+                        (int)dl.size(1), error_word(dl)));
+  return dw;
 }
 
 uint64_t bounds_word_distill(bool reset) {

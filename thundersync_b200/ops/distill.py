@@ -30,7 +30,7 @@ from torch.autograd.function import once_differentiable
 from thundersync_b200.ops import sink as _sink
 from thundersync_b200.ops._ext import native
 from thundersync_b200.ops.gemm import gemm, gemm_accumulate
-from thundersync_b200.ops.logprob import DEFAULT_ROWS, _logits_fp32, _row_block
+from thundersync_b200.ops.logprob import _logits_fp32, _row_block
 
 __all__ = ["topk_logprobs", "topk_distill_loss", "lm_head_topk_distill", "MAX_ENTRIES"]
 
@@ -182,6 +182,30 @@ def topk_distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
 
 
 # ------------------------------------------------------------------ the loss from hidden states
+# Rows of a block, where the caller names none: a block's buffers are its fp32 logits (2.5 GB at 4096 rows of a
+# 151,936-token vocabulary) and bf16 dlogits (half of that). One block writes the weight gradient in bf16 at once;
+# several add fp32 products and round at the end.
+BLOCK_ROWS = 4096
+# The forward's fp32 logits that a call may keep for its backward, in bytes. A block past it computes them again,
+# which at 2048 rows x 2048 x 151,936 takes a third of the backward's time on top; keeping them holds that memory from
+# the forward to the backward.
+KEEP_LOGITS_BYTES = 3 << 30
+
+
+def _fused_ok(hidden: torch.Tensor, weight: torch.Tensor) -> bool:
+    return (hidden.is_cuda and hidden.dtype == torch.bfloat16 and weight.dtype == torch.bfloat16
+            and hidden.shape[1] % 8 == 0 and hidden.shape[1] > 0 and weight.shape[0] % 8 == 0 and weight.shape[0] > 0
+            and weight.is_contiguous())
+
+
+def _to_eight(d: torch.Tensor, h: torch.Tensor):
+    """Zero rows up to a multiple of 8 for the accumulating GEMM's contraction."""
+    pad = (-d.shape[0]) % 8
+    if not pad:
+        return d, h
+    return (torch.cat((d, d.new_zeros(pad, d.shape[1]))), torch.cat((h, h.new_zeros(pad, h.shape[1]))))
+
+
 class _HeadTopkDistill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, ids, logprobs, rows, temperature, direction, tail):
@@ -190,17 +214,30 @@ class _HeadTopkDistill(torch.autograd.Function):
         ctx.weight = weight
         ctx.save_for_backward(hidden, ids, logprobs)
         ctx.blocks = []
+        fused = _fused_ok(hidden, weight)
+        reverse = direction == "reverse"
+        room = KEEP_LOGITS_BYTES if hidden.requires_grad or weight.requires_grad else 0
         loss = []
         for r0 in range(0, n, rows):
             r1 = min(n, r0 + rows)
+            if fused:
+                size = 4 * (r1 - r0) * weight.shape[0]
+                keep = size <= room
+                room -= size if keep else 0
+                part, *kept = native().distill_head_fwd(hidden[r0:r1], weight, ids[r0:r1], logprobs[r0:r1], temperature,
+                                                        reverse, tail, keep)
+                ctx.blocks.append(kept)
+                loss.append(part)
+                continue
             logits = _logits_fp32(hidden[r0:r1], weight)
             if _native_rows(logits):
-                part, *kept = native().distill_rows_fwd(logits, ids[r0:r1], logprobs[r0:r1], temperature,
-                                                        direction == "reverse", tail)
-                ctx.blocks.append(kept)
+                part, *kept = native().distill_rows_fwd(logits, ids[r0:r1], logprobs[r0:r1], temperature, reverse, tail)
+                ctx.blocks.append([*kept, None])
             else:
                 part = _loss_reference(logits, ids[r0:r1], logprobs[r0:r1], temperature, direction, tail)
             loss.append(part)
+        if len(loss) == 1:
+            return loss[0]
         return torch.cat(loss) if loss else hidden.new_zeros(0, dtype=torch.float32)
 
     @staticmethod
@@ -211,21 +248,26 @@ class _HeadTopkDistill(torch.autograd.Function):
         rows, temperature, direction, tail = ctx.conf
         n = hidden.shape[0]
         need_h, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+        fused = _fused_ok(hidden, weight)
         dh = torch.empty_like(hidden) if need_h else None
         s = _sink.active()
         sink_w = need_w and s is not None and s.owns(weight)
+        at_once = fused and need_w and not sink_w and 0 < n <= rows  # one block: no fp32 sum of blocks
         dw = None
-        if need_w and not sink_w:
+        if need_w and not sink_w and not at_once:
             wide = torch.float32 if weight.dtype != torch.float64 else torch.float64
             dw = torch.zeros(weight.shape, dtype=wide, device=weight.device)
         g = g.contiguous()
         for i, r0 in enumerate(range(0, n, rows)):
             r1 = min(n, r0 + rows)
             h = hidden[r0:r1]
-            logits = _logits_fp32(h, weight)
+            logits = ctx.blocks[i][-1] if ctx.blocks else None
+            if logits is None:
+                logits = native().distill_head_logits(h, weight) if fused else _logits_fp32(h, weight)
             if _native_rows(logits):
                 d = torch.empty(logits.shape, dtype=hidden.dtype, device=hidden.device)
-                native().distill_rows_bwd(logits, *ctx.blocks[i], g[r0:r1].float(), temperature, d)
+                native().distill_rows_bwd(logits, *ctx.blocks[i][:-1], g[r0:r1].float(), temperature, d)
+                ctx.blocks[i] = None
             else:
                 with torch.enable_grad():
                     z = logits.requires_grad_(True)
@@ -234,12 +276,18 @@ class _HeadTopkDistill(torch.autograd.Function):
                 d = d.to(hidden.dtype)
             del logits
             if need_h:
-                gemm(d, weight, b_t=False, out=dh[r0:r1])
-            if need_w:
-                if sink_w:
-                    s.addmm_(s.view(weight), d, h)
+                if fused:
+                    native().distill_head_dh(d, weight, dh[r0:r1])
                 else:
-                    gemm_accumulate(dw, d, h, a_t=True, b_t=False)
+                    gemm(d, weight, b_t=False, out=dh[r0:r1])
+            if at_once:
+                dw = native().distill_head_dw(d, h)
+            elif need_w:
+                d8, h8 = _to_eight(d, h) if d.is_cuda else (d, h)
+                if sink_w:
+                    s.addmm_(s.view(weight), d8, h8)
+                else:
+                    gemm_accumulate(dw, d8, h8, a_t=True, b_t=False)
         ctx.weight = None
         ctx.blocks = None
         return dh, None if dw is None else dw.to(weight.dtype), None, None, None, None, None, None
@@ -247,11 +295,16 @@ class _HeadTopkDistill(torch.autograd.Function):
 
 def lm_head_topk_distill(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torch.Tensor,
                          teacher_logprobs: torch.Tensor, *, temperature: float = 1.0, direction: str = "forward",
-                         tail: bool = True, rows: int = DEFAULT_ROWS) -> torch.Tensor:
+                         tail: bool = True, rows: int | None = None) -> torch.Tensor:
     """Loss [N] (fp32) of the student ``hidden`` [N, D] · ``weight`` [V, D]ᵀ against the teacher's entries [N, K],
-    differentiable in ``hidden`` and ``weight`` (whose gradient honours an active gradient sink). ``rows`` rows are
-    worked at a time: buffers over the vocabulary hold one block. Hidden rows must be finite (a row without entries
-    gives no gradient, but its zeros meet the hidden row in the weight gradient)."""
+    differentiable in ``hidden`` and ``weight`` (whose gradient honours an active gradient sink).
+
+    ``rows`` rows are worked at a time (default ``BLOCK_ROWS``), and up to ``KEEP_LOGITS_BYTES`` of fp32 logits stay
+    from the forward to the backward; both are attributes of this module. Hidden rows must be finite: a row without
+    entries gives no gradient, but its zeros meet the hidden row in the weight gradient.
+
+    In bf16 the dlogits are rounded to bf16 before the two gradient products, as in :func:`lm_head_logprob`: the
+    tensor cores take both operands in one type, and the weight is bf16."""
     if hidden.dim() != 2:
         raise ValueError(f"hidden must be [N, D], got {tuple(hidden.shape)}")
     if weight.dim() != 2 or weight.shape[1] != hidden.shape[1]:
@@ -259,13 +312,8 @@ def lm_head_topk_distill(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids
     if weight.dtype != hidden.dtype or weight.device != hidden.device:
         raise ValueError("hidden and weight must have one dtype and device")
     ids, lp = _check_teacher(hidden.shape[0], teacher_ids, teacher_logprobs, temperature, direction, hidden.device)
-    n = hidden.shape[0]
-    rows = _row_block(rows, hidden.is_cuda)
+    rows = _row_block(BLOCK_ROWS if rows is None else rows, hidden.is_cuda)
     h = hidden.contiguous()
-    pad = (-n) % 8 if hidden.is_cuda else 0  # the weight gradient's contraction runs over whole groups of 8 rows
-    if pad:
-        h = torch.cat((h, h.new_zeros(pad, h.shape[1])))
-        ids = torch.cat((ids, ids.new_full((pad, ids.shape[1]), -1)))
-        lp = torch.cat((lp, lp.new_zeros(pad, lp.shape[1])))
-    loss = _HeadTopkDistill.apply(h, weight, ids, lp, rows, float(temperature), direction, bool(tail))
-    return loss[:n] if pad else loss
+    if h.is_cuda and h.data_ptr() % 16:  # the GEMMs' loads begin on 16-byte boundaries
+        h = h.clone()
+    return _HeadTopkDistill.apply(h, weight, ids, lp, rows, float(temperature), direction, bool(tail))
