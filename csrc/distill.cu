@@ -58,19 +58,29 @@ __device__ void block_sum2(Block2& b, double& x, double& y) {
   }
 }
 
+// The block's largest m; then sums relative to it meet without a chain of rescalings, each of which would round.
+__device__ float block_max(float* red, float m) {
+  m = warp_max(m);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+  __syncthreads();
+  m = red[0];
+  for (int w = 1; w < kWarps; ++w) m = fmaxf(m, red[w]);
+  return m;
+}
+TS_DEVICE double rescaled(float m, float s, float to, float c) {
+  return m == -INFINITY || m == to ? (double)s : (double)s * exp2(((double)m - (double)to) * c);
+}
+
 // The row's loss and gradient coefficients, by one block: thread k holds entry k (logit z, log-prob t; `have` where it
 // counts), the tokens outside S come as (m, s_tail) with s_tail = sum 2^((z - m)·c), m = -inf if there are none.
 __device__ void finish_row(Block2& b, float* red, long long row, int k, float z, float t, bool have, float m,
-                           float s_tail, float c, float tau, bool reverse, bool tail, const DistillOut& out) {
+                           double s_tail, float c, float tau, bool reverse, bool tail, const DistillOut& out) {
   const int tid = threadIdx.x;
   const float m_tail = m;
-  const float wm = warp_max(have ? z : -INFINITY);
-  __syncthreads();
-  if ((tid & 31) == 0) red[tid >> 5] = wm;
-  __syncthreads();
-  for (int w = 0; w < kWarps; ++w) m = fmaxf(m, red[w]);
+  m = fmaxf(m_tail, block_max(red, have ? z : -INFINITY));
   if (m == -INFINITY) m = 0.f;
-  const double st = m_tail == -INFINITY ? (double)s_tail : (double)s_tail * exp2(((double)m_tail - (double)m) * c);
+  const double st = m_tail == -INFINITY ? s_tail : s_tail * exp2(((double)m_tail - (double)m) * c);
   const double a2 = ((double)z - (double)m) * c;
   const double e = have ? exp2(a2) : 0.0;
   const double q = have ? exp((double)t) : 0.0;
@@ -145,8 +155,9 @@ __device__ int entry_slot(int* ids_s, const int64_t* ids, const float* lp, long 
 
 struct RowShared {
   Block2 b;
-  float red[kWarps], wm[kWarps], ws[kWarps];
-  float pm, ps;
+  float red[kWarps];
+  float pm;
+  double ps;
   int ids[kMaxTop];
 };
 
@@ -224,35 +235,28 @@ __global__ void __launch_bounds__(kThreads) distill_rows_fwd_kernel(const T* __r
     stat_raise(m, s, zmax, c);
     s += sum_exp<U * VEC>(z, m, c);
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-    stat_merge(m, s, m2, s2, c);
-  }
-  if ((tid & 31) == 0) {
-    sh.wm[tid >> 5] = m;
-    sh.ws[tid >> 5] = s;
-  }
-  __syncthreads();
-  m = -INFINITY;
-  s = 0.f;
-  for (int w = 0; w < kWarps; ++w) stat_merge(m, s, sh.wm[w], sh.ws[w], c);
+  const float top = block_max(sh.red, m);
+  double total = rescaled(m, s, top, c), none = 0.0;
+  block_sum2(sh.b, total, none);
+  m = top;
   if (parts > 1) {
     if (tid == 0) {
       sh.pm = m;
-      sh.ps = s;
+      sh.ps = total;
     }
     cl.sync();
     if (part == 0) {
-      for (int r = 1; r < parts; ++r) {
+      for (int r = 1; r < parts; ++r) m = fmaxf(m, cl.map_shared_rank(&sh, r)->pm);
+      total = 0.0;
+      for (int r = 0; r < parts; ++r) {
         RowShared* o = cl.map_shared_rank(&sh, r);
-        stat_merge(m, s, o->pm, o->ps, c);
+        total += o->pm == -INFINITY || o->pm == m ? o->ps : o->ps * exp2(((double)o->pm - (double)m) * c);
       }
     }
     cl.sync();  // no part leaves before its sums are read
     if (part != 0) return;
   }
-  finish_row(sh.b, sh.red, row, k, zk, t, slot >= 0, m, s, c, tau, reverse, tail, out);
+  finish_row(sh.b, sh.red, row, k, zk, t, slot >= 0, m, total, c, tau, reverse, tail, out);
 }
 
 // d[n, j] = -g gs 2^((z - m)·c), and g · entry at the entries of S; rows without a gradient are zeros and are not read.
@@ -354,7 +358,7 @@ __global__ void __launch_bounds__(kThreads) sort_entries_kernel(const int64_t* _
 __global__ void __launch_bounds__(kThreads) head_finish_kernel(HeadStats st, const float* __restrict__ lp, float tau,
                                                                bool reverse, bool tail, DistillOut out) {
   __shared__ Block2 b;
-  __shared__ float red[kWarps], rs[kWarps];
+  __shared__ float red[kWarps];
   const long long row = blockIdx.x;
   const int tid = threadIdx.x;
   const int id = tid < st.k ? st.ids[row * st.k + tid] : 0x7fffffff;
@@ -365,26 +369,17 @@ __global__ void __launch_bounds__(kThreads) head_finish_kernel(HeadStats st, con
     if (tid == 0) out.loss[row] = out.ref[row] = out.gs[row] = 0.f;
     return;
   }
-  float m = -INFINITY, s = 0.f;
-  for (int i = tid; i < st.parts; i += kThreads)
-    stat_merge(m, s, st.pm[row * st.parts + i], st.ps[row * st.parts + i], st.c);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-    stat_merge(m, s, m2, s2, st.c);
-  }
-  if ((tid & 31) == 0) {
-    red[tid >> 5] = m;
-    rs[tid >> 5] = s;
-  }
-  __syncthreads();
-  m = -INFINITY;
-  s = 0.f;
-  for (int w = 0; w < kWarps; ++w) stat_merge(m, s, red[w], rs[w], st.c);
-  __syncthreads();
+  const float* pm = st.pm + row * st.parts;
+  const float* ps = st.ps + row * st.parts;
+  float m = -INFINITY;
+  for (int i = tid; i < st.parts; i += kThreads) m = fmaxf(m, pm[i]);
+  m = block_max(red, m);
+  double total = 0.0, none = 0.0;
+  for (int i = tid; i < st.parts; i += kThreads) total += rescaled(pm[i], ps[i], m, st.c);
+  block_sum2(b, total, none);
   const float z = have ? st.zk[row * st.k + tid] : 0.f;
   const float t = have ? lp[row * st.k + tid] : 0.f;
-  finish_row(b, red, row, st.k, z, t, have, m, s, st.c, tau, reverse, tail, out);
+  finish_row(b, red, row, st.k, z, t, have, m, total, st.c, tau, reverse, tail, out);
 }
 
 // Parts of a row: one where the rows alone fill the SMs, up to eight where there are few.

@@ -3,8 +3,8 @@
 //
 // CTA pairs (cta_group::2): a cluster of two CTAs computes a 256 x 256 tile, each staging 128 rows of A and 128 of B
 // per 64-deep K block through a six-stage TMA ring:
-//   warp 0  TMA producer, warp 1 MMA issuer (one lane each; the even CTA issues for the pair)
-//   warps 2-9  epilogue: two warps for each 32-row slab of tensor memory, half of the tile's columns each
+//   warp 0  TMA producer, warp 1 MMA issuer (one lane each; the even CTA issues for the pair), warps 2-3 idle
+//   warps 4-11  epilogue: two warps for each 32-row slab of tensor memory, half of the tile's columns each
 // The contraction is accumulated in chunks of 512: tensor memory holds one chunk's sum (two buffers, used in turn),
 // and the epilogue warps add the chunks in registers with rounded fp32 additions. The tensor core's own accumulation
 // truncates, which over a contraction of 2048 took the logits 5e-6 of their size towards zero and the loss 2e-5; and
@@ -24,11 +24,15 @@ namespace {
 using namespace vocab;
 
 constexpr int kBM = 128, kBN = 256, kBK = 64, kStages = 6;
-constexpr int kChunk = 8;                                  // K blocks of a chunk
+constexpr int kChunkLogits = 4, kChunkGrad = 32;           // K blocks of a chunk
 constexpr uint32_t kABytes = kBM * kBK * 2;                // 16 KB of A ...
 constexpr uint32_t kStageBytes = kABytes + 128 * kBK * 2;  // ... and 16 KB of B per CTA and K block
 constexpr int kEpiWarps = 8;
-constexpr int kThreads = 64 + 32 * kEpiWarps;
+constexpr int kThreads = 128 + 32 * kEpiWarps;
+// Registers of a thread after the split of the block's (384 threads x 168 at launch): the first warpgroup gives, the
+// epilogue's two take. 128 x 56 + 256 x 224 is the launch's 64,512.
+constexpr int kRegsLaunch = 168, kRegsGive = 56, kRegsTake = 224;
+static_assert(128 * kRegsGive + 32 * kEpiWarps * kRegsTake <= kThreads * kRegsLaunch, "no more registers than launched");
 constexpr uint32_t kEpiOff = kStages * kStageBytes;        // 4 KB of staging for each epilogue warp
 constexpr uint32_t kBarOff = kEpiOff + kEpiWarps * 4096;
 constexpr uint32_t kSmem = kBarOff + 256 + 1024;
@@ -74,7 +78,7 @@ TS_DEVICE void store_tile(const CUtensorMap* map, uint32_t src, int x, int y) {
                : "memory");
   asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
 }
-TS_DEVICE void store_read_wait() { asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory"); }
+template <int N> TS_DEVICE void store_read_wait() { asm volatile("cp.async.bulk.wait_group.read %0;\n" ::"n"(N) : "memory"); }
 TS_DEVICE void store_wait() { asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory"); }
 
 TS_DEVICE uint32_t pack2(float lo, float hi) {
@@ -82,16 +86,19 @@ TS_DEVICE uint32_t pack2(float lo, float hi) {
   return *reinterpret_cast<uint32_t*>(&v);
 }
 
-// This lane's 32 values (row `lane`) of a 32 x 32 chunk at (col, row0), through the warp's staging buffer: rows of 128
-// bytes (fp32) or 64 (bf16) in the output map's swizzle, which keeps the writes of 32 rows apart in the banks.
+// This lane's 32 values (row `lane`) of a 32 x 32 chunk at (col, row0), through the warp's 4 KB of staging: rows of 128
+// bytes (fp32, one buffer) or 64 (bf16, two in turn) in the output map's swizzle, which keeps the writes of 32 rows
+// apart in the banks. `n` chunks were stored before.
 template <int OUT>
-TS_DEVICE void store_chunk(uint32_t buf, bool& busy, const CUtensorMap* map, const float* o, int col, int row0) {
+TS_DEVICE void store_chunk(uint32_t buf, int& n, const CUtensorMap* map, const float* o, int col, int row0) {
   const int lane = threadIdx.x & 31;
-  if (busy) {  // the store before has read the buffer
-    if (lane == 0) store_read_wait();
+  constexpr int kBufs = OUT == kBf16 ? 2 : 1;
+  if (n >= kBufs) {  // the store that used this buffer has read it
+    if (lane == 0) store_read_wait<kBufs - 1>();
     __syncwarp();
   }
-  busy = true;
+  if (kBufs == 2) buf += (uint32_t)(n & 1) * 2048;
+  ++n;
   if constexpr (OUT == kF32) {
     const uint32_t rowb = buf + (uint32_t)lane * 128;
 #pragma unroll
@@ -127,7 +134,7 @@ TS_DEVICE int first_entry(const int* __restrict__ ids, int k, int col) {
   return lo;
 }
 
-template <bool A_MN, bool B_MN, int OUT, bool STATS>
+template <bool A_MN, bool B_MN, int OUT, bool STATS, int kChunk>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     head_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                      const __grid_constant__ CUtensorMap tm_c, Shape shape, HeadStats st, int* __restrict__ err) {
@@ -160,86 +167,90 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   tc::tc_fence_after();
   const uint32_t tmem = bars->tmem_slot;
 
-  if (warp == 0) {
-    if (lane == 0) {
-      tc::prefetch_tmap(&tm_a);
-      tc::prefetch_tmap(&tm_b);
-      int it = 0;
-      for (int u = cid; u < units; u += ncl) {
-        const Work w = work_of(shape, u);
-        const int arow = w.mb * 2 * kBM + (int)rank * kBM, bcol = w.nb * kBN + (int)rank * (kBN / 2);
-        for (int kb = w.kb0; kb < w.kb1; ++kb, ++it) {
-          const int s = it % kStages;
-          if (it >= kStages && !tc::mbar_wait(&bars->empty[s], ((it - kStages) / kStages) & 1, abort, err, 301))
-            goto producer_done;
-          if (rank == 0) tc::mbar_expect_tx(&bars->full[s], 2 * kStageBytes);
-          const uint32_t full0 = tc::map_cluster(tc::smem_addr(&bars->full[s]), 0);
-          uint8_t* a = smem + s * kStageBytes;
-          uint8_t* b = a + kABytes;
-          const int kx = kb * kBK;
-          if constexpr (!A_MN) {
-            tc::tma_load_2d_pair(a, &tm_a, kx, arow, full0);  // box 64 (k) x 128 (m)
-          } else {
-            tc::tma_load_2d_pair(a, &tm_a, arow, kx, full0);  // [K][M]: two boxes of 64 m x 64 k
-            tc::tma_load_2d_pair(a + 64 * 128, &tm_a, arow + 64, kx, full0);
-          }
-          if constexpr (!B_MN) {
-            tc::tma_load_2d_pair(b, &tm_b, kx, bcol, full0);  // box 64 (k) x 128 (n)
-          } else {
-            tc::tma_load_2d_pair(b, &tm_b, bcol, kx, full0);  // [K][N]: two boxes of 64 n x 64 k
-            tc::tma_load_2d_pair(b + 64 * 128, &tm_b, bcol + 64, kx, full0);
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kRegsGive));
+    if (warp == 0) {
+      if (lane == 0) {
+        tc::prefetch_tmap(&tm_a);
+        tc::prefetch_tmap(&tm_b);
+        int it = 0;
+        for (int u = cid; u < units; u += ncl) {
+          const Work w = work_of(shape, u);
+          const int arow = w.mb * 2 * kBM + (int)rank * kBM, bcol = w.nb * kBN + (int)rank * (kBN / 2);
+          for (int kb = w.kb0; kb < w.kb1; ++kb, ++it) {
+            const int s = it % kStages;
+            if (it >= kStages && !tc::mbar_wait(&bars->empty[s], ((it - kStages) / kStages) & 1, abort, err, 301))
+              goto producer_done;
+            if (rank == 0) tc::mbar_expect_tx(&bars->full[s], 2 * kStageBytes);
+            const uint32_t full0 = tc::map_cluster(tc::smem_addr(&bars->full[s]), 0);
+            uint8_t* a = smem + s * kStageBytes;
+            uint8_t* b = a + kABytes;
+            const int kx = kb * kBK;
+            if constexpr (!A_MN) {
+              tc::tma_load_2d_pair(a, &tm_a, kx, arow, full0);  // box 64 (k) x 128 (m)
+            } else {
+              tc::tma_load_2d_pair(a, &tm_a, arow, kx, full0);  // [K][M]: two boxes of 64 m x 64 k
+              tc::tma_load_2d_pair(a + 64 * 128, &tm_a, arow + 64, kx, full0);
+            }
+            if constexpr (!B_MN) {
+              tc::tma_load_2d_pair(b, &tm_b, kx, bcol, full0);  // box 64 (k) x 128 (n)
+            } else {
+              tc::tma_load_2d_pair(b, &tm_b, bcol, kx, full0);  // [K][N]: two boxes of 64 n x 64 k
+              tc::tma_load_2d_pair(b + 64 * 128, &tm_b, bcol + 64, kx, full0);
+            }
           }
         }
+      producer_done:;
       }
-    producer_done:;
-    }
-  } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
-      const uint32_t idesc = tc::idesc_bf16(2 * kBM, kBN, A_MN, B_MN);
-      int it = 0, chunk = 0;
-      bool ok = true;
-      for (int u = cid; ok && u < units; u += ncl) {
-        const Work w = work_of(shape, u);
-        for (int kc = w.kb0; ok && kc < w.kb1; kc += kChunk, ++chunk) {
-          const int buf = chunk & 1;
-          if (chunk >= 2 && !tc::mbar_wait(&bars->acc_empty[buf], ((chunk - 2) >> 1) & 1, abort, err, 311)) {
-            ok = false;
-            break;
-          }
-          tc::tc_fence_after();
-          const uint32_t acc = tmem + buf * kBN;
-          const int kend = min(kc + kChunk, w.kb1);
-          for (int kb = kc; kb < kend; ++kb, ++it) {
-            const int s = it % kStages;
-            if (!tc::mbar_wait(&bars->full[s], (it / kStages) & 1, abort, err, 312)) {
+    } else if (warp == 1) {
+      if (lane == 0 && rank == 0) {
+        const uint32_t idesc = tc::idesc_bf16(2 * kBM, kBN, A_MN, B_MN);
+        int it = 0, chunk = 0;
+        bool ok = true;
+        for (int u = cid; ok && u < units; u += ncl) {
+          const Work w = work_of(shape, u);
+          for (int kc = w.kb0; ok && kc < w.kb1; kc += kChunk, ++chunk) {
+            const int buf = chunk & 1;
+            if (chunk >= 2 && !tc::mbar_wait(&bars->acc_empty[buf], ((chunk - 2) >> 1) & 1, abort, err, 311)) {
               ok = false;
               break;
             }
             tc::tc_fence_after();
-            const uint32_t a = sbase + s * kStageBytes, b = a + kABytes;
-#pragma unroll
-            for (int kk = 0; kk < kBK / 16; ++kk) {
-              const uint64_t ad = A_MN ? tc::sdesc_sw128(a + kk * 16 * 128, 64 * 128, 1024)
-                                       : tc::sdesc_sw128(a + kk * 32, 16, 1024);
-              const uint64_t bd = B_MN ? tc::sdesc_sw128(b + kk * 16 * 128, 64 * 128, 1024)
-                                       : tc::sdesc_sw128(b + kk * 32, 16, 1024);
-              tc::mma_bf16_pair(acc, ad, bd, idesc, kb > kc || kk > 0);
+            const uint32_t acc = tmem + buf * kBN;
+            const int kend = min(kc + kChunk, w.kb1);
+            for (int kb = kc; kb < kend; ++kb, ++it) {
+              const int s = it % kStages;
+              if (!tc::mbar_wait(&bars->full[s], (it / kStages) & 1, abort, err, 312)) {
+                ok = false;
+                break;
+              }
+              tc::tc_fence_after();
+              const uint32_t a = sbase + s * kStageBytes, b = a + kABytes;
+  #pragma unroll
+              for (int kk = 0; kk < kBK / 16; ++kk) {
+                const uint64_t ad = A_MN ? tc::sdesc_sw128(a + kk * 16 * 128, 64 * 128, 1024)
+                                         : tc::sdesc_sw128(a + kk * 32, 16, 1024);
+                const uint64_t bd = B_MN ? tc::sdesc_sw128(b + kk * 16 * 128, 64 * 128, 1024)
+                                         : tc::sdesc_sw128(b + kk * 32, 16, 1024);
+                tc::mma_bf16_pair(acc, ad, bd, idesc, kb > kc || kk > 0);
+              }
+              tc::mma_commit_pair(&bars->empty[s]);
             }
-            tc::mma_commit_pair(&bars->empty[s]);
+            if (ok) tc::mma_commit_pair(&bars->acc_full[buf]);
           }
-          if (ok) tc::mma_commit_pair(&bars->acc_full[buf]);
         }
       }
     }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kRegsTake));
     const int sub = warp & 3;            // the 32-row slab of tensor memory that this warp can read
-    const int ew = warp - 2, half = ew >> 2;  // and its half of the tile's columns
+    const int ew = warp - 4, half = ew >> 2;  // and its half of the tile's columns
     const uint32_t lane_base = tmem + ((uint32_t)(sub * 32) << 16) + half * (kBN / 2);
     const uint32_t acc_empty0 = tc::map_cluster(tc::smem_addr(&bars->acc_empty[0]), 0);
     const uint32_t acc_empty1 = tc::map_cluster(tc::smem_addr(&bars->acc_empty[1]), 0);
     const uint32_t stage = sbase + kEpiOff + (uint32_t)ew * 4096;
-    bool busy = false, ok = true;
-    int chunk = 0;
+    bool ok = true;
+    int chunk = 0, stored = 0;
     for (int u = cid; ok && u < units; u += ncl) {
       const Work w = work_of(shape, u);
       const int row0 = w.mb * 2 * kBM + (int)rank * kBM + sub * 32, row = row0 + lane;
@@ -263,13 +274,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
         if (!ok) break;
         tc::tc_fence_after();
+        const uint32_t from = lane_base + buf * kBN;
 #pragma unroll
-        for (int g = 0; g < 8; ++g) {
-          float v[16];
-          tc::tmem_ld16(lane_base + buf * kBN + g * 16, v);
+        for (int g = 0; g < 4; g += 2) {
+          float va[32], vb[32];
+          tc::tmem_ld32(from + g * 32, va);
+          tc::tmem_ld32(from + g * 32 + 32, vb);
           tc::tmem_ld_wait();
 #pragma unroll
-          for (int x = 0; x < 16; ++x) acc[g * 16 + x] += v[x];
+          for (int x = 0; x < 32; ++x) {
+            acc[g * 32 + x] += va[x];
+            acc[g * 32 + 32 + x] += vb[x];
+          }
         }
         tc::tc_fence_before();
         __syncwarp();
@@ -283,7 +299,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const int col = col0 + g * 32;
         float* v = acc + g * 32;
         if (col < shape.n) {
-          if constexpr (OUT != kNone) store_chunk<OUT>(stage, busy, &tm_c, v, col, w.row_off + row0);
+          if constexpr (OUT != kNone) store_chunk<OUT>(stage, stored, &tm_c, v, col, w.row_off + row0);
           if constexpr (STATS) {
             // the entries' logits go to their places and out of the sums
             uint32_t hit = 0;
@@ -351,7 +367,7 @@ __global__ void __launch_bounds__(256) sum_slices_kernel(const float* __restrict
 }
 
 // Pairs of CTAs that the device holds at one time (the persistent grid).
-template <bool A_MN, bool B_MN, int OUT, bool STATS>
+template <bool A_MN, bool B_MN, int OUT, bool STATS, int kChunk>
 cudaError_t resident_pairs(const VocabLaunch& l, int& pairs) {
   static int have[16] = {0};
   int dev = 0;
@@ -359,7 +375,7 @@ cudaError_t resident_pairs(const VocabLaunch& l, int& pairs) {
   if (e != cudaSuccess) return e;
   int& n = have[dev & 15];
   if (n == 0) {
-    const auto kernel = head_gemm_kernel<A_MN, B_MN, OUT, STATS>;
+    const auto kernel = head_gemm_kernel<A_MN, B_MN, OUT, STATS, kChunk>;
     e = l.set_smem((const void*)kernel, (int)kSmem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
@@ -382,12 +398,12 @@ cudaError_t resident_pairs(const VocabLaunch& l, int& pairs) {
   return cudaSuccess;
 }
 
-template <bool A_MN, bool B_MN, int OUT, bool STATS>
+template <bool A_MN, bool B_MN, int OUT, bool STATS, int kChunk>
 cudaError_t launch(const VocabLaunch& l, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& c,
                    const Shape& shape, const HeadStats& st, int* err) {
-  const auto kernel = head_gemm_kernel<A_MN, B_MN, OUT, STATS>;
+  const auto kernel = head_gemm_kernel<A_MN, B_MN, OUT, STATS, kChunk>;
   int pairs = 0;
-  const cudaError_t e = resident_pairs<A_MN, B_MN, OUT, STATS>(l, pairs);
+  const cudaError_t e = resident_pairs<A_MN, B_MN, OUT, STATS, kChunk>(l, pairs);
   if (e != cudaSuccess) return e;
   const int units = ((shape.m + 2 * kBM - 1) / (2 * kBM)) * ((shape.n + kBN - 1) / kBN) * shape.splits;
   kernel<<<2 * std::min(units, pairs), kThreads, kSmem, l.stream>>>(a, b, c, shape, st, err);
@@ -401,12 +417,12 @@ int head_parts(int v) { return 2 * ((v + kBN - 1) / kBN); }
 // Slices of dH's contraction over the vocabulary: the fewest that fill the pairs' rounds to 95%, or the fullest.
 int head_splits(const VocabLaunch& l, int rows, int d, int v) {
   int pairs = 0;
-  if (resident_pairs<false, true, kF32, false>(l, pairs) != cudaSuccess) return 1;
+  if (resident_pairs<false, true, kF32, false, kChunkGrad>(l, pairs) != cudaSuccess) return 1;
   const int tiles = ((rows + 2 * kBM - 1) / (2 * kBM)) * ((d + kBN - 1) / kBN);
   const int kt = (v + kBK - 1) / kBK;
   int best = 1;
   double full = 0.0;
-  for (int s = 1; s <= 16 && kt / s >= 4 * kChunk; ++s) {
+  for (int s = 1; s <= 16 && kt / s >= 32; ++s) {
     const int units = tiles * s, rounds = (units + pairs - 1) / pairs;
     const double f = (double)units / ((double)rounds * pairs);
     if (f > full + 1e-9) {
@@ -421,20 +437,20 @@ int head_splits(const VocabLaunch& l, int rows, int d, int v) {
 cudaError_t head_logits(const VocabLaunch& l, const CUtensorMap& h, const CUtensorMap& w, const CUtensorMap* out,
                         int rows, int d, int v, const HeadStats& st, int* err) {
   const Shape s{rows, v, d, 1, 0};
-  if (out != nullptr) return launch<false, false, kF32, true>(l, h, w, *out, s, st, err);
-  return launch<false, false, kNone, true>(l, h, w, h, s, st, err);
+  if (out != nullptr) return launch<false, false, kF32, true, kChunkLogits>(l, h, w, *out, s, st, err);
+  return launch<false, false, kNone, true, kChunkLogits>(l, h, w, h, s, st, err);
 }
 
 cudaError_t head_logits_again(const VocabLaunch& l, const CUtensorMap& h, const CUtensorMap& w, const CUtensorMap& out,
                               int rows, int d, int v, int* err) {
-  return launch<false, false, kF32, false>(l, h, w, out, Shape{rows, v, d, 1, 0}, HeadStats{}, err);
+  return launch<false, false, kF32, false, kChunkLogits>(l, h, w, out, Shape{rows, v, d, 1, 0}, HeadStats{}, err);
 }
 
 cudaError_t head_dh(const VocabLaunch& l, const CUtensorMap& dl, const CUtensorMap& w, const CUtensorMap& out, int rows,
                     int d, int v, int splits, int split_rows, const float* parts, void* dh, int* err) {
   const Shape s{rows, d, v, splits, split_rows};
-  if (splits == 1) return launch<false, true, kBf16, false>(l, dl, w, out, s, HeadStats{}, err);
-  const cudaError_t e = launch<false, true, kF32, false>(l, dl, w, out, s, HeadStats{}, err);
+  if (splits == 1) return launch<false, true, kBf16, false, kChunkGrad>(l, dl, w, out, s, HeadStats{}, err);
+  const cudaError_t e = launch<false, true, kF32, false, kChunkGrad>(l, dl, w, out, s, HeadStats{}, err);
   if (e != cudaSuccess) return e;
   const long long n4 = (long long)rows * d / 4;
   const int blocks = (int)std::min<long long>((n4 + 255) / 256, 8ll * l.sms);
@@ -444,7 +460,7 @@ cudaError_t head_dh(const VocabLaunch& l, const CUtensorMap& dl, const CUtensorM
 
 cudaError_t head_dw(const VocabLaunch& l, const CUtensorMap& dl, const CUtensorMap& h, const CUtensorMap& out, int rows,
                     int d, int v, int* err) {
-  return launch<true, true, kBf16, false>(l, dl, h, out, Shape{v, d, rows, 1, 0}, HeadStats{}, err);
+  return launch<true, true, kBf16, false, kChunkGrad>(l, dl, h, out, Shape{v, d, rows, 1, 0}, HeadStats{}, err);
 }
 
 }  // namespace ts

@@ -25,7 +25,8 @@ TS_DEVICE float ex2(float x) {
 TS_DEVICE float rel_exp(float z, float m, float c) { return ex2((z - (m == -INFINITY ? 0.f : m)) * c); }
 
 // Sum of rel_exp over N values. z·c - m·c as one multiply-add: the product is exact inside it, so what is rounded is
-// m·c, the same for all values, and the difference. Masks of a type's lowest value (m·c past fp32) subtract first.
+// r = m·c, the same for all values (2^-24 of r; taken back from the sum to first order), and the difference. Masks of
+// a type's lowest value (m·c past fp32) subtract first.
 template <int N>
 TS_DEVICE float sum_exp(const float* z, float m, float c) {
   float s0 = 0.f, s1 = 0.f;
@@ -37,11 +38,12 @@ TS_DEVICE float sum_exp(const float* z, float m, float c) {
       s1 += ex2(fmaf(z[e + 1], c, -r));
     }
     if (N & 1) s0 += ex2(fmaf(z[N - 1], c, -r));
-  } else {
-#pragma unroll
-    for (int e = 0; e < N; ++e) s0 += rel_exp(z[e], m, c);
+    s0 += s1;
+    return fmaf(s0, -kLn2 * fmaf(m, c, -r), s0);
   }
-  return s0 + s1;
+#pragma unroll
+  for (int e = 0; e < N; ++e) s0 += rel_exp(z[e], m, c);
+  return s0;
 }
 
 // (m, s): raise the reference to `to`, or merge another pair. An empty side has m = -inf and s = 0 (or NaN: it stays).
