@@ -68,6 +68,8 @@ std::vector<at::Tensor> attn_bwd_packed(const at::Tensor& dout, const at::Tensor
                                         const c10::optional<at::Tensor>& dq_out,
                                         const c10::optional<at::Tensor>& dk_out,
                                         const c10::optional<at::Tensor>& dv_out);
+at::Tensor distill_rows(const at::Tensor& logits, const at::Tensor& ids, const at::Tensor& lp, double tau, bool reverse,
+                        bool tail);
 std::vector<c10::optional<at::Tensor>> distill_head_fwd(const at::Tensor& h, const at::Tensor& w, const at::Tensor& ids,
                                                         const at::Tensor& lp, double tau, bool reverse, bool tail,
                                                         bool keep);
@@ -241,6 +243,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("sample_tokens", &ts::sample_tokens);
   m.def("distill_rows_fwd", &ts::distill_rows_fwd);
   m.def("distill_rows_bwd", &ts::distill_rows_bwd);
+  m.def("distill_rows", &ts::distill_rows);
   m.def("distill_head_fwd", &ts::distill_head_fwd);
   m.def("distill_head_logits", &ts::distill_head_logits);
   m.def("distill_head_dh", &ts::distill_head_dh);

@@ -22,6 +22,8 @@
 #include "vocab.cuh"
 #include "vocab.h"
 
+#include <algorithm>
+
 namespace ts {
 namespace {
 
@@ -169,7 +171,9 @@ __global__ void __launch_bounds__(kThreads) distill_rows_fwd_kernel(const T* __r
                                                                     int words) {
   constexpr int VEC = Slice<T>::kVec;
   __shared__ RowShared sh;
-  extern __shared__ uint32_t bitmap[];  // bit of token id: id - lo - head + VEC, so a vector's bits share a byte
+  extern __shared__ __align__(16) uint4 room[];  // the threads' rings, then
+  uint32_t* bitmap = reinterpret_cast<uint32_t*>(room + kRing * kThreads);
+  // ... a bit for each token: id - lo - head + VEC, so that a vector's bits share a byte
   cg::cluster_group cl = cg::this_cluster();
   const int parts = (int)cl.num_blocks(), part = (int)cl.block_rank();
   const long long row = blockIdx.x / parts;
@@ -187,8 +191,9 @@ __global__ void __launch_bounds__(kThreads) distill_rows_fwd_kernel(const T* __r
     }
     return;
   }
-  const float zk = part == 0 && slot >= 0 ? to_f(lrow[slot]) : 0.f;
   Slice<T> sl(lrow, v, part, parts);
+  Steps<T, kThreads> steps(sl, room);
+  const float zk = part == 0 && slot >= 0 ? to_f(lrow[slot]) : 0.f;
   if (slot >= sl.lo && slot < sl.lo + sl.n) {
     const int bit = slot - sl.lo - sl.head + VEC;
     atomicOr(&bitmap[bit >> 5], 1u << (bit & 31));
@@ -204,37 +209,27 @@ __global__ void __launch_bounds__(kThreads) distill_rows_fwd_kernel(const T* __r
       s += sum_exp<1>(&z, m, c);
     }
   }
-  const T* body = sl.body();
   const uint8_t* bytes = reinterpret_cast<const uint8_t*>(bitmap);
-  constexpr int U = 16 / VEC;
-  for (int i0 = tid; i0 < sl.nvec; i0 += U * kThreads) {
-    uint4 raw[U];
+  for (int step = 0; step < steps.count; ++step) {
+    constexpr int Q = Steps<T, kThreads>::kVecs;
+    float z[Q][VEC];
+    steps.read(step, z);
 #pragma unroll
-    for (int j = 0; j < U; ++j)
-      if (i0 + j * kThreads < sl.nvec) raw[j] = load_stream(body + (long long)(i0 + j * kThreads) * VEC);
-    float z[U * VEC];
-    float zmax = -INFINITY;
+    for (int q = 0; q < Q; ++q) {
+      const int i = (step * Q + q) * kThreads + tid;  // (past the end: no bits, and -inf)
+      const uint32_t in = i >= sl.nvec ? 0u
+                          : VEC == 8   ? (uint32_t)bytes[i + 1]
+                                       : (bytes[(i + 1) >> 1] >> (((i + 1) & 1) * 4)) & 15u;
+      if (in) {
 #pragma unroll
-    for (int j = 0; j < U; ++j) {
-      const int i = i0 + j * kThreads;
-      if (i < sl.nvec) {
-        unpack<T>(raw[j], z + j * VEC);
-        const uint32_t in = VEC == 8 ? bytes[i + 1] : (bytes[(i + 1) >> 1] >> (((i + 1) & 1) * 4)) & 15u;
-        if (in) {
-#pragma unroll
-          for (int e = 0; e < VEC; ++e)
-            if ((in >> e) & 1) z[j * VEC + e] = -INFINITY;
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) z[j * VEC + e] = -INFINITY;
+        for (int e = 0; e < VEC; ++e)
+          if ((in >> e) & 1) z[q][e] = -INFINITY;
       }
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) zmax = fmaxf(zmax, z[j * VEC + e]);
     }
-    stat_raise(m, s, zmax, c);
-    s += sum_exp<U * VEC>(z, m, c);
+    stat_raise(m, s, vec_max<16>(&z[0][0]), c);
+    s += sum_exp<16>(&z[0][0], m, c);
   }
+  copy_wait<0>();
   const float top = block_max(sh.red, m);
   double total = rescaled(m, s, top, c), none = 0.0;
   block_sum2(sh.b, total, none);
@@ -382,25 +377,29 @@ __global__ void __launch_bounds__(kThreads) head_finish_kernel(HeadStats st, con
   finish_row(b, red, row, st.k, z, t, have, m, total, st.c, tau, reverse, tail, out);
 }
 
-// Parts of a row: one where the rows alone fill the SMs, up to eight where there are few.
-int row_parts(int64_t rows, int v, int sms) {
+// Parts of a row, in doublings up to eight while they are at most `most` CTAs an SM in all and a part has `least`
+// logits. The forward's parts are a cluster that joins its sums (in us, with 1 / 2 / 4 / 8 parts, V = 151,936: 64 bf16
+// rows 25 / 19 / 17 / 21, 1000 79 / 92 / 123 / 194); the backward's know nothing of each other, and shorter ones even
+// out the last round (1000 bf16 rows 132 / 117 / 107 / 107).
+int row_parts(int64_t rows, int v, int sms, int most, int least) {
   int parts = 1;
-  while (parts < kMaxParts && rows * parts < 4 * sms && v / (2 * parts) >= 4096) parts *= 2;
+  while (parts < kMaxParts && 2 * rows * parts <= (int64_t)most * sms && v / (2 * parts) >= least) parts *= 2;
   return parts;
 }
 
 template <typename T>
 cudaError_t fwd_of(const VocabLaunch& l, const VocabRows& x, const DistillArgs& a, const DistillOut& out) {
-  int parts = row_parts(x.n, x.v, l.sms);
+  int parts = row_parts(x.n, x.v, l.sms, 3, 32768);
   while (parts < kMaxParts && x.v / parts > 1000000) parts *= 2;  // the bitmap has to fit
   const int len = ((x.v + parts - 1) / parts + 63) / 64 * 64;
   const int words = (len + 16 + 31) / 32 + 1;
-  const cudaError_t e = l.set_smem((const void*)distill_rows_fwd_kernel<T>, words * 4);
+  const int bytes = kRing * kThreads * 16 + words * 4;
+  const cudaError_t e = l.set_smem((const void*)distill_rows_fwd_kernel<T>, bytes);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(x.n * parts));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = words * 4;
+  cfg.dynamicSmemBytes = bytes;
   cfg.stream = l.stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -416,7 +415,7 @@ cudaError_t fwd_of(const VocabLaunch& l, const VocabRows& x, const DistillArgs& 
 template <typename T, typename O>
 cudaError_t bwd_of(const VocabLaunch& l, const VocabRows& x, const DistillArgs& a, const DistillOut& f,
                    const float* grad, void* out, long long ostride) {
-  const int parts = row_parts(x.n, x.v, l.sms);
+  const int parts = std::max(row_parts(x.n, x.v, l.sms, 1 << 20, 16384), row_parts(x.n, x.v, l.sms, 6, 4096));
   distill_rows_bwd_kernel<T, O><<<(unsigned)(x.n * parts), kThreads, 0, l.stream>>>(
       (const T*)x.logits, x.stride, x.v, f.slots, f.ref, f.gs, f.entry, grad, a.k, a.tau, parts, (O*)out, ostride);
   return cudaGetLastError();

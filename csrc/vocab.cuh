@@ -107,5 +107,81 @@ TS_DEVICE uint64_t rank_key(float v, int id) { return ((uint64_t)order_key(v) <<
 TS_DEVICE int rank_id(uint64_t k) { return (int)~(uint32_t)k; }
 TS_DEVICE float rank_value(uint64_t k) { return key_value((uint32_t)(k >> 32)); }
 
+TS_DEVICE void copy16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
+               : "memory");
+}
+TS_DEVICE void copy4(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
+               : "memory");
+}
+TS_DEVICE void copy_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+template <int N> TS_DEVICE void copy_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
+
+// Largest of a vector's values; NaN is left out (-inf if there is nothing else).
+template <int N>
+TS_DEVICE float vec_max(const float* z) {
+  float x = -INFINITY;
+#pragma unroll
+  for (int e = 0; e < N; ++e) x = fmaxf(x, z[e]);
+  return x;
+}
+
+constexpr int kRing = 8;  // vectors of a thread in its ring
+
+// This thread's vectors of a slice through its private ring, a step of 16 elements (four vectors, or two of 16-bit
+// types) at a time: vectors t·kVecs + q, q < kVecs, of every thread. Places past the end read as -inf.
+template <typename T, int NT>
+struct Steps {
+  static constexpr int VEC = Slice<T>::kVec;
+  static constexpr int kVecs = 16 / VEC;
+  static constexpr int kAhead = kRing / kVecs;  // steps in flight
+  const T* src;
+  uint4* ring;
+  int nvec, count;
+
+  __device__ Steps(const Slice<T>& sl, uint4* rings)
+      : src(sl.body() + threadIdx.x * VEC), ring(rings + threadIdx.x), nvec(sl.nvec),
+        count((sl.nvec + kVecs * NT - 1) / (kVecs * NT)) {
+#pragma unroll
+    for (int t = 0; t < kAhead; ++t) fetch(t);
+  }
+  TS_DEVICE bool has(int t, int q) const { return (t * kVecs + q) * NT + (int)threadIdx.x < nvec; }
+  TS_DEVICE void fetch(int t) {
+    uint4* to = ring + (t % kAhead) * (kVecs * NT);
+    const T* from = src + (long long)t * (kVecs * NT * VEC);
+    if ((t + 1) * kVecs * NT <= nvec) {
+#pragma unroll
+      for (int q = 0; q < kVecs; ++q) copy16(to + q * NT, from + q * NT * VEC);
+    } else {
+#pragma unroll
+      for (int q = 0; q < kVecs; ++q)
+        if (has(t, q)) copy16(to + q * NT, from + q * NT * VEC);
+    }
+    copy_commit();
+  }
+  // step t (in order), and the fetch of the one that takes its place
+  TS_DEVICE void read(int t, float (&z)[kVecs][VEC]) {
+    copy_wait<kAhead - 1>();
+    const uint4* at = ring + (t % kAhead) * (kVecs * NT);
+#pragma unroll
+    for (int q = 0; q < kVecs; ++q) unpack<T>(at[q * NT], z[q]);
+    if ((t + 1) * kVecs * NT > nvec) {
+#pragma unroll
+      for (int q = 0; q < kVecs; ++q) {
+        if (!has(t, q)) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) z[q][e] = -INFINITY;
+        }
+      }
+    }
+    fetch(t + kAhead);
+  }
+};
+
+struct Stat {
+  float m = -INFINITY, s = 0.f;
+};
+
 }  // namespace vocab
 }  // namespace ts

@@ -140,6 +140,29 @@ void distill_rows_bwd(const at::Tensor& logits, const at::Tensor& slots, const a
 
 namespace {
 
+// The loss on logits as a native autograd node: its backward needs no interpreter, which for a few rows was most of
+// the call's time.
+struct DistillRows : torch::autograd::Function<DistillRows> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& ids,
+                            const at::Tensor& lp, double tau, bool reverse, bool tail) {
+    auto r = distill_rows_fwd(logits, ids, lp, tau, reverse, tail);
+    ctx->save_for_backward({logits, r[1], r[2], r[3], r[4]});
+    ctx->saved_data["tau"] = tau;
+    return r[0];
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    at::Tensor d;
+    if (grads[0].defined()) {
+      const auto s = ctx->get_saved_variables();
+      d = at::empty(s[0].sizes(), s[0].options());
+      distill_rows_bwd(s[0], s[1], s[2], s[3], s[4], grads[0].to(at::kFloat).contiguous(),
+                       ctx->saved_data["tau"].toDouble(), d);
+    }
+    return {d, {}, {}, {}, {}, {}};
+  }
+};
+
 void check_bf16(const at::Tensor& t, const char* name) {
   check_cuda(t, name);
   TS_CHECK(t.dim() == 2 && t.scalar_type() == at::kBFloat16 && t.size(1) % 8 == 0 && t.size(0) < (int64_t(1) << 30) &&
@@ -165,6 +188,12 @@ CUtensorMap out_map(const at::Tensor& t) {
 }
 
 }  // namespace
+
+// distill_rows_fwd's loss, differentiable in the logits
+at::Tensor distill_rows(const at::Tensor& logits, const at::Tensor& ids, const at::Tensor& lp, double tau, bool reverse,
+                        bool tail) {
+  return DistillRows::apply(logits, ids, lp, tau, reverse, tail);
+}
 
 // hidden [N, D] and weight [V, D] bf16, teacher entries [N, K]: loss and what the backward reads, as distill_rows_fwd;
 // with `keep` the fp32 logits [N, V] too (else None).

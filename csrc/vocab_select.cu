@@ -29,7 +29,6 @@ constexpr int kMaxTop = 256;
 constexpr int kMaxParts = 8;
 constexpr int kGroups = 4096;                // groups of a slice whose maxima are kept
 constexpr int kMaxList = 512;                // groups that are read again, at most
-constexpr int kRing = 8;                     // vectors of a thread in its ring
 constexpr float kColdest = 1e-6f;            // colder rows are greedy
 
 template <typename T, int NT>
@@ -45,8 +44,9 @@ struct Shared {
   int count;          // candidates (may pass the room for them: then they were not stored)
   int nwin;           // entries in win
   int sel_need, sel_bin, sel_done, sel_have;
-  int nlist;
+  int nlist;          // groups on the list (may pass its room: then they were not noted)
   uint16_t list[kMaxList];
+  uint32_t top[kMaxTop];
   __align__(16) uint32_t keys[kGroups];          // order of the groups' maxima
   __align__(16) uint4 ring[kRing * NT];          // the rings; afterwards the candidates
 
@@ -55,71 +55,6 @@ struct Shared {
   static_assert(kCand >= kMaxParts * kMaxTop && kCand >= kMaxTop + NT * Slice<T>::kVec + 16, "room for the candidates");
   __device__ uint64_t* cand() { return reinterpret_cast<uint64_t*>(ring); }
   __device__ uint4* work() { return reinterpret_cast<uint4*>(keys); }  // all of it, for the race's ring
-};
-
-TS_DEVICE void copy16(void* dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
-               : "memory");
-}
-TS_DEVICE void copy4(void* dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
-               : "memory");
-}
-TS_DEVICE void copy_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
-template <int N> TS_DEVICE void copy_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
-
-// This thread's vectors of a slice through its private ring, a step of 16 elements (four vectors, or two of 16-bit
-// types) at a time: vectors t·kVecs + q, q < kVecs, of every thread. Places past the end read as -inf.
-template <typename T, int NT>
-struct Steps {
-  static constexpr int VEC = Slice<T>::kVec;
-  static constexpr int kVecs = 16 / VEC;
-  static constexpr int kAhead = kRing / kVecs;  // steps in flight
-  const T* src;
-  uint4* ring;
-  int nvec, count;
-
-  __device__ Steps(const Slice<T>& sl, uint4* rings)
-      : src(sl.body() + threadIdx.x * VEC), ring(rings + threadIdx.x), nvec(sl.nvec),
-        count((sl.nvec + kVecs * NT - 1) / (kVecs * NT)) {
-#pragma unroll
-    for (int t = 0; t < kAhead; ++t) fetch(t);
-  }
-  TS_DEVICE bool has(int t, int q) const { return (t * kVecs + q) * NT + (int)threadIdx.x < nvec; }
-  TS_DEVICE void fetch(int t) {
-    uint4* to = ring + (t % kAhead) * (kVecs * NT);
-    const T* from = src + (long long)t * (kVecs * NT * VEC);
-    if ((t + 1) * kVecs * NT <= nvec) {
-#pragma unroll
-      for (int q = 0; q < kVecs; ++q) copy16(to + q * NT, from + q * NT * VEC);
-    } else {
-#pragma unroll
-      for (int q = 0; q < kVecs; ++q)
-        if (has(t, q)) copy16(to + q * NT, from + q * NT * VEC);
-    }
-    copy_commit();
-  }
-  // step t (in order), and the fetch of the one that takes its place
-  TS_DEVICE void read(int t, float (&z)[kVecs][VEC]) {
-    copy_wait<kAhead - 1>();
-    const uint4* at = ring + (t % kAhead) * (kVecs * NT);
-#pragma unroll
-    for (int q = 0; q < kVecs; ++q) unpack<T>(at[q * NT], z[q]);
-    if ((t + 1) * kVecs * NT > nvec) {
-#pragma unroll
-      for (int q = 0; q < kVecs; ++q) {
-        if (!has(t, q)) {
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) z[q][e] = -INFINITY;
-        }
-      }
-    }
-    fetch(t + kAhead);
-  }
-};
-
-struct Stat {
-  float m = -INFINITY, s = 0.f;
 };
 
 // A lower bound of the k-th largest of x[0, n) above or at which exactly `reach` >= k of them are: k, or more where
@@ -236,13 +171,38 @@ __device__ void select_k(Shared<T, NT>& sh, int n, int k, uint64_t& least) {
   __syncthreads();
 }
 
-// Largest of a vector's values; NaN is left out (-inf if there is nothing else).
-template <int N>
-TS_DEVICE float vec_max(const float* z) {
-  float x = -INFINITY;
+// A threshold that at least k of 256 groups' values (`mine`, the greatest of a group's threads) reach, the same in all
+// threads, or 0: exact but for the last 12 bits. Each warp looks for itself, bit by bit, with 8 values in a lane.
+template <typename T, int NT>
+__device__ __noinline__ uint32_t group_threshold(Shared<T, NT>& sh, uint32_t mine, int k) {
+  constexpr int kWidth = NT / kMaxTop;  // threads of a group
+  const int tid = threadIdx.x, lane = tid & 31;
 #pragma unroll
-  for (int e = 0; e < N; ++e) x = fmaxf(x, z[e]);
-  return x;
+  for (int o = 1; o < kWidth; o <<= 1) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+  if (tid % kWidth == 0) sh.top[tid / kWidth] = mine;
+  __syncthreads();
+  uint32_t v[8], mx = 0, mn = 0xffffffffu;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    v[j] = sh.top[lane + 32 * j];
+    mx = max(mx, v[j]);
+    mn = min(mn, v[j]);
+  }
+  mx = __reduce_max_sync(0xffffffffu, mx);
+  mn = __reduce_min_sync(0xffffffffu, mn);
+  if (mn == mx) return mx;
+  const int first = 31 - __clz(mn ^ mx);
+  uint32_t lo = first >= 31 ? 0u : (mx >> (first + 1)) << (first + 1);  // the digits that all have
+  for (int bit = first; bit >= 12; --bit) {
+    const uint32_t cand = lo | (1u << bit);
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) n += v[j] >= cand;
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (n >= k) lo = cand;
+    if (n == k) break;
+  }
+  return lo;
 }
 
 // Leaves the slice's k largest (all of it where it is shorter) in sh.win, sh.nwin entries of which some may be
@@ -288,20 +248,39 @@ __device__ __noinline__ Stat scan_slice(Shared<T, NT>& sh, const Slice<T> sl, in
     sh.count = 0;
     sh.nlist = 0;
   }
-  __syncthreads();
-
-  // elements whose order is at least `least` are candidates
-  int reach;
-  uint32_t least = kth_largest<uint32_t>(sh, sh.keys, groups, k, kMinusInf, reach);
-  if (reach == 0) ++least;           // fewer than k groups with a logit above -inf: all such logits
-  const uint32_t even = least;       // where very many logits are equal, of these only the first tokens
-  const bool many = reach > kMaxList;
-  if (many) ++least;
-  for (int i = tid; i < groups; i += NT) {
-    if (sh.keys[i] >= least) {
-      const int at = atomicAdd(&sh.nlist, 1);
-      if (at < kMaxList) sh.list[at] = (uint16_t)i;
+  // Elements whose order is at least `least` are candidates. The k-th largest of 256 threads' maxima is a little lower
+  // than that of the 4096 groups (73 groups reach it instead of 64 where k is 64, 173 instead of 128) and costs one
+  // barrier instead of about ten; from half of the threads on it says too little.
+  uint32_t least = 0, even = 0;
+  bool many = false;
+  auto note_groups = [&]() {
+    for (int i = tid; i < groups; i += NT) {
+      if (sh.keys[i] >= least) {
+        const int at = atomicAdd(&sh.nlist, 1);
+        if (at < kMaxList) sh.list[at] = (uint16_t)i;
+      }
     }
+    __syncthreads();
+  };
+  bool found = false;
+  if (k <= kMaxTop / 2) {
+    least = group_threshold<T, NT>(sh, st.m > -INFINITY ? order_key(st.m) : 0u, k);
+    if (least > kMinusInf) {
+      note_groups();
+      found = sh.nlist <= kMaxList;
+    }
+  }
+  __syncthreads();
+  if (!found) {  // the same in all threads
+    int reach;
+    least = kth_largest<uint32_t>(sh, sh.keys, groups, k, kMinusInf, reach);
+    if (reach == 0) ++least;  // fewer than k groups with a logit above -inf: all such logits
+    even = least;             // where very many logits are equal, of these only the first tokens
+    many = reach > kMaxList;
+    if (many) ++least;
+    if (tid == 0) sh.nlist = 0;
+    __syncthreads();
+    note_groups();
   }
   uint64_t* cand = sh.cand();
   auto push = [&](uint64_t x) {
@@ -972,14 +951,17 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) sample_kernel(const T* 
   cl.sync();  // no part leaves while another may still read its shared memory
 }
 
-// Parts (CTAs) of a row and threads of a part: one part where the rows alone fill the SMs, up to a cluster of eight
-// where there are few, and then with all the threads of an SM.
-int row_parts(int64_t rows, int v, int sms) {
+// Parts (CTAs, a cluster) of a row, in doublings up to eight while they are at most `most` CTAs an SM in all and a part
+// has `least` logits. Joining the parts of a row costs more than it brings where the rows alone fill the SMs. Measured
+// in us, with 1 / 2 / 4 / 8 parts, V = 151,936: top 20 of 64 bf16 rows 24 / 19 / 19 / 23, of 200 31 / 29 / 43 / 62;
+// top 64 of 300 fp32 rows 45 / 58 / 64 / 82.
+int row_parts(int64_t rows, int v, int sms, int most, int least) {
   int parts = 1;
-  while (parts < kMaxParts && rows * parts < 4 * sms && v / (2 * parts) >= 4096) parts *= 2;
+  while (parts < kMaxParts && 2 * rows * parts <= (int64_t)most * sms && v / (2 * parts) >= least) parts *= 2;
   return parts;
 }
-bool few_rows(int64_t rows, int parts, int sms) { return rows * parts <= sms && parts == kMaxParts; }
+// A part takes all the threads of an SM where there are fewer parts than SMs.
+bool few_rows(int64_t rows, int parts, int sms) { return rows * parts <= sms; }
 
 template <typename T, int NT, typename... KArgs, typename... Args>
 cudaError_t launch_rows(const VocabLaunch& l, void (*kernel)(KArgs...), int64_t rows, int parts, Args&&... args) {
@@ -1003,7 +985,7 @@ cudaError_t launch_rows(const VocabLaunch& l, void (*kernel)(KArgs...), int64_t 
 
 template <typename T>
 cudaError_t topk_of(const VocabLaunch& l, const VocabRows& x, int k, float temperature, int64_t* ids, float* lp) {
-  const int parts = row_parts(x.n, x.v, l.sms);
+  const int parts = row_parts(x.n, x.v, l.sms, 3, 32768);
   if (few_rows(x.n, parts, l.sms))
     return launch_rows<T, 1024>(l, topk_kernel<T, 1024>, x.n, parts, (const T*)x.logits, x.stride, x.v, k, temperature,
                                 ids, lp);
@@ -1013,7 +995,16 @@ cudaError_t topk_of(const VocabLaunch& l, const VocabRows& x, int k, float tempe
 template <typename T>
 cudaError_t sample_of(const VocabLaunch& l, const VocabRows& x, const float* noise, long long nstride,
                       const SampleArgs& a, int64_t* tokens, float* lp) {
-  const int parts = row_parts(x.n, x.v, l.sms);
+  // The settings decide how often a row is read: once for a small top-k, once with the random numbers without a filter,
+  // and again for each winner of the race that has to be looked at under a top-p or min-p, which wants more parts (512
+  // fp32 rows, top-p 0.9, 1 / 2 / 4 / 8 parts: 450 / 331 / 280 / 334 us). Settings of each row may be any of these.
+  const bool mixed = a.temperature || a.top_k || a.top_p || a.min_p;
+  const bool list = a.temperature_s < kColdest || (a.top_k_s > 0 && a.top_k_s <= kMaxTop);
+  const bool filter = a.top_p_s < 1.f || a.min_p_s > 0.f || a.top_k_s > 0;
+  const int parts = mixed    ? row_parts(x.n, x.v, l.sms, 8, 16384)
+                    : list   ? row_parts(x.n, x.v, l.sms, 3, 32768)
+                    : filter ? row_parts(x.n, x.v, l.sms, 16, 16384)
+                             : row_parts(x.n, x.v, l.sms, 3, 16384);
   if (few_rows(x.n, parts, l.sms))
     return launch_rows<T, 1024>(l, sample_kernel<T, 1024>, x.n, parts, (const T*)x.logits, x.stride, noise, nstride,
                                 x.v, a, tokens, lp);

@@ -150,24 +150,6 @@ def _loss_reference(z, ids, logprobs, temperature, direction, tail):
     return loss
 
 
-class _TopkDistillRows(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, ids, logprobs, temperature, direction, tail):
-        ctx.temperature = temperature
-        loss, slots, ref, gs, entry = native().distill_rows_fwd(logits, ids, logprobs, temperature,
-                                                                direction == "reverse", tail)
-        ctx.save_for_backward(logits, slots, ref, gs, entry)
-        return loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        logits, slots, ref, gs, entry = ctx.saved_tensors
-        d = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        native().distill_rows_bwd(logits, slots, ref, gs, entry, g.float().contiguous(), ctx.temperature, d)
-        return d, None, None, None, None, None
-
-
 def topk_distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logprobs: torch.Tensor, *,
                       temperature: float = 1.0, direction: str = "forward", tail: bool = True) -> torch.Tensor:
     """Loss [N] (fp32) of student ``logits`` [N, V] against the teacher's entries [N, K], differentiable in ``logits``.
@@ -176,7 +158,8 @@ def topk_distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     _check_logits(logits)
     ids, lp = _check_teacher(logits.shape[0], teacher_ids, teacher_logprobs, temperature, direction, logits.device)
     if _native_rows(logits):
-        return _TopkDistillRows.apply(_rows_contiguous(logits), ids, lp, float(temperature), direction, bool(tail))
+        return native().distill_rows(_rows_contiguous(logits), ids, lp, float(temperature), direction == "reverse",
+                                     bool(tail))
     z = logits if logits.dtype == torch.float64 else logits.float()
     return _loss_reference(z, ids, lp, temperature, direction, tail)
 
