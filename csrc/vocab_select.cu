@@ -39,7 +39,10 @@ struct Shared {
   float wm[NT / 32], ws[NT / 32];
   int wc[NT / 32];
   uint32_t hist[2][256], sel_min, sel_max;
-  float pm[2], ps[2];
+  float pm[2], ps[2], jm, js;
+  float ybest;        // of the race so far: some thread's, not always the latest
+  uint64_t jbest;
+  int jcount, jflag;
   int pcount[2], pflag[2];
   int count;          // candidates (may pass the room for them: then they were not stored)
   int nwin;           // entries in win
@@ -395,6 +398,40 @@ __device__ void block_stat(Shared<T, NT>& sh, Stat& st, float c) {
   }
 }
 
+// The row's statistics from the parts': one warp of each part reads them. All threads get them.
+template <typename T, int NT>
+__device__ Stat join_stat(Shared<T, NT>& sh, Stat st, float c) {
+  cg::cluster_group cl = cg::this_cluster();
+  const int parts = (int)cl.num_blocks();
+  if (parts == 1) return st;
+  if (threadIdx.x == 0) {
+    sh.pm[0] = st.m;
+    sh.ps[0] = st.s;
+  }
+  cl.sync();
+  if (threadIdx.x < 32) {
+    const int r = threadIdx.x;
+    st.m = -INFINITY;
+    st.s = 0.f;
+    if (r < parts) {
+      const Shared<T, NT>* o = cl.map_shared_rank(&sh, r);
+      st.m = o->pm[0];
+      st.s = o->ps[0];
+    }
+#pragma unroll
+    for (int o = kMaxParts / 2; o > 0; o >>= 1) {
+      const float m2 = __shfl_xor_sync(0xffffffffu, st.m, o), s2 = __shfl_xor_sync(0xffffffffu, st.s, o);
+      stat_merge(st.m, st.s, m2, s2, c);
+    }
+    if (r == 0) {
+      sh.jm = st.m;
+      sh.js = st.s;
+    }
+  }
+  __syncthreads();
+  return {sh.jm, sh.js};
+}
+
 // The row's k largest from the parts' lists: part 0 gets them in sh.win in rank order (sh.nwin of them); every part
 // gets the row's statistics.
 template <typename T, int NT>
@@ -403,32 +440,24 @@ __device__ void join_parts(Shared<T, NT>& sh, int k, float c, Stat& st) {
   cg::cluster_group cl = cg::this_cluster();
   const int parts = (int)cl.num_blocks();
   if (parts > 1) {
-    if (tid == 0) {
-      sh.pm[0] = st.m;
-      sh.ps[0] = st.s;
-    }
-    cl.sync();
-    Stat row;
-    int off[kMaxParts], n = 0;
-#pragma unroll
-    for (int r = 0; r < kMaxParts; ++r) {
-      if (r < parts) {
-        Shared<T, NT>* o = cl.map_shared_rank(&sh, r);
-        stat_merge(row.m, row.s, o->pm[0], o->ps[0], c);
-        off[r] = n;
-        n += o->nwin;
-      }
-    }
-    st = row;
     const bool first = cl.block_rank() == 0;
+    st = join_stat(sh, st, c);
+    int n = 0;
     if (first) {
+      // list r goes behind those before it
+      const int lane = tid & 31, warp = tid >> 5;
+      const int cnt = lane < parts ? cl.map_shared_rank(&sh, lane)->nwin : 0;
+      int incl = cnt;
 #pragma unroll
-      for (int r = 0; r < kMaxParts; ++r) {
-        if (r < parts) {
-          Shared<T, NT>* o = cl.map_shared_rank(&sh, r);
-          const int cnt = (r + 1 < parts ? off[r + 1 < kMaxParts ? r + 1 : r] : n) - off[r];
-          if (tid < cnt) sh.cand()[off[r] + tid] = o->win[tid];
-        }
+      for (int o = 1; o < kMaxParts; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
+      }
+      n = __shfl_sync(0xffffffffu, incl, kMaxParts - 1);
+      for (int r = warp; r < parts; r += NT / 32) {
+        const int at = __shfl_sync(0xffffffffu, incl - cnt, r), len = __shfl_sync(0xffffffffu, cnt, r);
+        const Shared<T, NT>* o = cl.map_shared_rank(&sh, r);
+        for (int i = lane; i < len; i += 32) sh.cand()[at + i] = o->win[i];
       }
     }
     cl.sync();
@@ -494,7 +523,8 @@ TS_DEVICE float lg2(float x) {
 // The race's winner so far among this thread's tokens, by y = z·c - log2 e (log2 of the key, up to the row's
 // constant). y is off by less than margin(y), so what counts in the end is the exact key w / e of the few tokens
 // within the margin of the best. A thread keeps one token: `tie` says that another one came as near, and then the
-// tokens are gone over again with exact keys.
+// tokens are gone over again with exact keys. Threads look only at tokens within the margin of the best that any of
+// the block has seen (sh.ybest, read and written without order: whatever it holds is some token's y).
 struct Race {
   float y = -INFINITY, z = 0.f, e = 1.f;
   int id = -1;
@@ -560,6 +590,8 @@ __device__ __noinline__ void scan_free(Shared<T, NT>& sh, const Slice<T> sl, con
   };
 #pragma unroll
   for (int j = 0; j < R; ++j) fetch(j);
+  if (tid == 0) sh.ybest = -INFINITY;
+  __syncthreads();
   if (tid < sl.head + sl.tail) {
     const int i = tid < sl.head ? tid : sl.nvec * VEC + tid;
     const float z = to_f(sl.p[i]), e = noise[i];
@@ -567,8 +599,7 @@ __device__ __noinline__ void scan_free(Shared<T, NT>& sh, const Slice<T> sl, con
     st.s += sum_exp<1>(&z, st.m, c);
     race.take(fmaf(z, c, -lg2(e)), z, e, sl.lo + i);
   }
-  float least = race.y - Race::margin(race.y);
-  if (race.y == -INFINITY) least = -INFINITY;
+  volatile float* shared_y = &sh.ybest;
   for (int j = 0; j < mine; ++j) {
     copy_wait<R - 1>();
     const uint4* slot = ring + (j % R) * (1 + Q) * NT;
@@ -581,10 +612,12 @@ __device__ __noinline__ void scan_free(Shared<T, NT>& sh, const Slice<T> sl, con
     st.s += sum_exp<VEC>(z, st.m, c);
 #pragma unroll
     for (int q = 0; q < VEC; ++q) y[q] = fmaf(z[q], c, -lg2(e[q]));
+    const float known = *shared_y, least = known - Race::margin(known);
     if (vec_max<VEC>(y) > least) {
 #pragma unroll
-      for (int q = 0; q < VEC; ++q) race.take(y[q], z[q], e[q], sl.lo + sl.head + (j * NT + tid) * VEC + q);
-      least = race.y - Race::margin(race.y);
+      for (int q = 0; q < VEC; ++q)
+        if (y[q] > least) race.take(y[q], z[q], e[q], sl.lo + sl.head + (j * NT + tid) * VEC + q);
+      if (race.y > known) *shared_y = race.y;
     }
   }
   copy_wait<0>();
@@ -659,7 +692,7 @@ __device__ __noinline__ void count_before(Shared<T, NT>& sh, const Slice<T> sl, 
 // The race among the tokens before `bound` with weight min_p at least (none is below zmin). Random numbers are read
 // where a vector holds such a token.
 template <typename T, int NT>
-__device__ __noinline__ void race_before(const Slice<T> sl, const float* __restrict__ noise, float m,
+__device__ __noinline__ void race_before(Shared<T, NT>& sh, const Slice<T> sl, const float* __restrict__ noise, float m,
                                          float temperature, float c, float min_p, float zmin, const Bound& bound,
                                          Race& race) {
   constexpr int VEC = Slice<T>::kVec;
@@ -670,13 +703,15 @@ __device__ __noinline__ void race_before(const Slice<T> sl, const float* __restr
   const float floor = fmaxf(bz, zmin);
   const bool all = !(min_p > 0.f);
   Race r;
-  float least = -INFINITY;
+  volatile float* shared_y = &sh.ybest;
+  if (tid == 0) sh.ybest = -INFINITY;
+  __syncthreads();
   auto one = [&](float z, float e, int id) {
-    const float y = fmaf(z, c, -lg2(e));
-    if (y > least && (z > bz || (z == bz && id < bi)) && z >= zmin &&
+    const float y = fmaf(z, c, -lg2(e)), known = *shared_y;
+    if (y > known - Race::margin(known) && (z > bz || (z == bz && id < bi)) && z >= zmin &&
         (all || weight(z, m, temperature) >= min_p || z == m)) {
       r.take(y, z, e, id);
-      least = r.y - Race::margin(r.y);
+      if (r.y > known) *shared_y = r.y;
     }
   };
   if (tid < sl.head + sl.tail) {
@@ -776,17 +811,33 @@ __device__ void join_keys(Shared<T, NT>& sh, int& turn, int& count, float& mass,
     }
   }
   cl.sync();
-  count = 0;
-  mass = 0.f;
-  best = 0;
-  flag = 0;
-  for (int r = 0; r < (int)cl.num_blocks(); ++r) {
-    Shared<T, NT>* o = cl.map_shared_rank(&sh, r);
-    mass += o->ps[turn];
-    count += o->pcount[turn];
-    best = o->pbest[turn] > best ? o->pbest[turn] : best;
-    flag |= o->pflag[turn];
+  const int parts = (int)cl.num_blocks();
+  if (warp == 0) {
+    count = 0;
+    mass = 0.f;
+    best = 0;
+    flag = 0;
+    if (lane < parts) {
+      const Shared<T, NT>* o = cl.map_shared_rank(&sh, lane);
+      mass = o->ps[turn];
+      count = o->pcount[turn];
+      best = o->pbest[turn];
+      flag = o->pflag[turn];
+    }
+    fold();
+    flag = __reduce_or_sync(0xffffffffu, flag);
+    if (lane == 0) {
+      sh.js = mass;
+      sh.jcount = count;
+      sh.jbest = best;
+      sh.jflag = flag;
+    }
   }
+  __syncthreads();
+  mass = sh.js;
+  count = sh.jcount;
+  best = sh.jbest;
+  flag = sh.jflag;
   turn ^= 1;
 }
 
@@ -835,20 +886,8 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) sample_kernel(const T* 
   if (race_first) {
     scan_free<T, NT>(sh, sl, ns, c, st, race);
     block_stat(sh, st, c);
-    if (parts > 1) {  // the row's statistics
-      if (tid == 0) {
-        sh.pm[0] = st.m;
-        sh.ps[0] = st.s;
-      }
-      cl.sync();
-      Stat all;
-      for (int r = 0; r < parts; ++r) {
-        Shared<T, NT>* o = cl.map_shared_rank(&sh, r);
-        stat_merge(all.m, all.s, o->pm[0], o->ps[0], c);
-      }
-      st = all;
-      turn = 1;
-    }
+    st = join_stat(sh, st, c);
+    turn = 1;
   } else {
     st = scan_slice<T, NT>(sh, sl, k, c);
     block_stat(sh, st, c);
@@ -945,7 +984,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) sample_kernel(const T* 
       if (count == 0 || ((!by_k || count < top_k) && (!by_p || mass < top_p * total))) break;
     }
     race = Race();
-    race_before<T, NT>(sl, ns, m, temperature, c, min_p, zmin, bound, race);
+    race_before<T, NT>(sh, sl, ns, m, temperature, c, min_p, zmin, bound, race);
   }
   if (part == 0 && tid == 0) result(id);
   cl.sync();  // no part leaves while another may still read its shared memory
