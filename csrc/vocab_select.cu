@@ -553,43 +553,60 @@ TS_DEVICE uint64_t race_key(float w, float e, int id) {
   return key >= 0.f ? ((uint64_t)__float_as_uint(key) << 32) | (uint32_t)~(uint32_t)id : 0;
 }
 
-// One pass over logits and random numbers together: statistics and the race among all tokens.
+// One pass over logits and random numbers together: statistics and the race among all tokens. A step is 8 elements of
+// each thread (two vectors of fp32 logits or one of 16-bit ones, and two of random numbers) through its ring. The 32
+// bytes of random numbers beside one 16-bit vector are copied by the warp, 512 bytes at a time: each thread for itself
+// would fetch every 32-byte sector twice.
 template <typename T, int NT>
 __device__ __noinline__ void scan_free(Shared<T, NT>& sh, const Slice<T> sl, const float* __restrict__ noise, float c,
                                        Stat& st_out, Race& race_out) {
+  constexpr int VEC = Slice<T>::kVec, Q = 8 / VEC;
+  constexpr int kPieces = Q + 2;  // 16-byte pieces of a step
+  constexpr int kFit = Shared<T, NT>::kWork / (NT * 16 * kPieces);
+  constexpr int R = kFit < 4 ? kFit : 4;  // steps in flight
+  static_assert(R >= 2, "a ring of two");
+  const int tid = threadIdx.x;
   Stat st;
   Race race;
-  constexpr int VEC = Slice<T>::kVec;
-  constexpr int Q = VEC / 4;  // 16-byte pieces of a vector's random numbers
-  constexpr int kFit = Shared<T, NT>::kWork / (NT * 16 * (1 + Q));
-  constexpr int R = kFit < 6 ? kFit : 6;
-  static_assert(R >= 3, "a ring of three");
-  const int tid = threadIdx.x;
-  const T* body = sl.body();
-  const float* nb = noise + sl.head;
-  uint4* ring = sh.work() + tid;
-  const bool wide = (reinterpret_cast<uintptr_t>(nb) & 15) == 0;
-  const int mine = tid < sl.nvec ? (sl.nvec - tid + NT - 1) / NT : 0;
-  auto fetch = [&](int j) {
-    if (j < mine) {
-      uint4* slot = ring + (j % R) * (1 + Q) * NT;
-      const long long i = (long long)(j * NT + tid) * VEC;
-      copy16(slot, body + i);
+  uint4* const ring = sh.work() + tid;
+  const T* src = sl.body() + tid * VEC;
+  const float* nsrc = noise + sl.head;
+  const bool wide = (reinterpret_cast<uintptr_t>(nsrc) & 15) == 0;
+  const int steps = (sl.nvec + Q * NT - 1) / (Q * NT), whole = sl.nvec / (Q * NT);
+  const int lane = tid & 31, warp0 = tid - lane;
+  auto has = [&](int t, int q) { return (t * Q + q) * NT + tid < sl.nvec; };
+  auto copy_noise = [&](uint4* to, const float* from) {
+    if (wide) {
+      copy16(to, from);
+    } else {
 #pragma unroll
-      for (int q = 0; q < Q; ++q) {
-        uint4* to = slot + (1 + q) * NT;
-        if (wide) {
-          copy16(to, nb + i + 4 * q);
-        } else {
+      for (int w = 0; w < 4; ++w) copy4(reinterpret_cast<float*>(to) + w, from + w);
+    }
+  };
+  // `slot` is the step's place in the ring, at this thread
+  auto fetch = [&](int t, uint4* slot) {
+    if (VEC == 4) {
 #pragma unroll
-          for (int w = 0; w < 4; ++w) copy4(reinterpret_cast<float*>(to) + w, nb + i + 4 * q + w);
+      for (int q = 0; q < 2; ++q) {
+        if (t < whole || (t < steps && has(t, q))) {
+          const long long i = (long long)(t * 2 + q) * (NT * VEC);
+          copy16(slot + q * NT, src + i);
+          copy_noise(slot + (2 + q) * NT, nsrc + i + tid * VEC);
         }
+      }
+    } else {
+      if (t < whole || (t < steps && has(t, 0))) copy16(slot, src + (long long)t * (NT * VEC));
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int v = t * NT + warp0 + q * 16 + lane / 2;  // the vector whose random numbers these are
+        if (t < whole || (t < steps && v < sl.nvec))
+          copy_noise(slot + NT - tid + warp0 * 2 + q * 32 + lane, nsrc + (long long)v * VEC + (lane & 1) * 4);
       }
     }
     copy_commit();
   };
 #pragma unroll
-  for (int j = 0; j < R; ++j) fetch(j);
+  for (int t = 0; t < R; ++t) fetch(t, ring + t * kPieces * NT);
   if (tid == 0) sh.ybest = -INFINITY;
   __syncthreads();
   if (tid < sl.head + sl.tail) {
@@ -600,23 +617,42 @@ __device__ __noinline__ void scan_free(Shared<T, NT>& sh, const Slice<T> sl, con
     race.take(fmaf(z, c, -lg2(e)), z, e, sl.lo + i);
   }
   volatile float* shared_y = &sh.ybest;
-  for (int j = 0; j < mine; ++j) {
+  int place = 0;
+  for (int t = 0; t < steps; ++t) {
     copy_wait<R - 1>();
-    const uint4* slot = ring + (j % R) * (1 + Q) * NT;
-    float z[VEC], e[VEC], y[VEC];
-    unpack<T>(slot[0], z);
+    if (VEC == 8) __syncwarp();
+    uint4* const slot = ring + place * kPieces * NT;
+    float z[8], e[8], y[8];
 #pragma unroll
-    for (int q = 0; q < Q; ++q) unpack<float>(slot[(1 + q) * NT], e + 4 * q);
-    fetch(j + R);
-    stat_raise(st.m, st.s, vec_max<VEC>(z), c);
-    st.s += sum_exp<VEC>(z, st.m, c);
+    for (int q = 0; q < Q; ++q) unpack<T>(slot[q * NT], z + q * VEC);
 #pragma unroll
-    for (int q = 0; q < VEC; ++q) y[q] = fmaf(z[q], c, -lg2(e[q]));
+    for (int q = 0; q < 2; ++q)
+      unpack<float>(VEC == 4 ? slot[(2 + q) * NT] : slot[NT + tid + q], e + 4 * q);
+    if (VEC == 8) __syncwarp();
+    if (t >= whole) {
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        if (!has(t, q)) {
+#pragma unroll
+          for (int x = 0; x < VEC; ++x) {
+            z[q * VEC + x] = -INFINITY;  // (y is then -inf too, which never wins)
+            e[q * VEC + x] = 1.f;
+          }
+        }
+      }
+    }
+    fetch(t + R, slot);
+    place = place + 1 == R ? 0 : place + 1;
+    stat_raise(st.m, st.s, vec_max<8>(z), c);
+    st.s += sum_exp<8>(z, st.m, c);
+#pragma unroll
+    for (int x = 0; x < 8; ++x) y[x] = fmaf(z[x], c, -lg2(e[x]));
     const float known = *shared_y, least = known - Race::margin(known);
-    if (vec_max<VEC>(y) > least) {
+    if (vec_max<8>(y) > least) {
 #pragma unroll
-      for (int q = 0; q < VEC; ++q)
-        if (y[q] > least) race.take(y[q], z[q], e[q], sl.lo + sl.head + (j * NT + tid) * VEC + q);
+      for (int x = 0; x < 8; ++x)
+        if (y[x] > least)
+          race.take(y[x], z[x], e[x], sl.lo + sl.head + ((t * Q + x / VEC) * NT + tid) * VEC + x % VEC);
       if (race.y > known) *shared_y = race.y;
     }
   }
