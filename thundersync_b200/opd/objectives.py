@@ -17,6 +17,8 @@ per group through the run's boundary cut.
   arrive (``StreamingRun(turn_boundary_rebuild=True)`` cuts each turn's
   outgoing state) and replays the deferred state adjoints in reverse at
   trajectory close.
+* :func:`teacher_topk_logprobs` and :func:`topk_distillation_losses` distil from the teacher's most likely tokens at
+  each scored position instead of its log-prob of the sampled one (no stream: one trajectory, one graph).
 * :class:`OPDStream` backwards a whole trajectory at its close; the teacher
   scores are either given or computed by an optional teacher model, which may
   live on a second GPU and run concurrently.
@@ -32,9 +34,10 @@ from typing import Any
 import torch
 
 from thundersync_b200.engine.layers import Executor, Segment
-from thundersync_b200.ops.logprob import lm_head_logprob
+from thundersync_b200.ops.distill import lm_head_topk_distill, topk_logprobs
+from thundersync_b200.ops.logprob import _logits_fp32, lm_head_logprob
 
-__all__ = ["OPDStream", "OPDTurnStream", "teacher_logprobs"]
+__all__ = ["OPDStream", "OPDTurnStream", "teacher_logprobs", "teacher_topk_logprobs", "topk_distillation_losses"]
 
 _NORMALIZATIONS = ("token_mean", "sum")
 
@@ -301,23 +304,60 @@ class OPDTurnStream(_TokenLoss, _ImmediateBackward):
         self._finalized = True
 
 
-def teacher_logprobs(teacher: torch.nn.Module, prompt: list[int], turns: list[tuple[list[int], list[bool]]],
-                     *, device: torch.device | None = None) -> torch.Tensor:
-    """The frozen teacher's fp32 log-probs of every scored turn token (no graph)."""
-    dev = device or next(teacher.parameters()).device
+def _scored_rows(model: torch.nn.Module, prompt: list[int], turns: list[tuple[list[int], list[bool]]],
+                 device: torch.device | None):
+    """(hidden states [n, D] that predict the scored turn tokens, those tokens, LM-head weight); the first two are None
+    where nothing is scored."""
+    dev = device or next(model.parameters()).device
     toks = list(prompt) + [t for tk, _ in turns for t in tk]
     scored = [False] * len(prompt) + [bool(s) for _, sc in turns for s in sc]
     ids = torch.tensor(toks, device=dev)
     pos = torch.arange(len(toks), device=dev)
+    ex = Executor(model)
+    h, _ = ex.run(ids, pos, [Segment(0, len(toks), [])])
+    idx = [i for i, s in enumerate(scored) if s and i > 0]
+    if not idx:
+        return None, None, ex.head_weight()
+    src = torch.tensor([i - 1 for i in idx], device=dev)
+    tgt = torch.tensor([toks[i] for i in idx], device=dev)
+    return h.index_select(0, src), tgt, ex.head_weight()
+
+
+def teacher_logprobs(teacher: torch.nn.Module, prompt: list[int], turns: list[tuple[list[int], list[bool]]],
+                     *, device: torch.device | None = None) -> torch.Tensor:
+    """The frozen teacher's fp32 log-probs of every scored turn token (no graph)."""
     with torch.no_grad():
-        ex = Executor(teacher)
-        h, _ = ex.run(ids, pos, [Segment(0, len(toks), [])])
-        idx = [i for i, s in enumerate(scored) if s and i > 0]
-        if not idx:
-            return torch.zeros(0, dtype=torch.float32, device=dev)
-        src = torch.tensor([i - 1 for i in idx], device=dev)
-        tgt = torch.tensor([toks[i] for i in idx], device=dev)
-        return lm_head_logprob(h.index_select(0, src), ex.head_weight(), tgt)
+        h, tgt, w = _scored_rows(teacher, prompt, turns, device)
+        if h is None:
+            return torch.zeros(0, dtype=torch.float32, device=w.device)
+        return lm_head_logprob(h, w, tgt)
+
+
+def teacher_topk_logprobs(teacher: torch.nn.Module, prompt: list[int], turns: list[tuple[list[int], list[bool]]],
+                          k: int, *, temperature: float = 1.0, device: torch.device | None = None,
+                          rows: int = 1024) -> tuple[torch.Tensor, torch.Tensor]:
+    """The frozen teacher's ``k`` most likely tokens at every scored position (no graph): ids int64 [n, k] and fp32
+    log-probs [n, k] at ``temperature``, most likely first. Logits exist for ``rows`` positions at a time."""
+    with torch.no_grad():
+        h, _, w = _scored_rows(teacher, prompt, turns, device)
+        if h is None:
+            return (torch.zeros(0, k, dtype=torch.int64, device=w.device),
+                    torch.zeros(0, k, dtype=torch.float32, device=w.device))
+        parts = [topk_logprobs(_logits_fp32(x, w), k, temperature=temperature) for x in h.split(rows)]
+        return torch.cat([p[0] for p in parts]), torch.cat([p[1] for p in parts])
+
+
+def topk_distillation_losses(student: torch.nn.Module, prompt: list[int], turns: list[tuple[list[int], list[bool]]],
+                             teacher_ids: torch.Tensor, teacher_logprobs: torch.Tensor, *, temperature: float = 1.0,
+                             direction: str = "forward", tail: bool = True) -> torch.Tensor:
+    """Loss [n] of the student at every scored position against the teacher's entries there
+    (:func:`teacher_topk_logprobs`), with its graph; ``direction`` and ``tail`` as in
+    :func:`thundersync_b200.ops.distill.lm_head_topk_distill`."""
+    h, _, w = _scored_rows(student, prompt, turns, None)
+    if h is None:
+        return torch.zeros(0, dtype=torch.float32, device=w.device)
+    return lm_head_topk_distill(h, w, teacher_ids, teacher_logprobs, temperature=temperature, direction=direction,
+                                tail=tail)
 
 
 class OPDStream(_TokenLoss, _ImmediateBackward):
