@@ -2,7 +2,8 @@
 // slices of the vocabulary, dW = dᵀ h.
 //
 // CTA pairs (cta_group::2): a cluster of two CTAs computes a 256 x 256 tile, each staging 128 rows of A and 128 of B
-// per 64-deep K block through a six-stage TMA ring:
+// per 64-deep K block through a six-stage TMA ring. Where too many of such tiles' rows would be past the last one,
+// single CTAs compute 128 x 256 tiles, each staging 128 rows of A and 256 of B through four stages.
 //   warp 0  TMA producer, warp 1 MMA issuer (one lane each; the even CTA issues for the pair), warps 2-3 idle
 //   warps 4-11  epilogue: two warps for each 32-row slab of tensor memory, half of the tile's columns each
 // The contraction is accumulated in chunks of 512: tensor memory holds one chunk's sum (two buffers, used in turn),
@@ -23,17 +24,23 @@ namespace {
 
 using namespace vocab;
 
-constexpr int kBM = 128, kBN = 256, kBK = 64, kStages = 6;
+constexpr int kBM = 128, kBN = 256, kBK = 64;
 constexpr int kChunkLogits = 4, kChunkGrad = 32;           // K blocks of a chunk
-constexpr uint32_t kABytes = kBM * kBK * 2;                // 16 KB of A ...
-constexpr uint32_t kStageBytes = kABytes + 128 * kBK * 2;  // ... and 16 KB of B per CTA and K block
+constexpr uint32_t kABytes = kBM * kBK * 2;  // 16 KB
+template <bool PAIR>
+struct Ring {
+  static constexpr int kStages = PAIR ? 6 : 4;
+  static constexpr int kBRows = PAIR ? 128 : 256;  // of B in each CTA
+  static constexpr uint32_t kStageBytes = kABytes + kBRows * kBK * 2;
+  static_assert(kStages * kStageBytes == 6 * 32768, "the rings take the same room");
+};
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 128 + 32 * kEpiWarps;
 // Registers of a thread after the split of the block's (384 threads x 168 at launch): the first warpgroup gives, the
 // epilogue's two take. 128 x 56 + 256 x 224 is the launch's 64,512.
 constexpr int kRegsLaunch = 168, kRegsGive = 56, kRegsTake = 224;
 static_assert(128 * kRegsGive + 32 * kEpiWarps * kRegsTake <= kThreads * kRegsLaunch, "no more registers than launched");
-constexpr uint32_t kEpiOff = kStages * kStageBytes;        // 4 KB of staging for each epilogue warp
+constexpr uint32_t kEpiOff = 6 * 32768;  // 4 KB of staging for each epilogue warp
 constexpr uint32_t kBarOff = kEpiOff + kEpiWarps * 4096;
 constexpr uint32_t kSmem = kBarOff + 256 + 1024;
 static_assert(kSmem <= 232448, "shared memory");
@@ -41,13 +48,14 @@ static_assert(kSmem <= 232448, "shared memory");
 enum Out { kNone = 0, kF32 = 1, kBf16 = 2 };
 
 struct Bars {
-  uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2];
+  uint64_t full[6], empty[6], acc_full[2], acc_empty[2];
   uint32_t tmem_slot;
   int abort;
 };
 
 struct Shape {
   int m, n, k;      // C [m, n] = A [m, k] B [k, n]
+  int tile;         // rows of a unit's tile: 256 (pairs) or 128
   int splits;       // slices of the contraction, one unit of work each
   int split_rows;   // rows of C between two slices' outputs
 };
@@ -59,7 +67,7 @@ struct Work {
 // Unit u: slices outermost, so that what runs at one time reads the same part of both operands; then groups of eight
 // row blocks, which share B's columns.
 TS_DEVICE Work work_of(const Shape& s, int u) {
-  const int mt = (s.m + 2 * kBM - 1) / (2 * kBM), nt = (s.n + kBN - 1) / kBN, kt = (s.k + kBK - 1) / kBK;
+  const int mt = (s.m + s.tile - 1) / s.tile, nt = (s.n + kBN - 1) / kBN, kt = (s.k + kBK - 1) / kBK;
   const int z = u / (mt * nt), t = u % (mt * nt);
   const int group = t / (8 * nt), r = t % (8 * nt), first = group * 8, gm = min(8, mt - first);
   Work w;
@@ -78,7 +86,7 @@ TS_DEVICE void store_tile(const CUtensorMap* map, uint32_t src, int x, int y) {
                : "memory");
   asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
 }
-template <int N> TS_DEVICE void store_read_wait() { asm volatile("cp.async.bulk.wait_group.read %0;\n" ::"n"(N) : "memory"); }
+TS_DEVICE void store_read_wait() { asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory"); }
 TS_DEVICE void store_wait() { asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory"); }
 
 TS_DEVICE uint32_t pack2(float lo, float hi) {
@@ -86,34 +94,29 @@ TS_DEVICE uint32_t pack2(float lo, float hi) {
   return *reinterpret_cast<uint32_t*>(&v);
 }
 
-// This lane's 32 values (row `lane`) of a 32 x 32 chunk at (col, row0), through the warp's 4 KB of staging: rows of 128
-// bytes (fp32, one buffer) or 64 (bf16, two in turn) in the output map's swizzle, which keeps the writes of 32 rows
-// apart in the banks. `n` chunks were stored before.
+// This lane's values (row `lane`) of a chunk of 32 rows of 128 bytes (32 fp32 or 64 bf16) at (col, row0), through the
+// warp's 4 KB of staging in the output map's 128-byte swizzle, which keeps the writes of 32 rows apart in the banks.
+// bf16 chunks of 64-byte rows took the output of a short contraction (97 rows' dW) 0.24 ms.
 template <int OUT>
-TS_DEVICE void store_chunk(uint32_t buf, int& n, const CUtensorMap* map, const float* o, int col, int row0) {
+TS_DEVICE void store_chunk(uint32_t buf, bool& busy, const CUtensorMap* map, const float* o, int col, int row0) {
   const int lane = threadIdx.x & 31;
-  constexpr int kBufs = OUT == kBf16 ? 2 : 1;
-  if (n >= kBufs) {  // the store that used this buffer has read it
-    if (lane == 0) store_read_wait<kBufs - 1>();
+  if (busy) {  // the store before has read the buffer
+    if (lane == 0) store_read_wait();
     __syncwarp();
   }
-  if (kBufs == 2) buf += (uint32_t)(n & 1) * 2048;
-  ++n;
-  if constexpr (OUT == kF32) {
-    const uint32_t rowb = buf + (uint32_t)lane * 128;
+  busy = true;
+  const uint32_t rowb = buf + (uint32_t)lane * 128;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};\n" ::"r"(rowb + (uint32_t)((j ^ (lane & 7)) << 4)),
-                   "f"(o[4 * j]), "f"(o[4 * j + 1]), "f"(o[4 * j + 2]), "f"(o[4 * j + 3])
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t at = rowb + (uint32_t)((j ^ (lane & 7)) << 4);
+    if constexpr (OUT == kF32) {
+      asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};\n" ::"r"(at), "f"(o[4 * j]), "f"(o[4 * j + 1]),
+                   "f"(o[4 * j + 2]), "f"(o[4 * j + 3])
                    : "memory");
-    }
-  } else {
-    const uint32_t rowb = buf + (uint32_t)lane * 64;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(rowb + (uint32_t)((j ^ ((lane >> 1) & 3)) << 4)),
-                   "r"(pack2(o[8 * j], o[8 * j + 1])), "r"(pack2(o[8 * j + 2], o[8 * j + 3])),
-                   "r"(pack2(o[8 * j + 4], o[8 * j + 5])), "r"(pack2(o[8 * j + 6], o[8 * j + 7]))
+    } else {
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(at), "r"(pack2(o[8 * j], o[8 * j + 1])),
+                   "r"(pack2(o[8 * j + 2], o[8 * j + 3])), "r"(pack2(o[8 * j + 4], o[8 * j + 5])),
+                   "r"(pack2(o[8 * j + 6], o[8 * j + 7]))
                    : "memory");
     }
   }
@@ -134,8 +137,8 @@ TS_DEVICE int first_entry(const int* __restrict__ ids, int k, int col) {
   return lo;
 }
 
-template <bool A_MN, bool B_MN, int OUT, bool STATS, int kChunk>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+template <bool A_MN, bool B_MN, int OUT, bool STATS, int kChunk, bool PAIR>
+__global__ void __launch_bounds__(kThreads, 1)
     head_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                      const __grid_constant__ CUtensorMap tm_c, Shape shape, HeadStats st, int* __restrict__ err) {
   extern __shared__ uint8_t smem_raw[];
@@ -143,9 +146,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   Bars* bars = reinterpret_cast<Bars*>(smem + kBarOff);
   const uint32_t sbase = tc::smem_addr(smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = tc::cluster_rank();
-  const int units = ((shape.m + 2 * kBM - 1) / (2 * kBM)) * ((shape.n + kBN - 1) / kBN) * shape.splits;
-  const int cid = blockIdx.x >> 1, ncl = gridDim.x >> 1;
+  constexpr int kStages = Ring<PAIR>::kStages;
+  constexpr uint32_t kStageBytes = Ring<PAIR>::kStageBytes;
+  constexpr int kTileM = PAIR ? 2 * kBM : kBM;
+  const uint32_t rank = PAIR ? tc::cluster_rank() : 0;
+  const int units = ((shape.m + kTileM - 1) / kTileM) * ((shape.n + kBN - 1) / kBN) * shape.splits;
+  const int cid = PAIR ? blockIdx.x >> 1 : blockIdx.x, ncl = PAIR ? gridDim.x >> 1 : gridDim.x;
   volatile int* abort = &bars->abort;
 
   if (threadIdx.x == 0) {
@@ -155,15 +161,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       tc::mbar_init(&bars->acc_full[b], 1);
-      tc::mbar_init(&bars->acc_empty[b], 2 * kEpiWarps);  // the epilogue warps of both CTAs
+      tc::mbar_init(&bars->acc_empty[b], (PAIR ? 2 : 1) * kEpiWarps);  // the epilogue warps (of both CTAs)
     }
     bars->abort = 0;
     tc::fence_barrier_init();
   }
-  if (warp == 1) tc::tmem_alloc_pair(&bars->tmem_slot, 512);
+  if (warp == 1) {
+    if constexpr (PAIR) tc::tmem_alloc_pair(&bars->tmem_slot, 512);
+    else tc::tmem_alloc(&bars->tmem_slot, 512);
+  }
   tc::tc_fence_before();
   __syncthreads();
-  tc::cluster_sync();  // both CTAs' barriers exist before any remote arrive or byte count
+  if constexpr (PAIR) tc::cluster_sync();  // both CTAs' barriers exist before any remote arrive or byte count
   tc::tc_fence_after();
   const uint32_t tmem = bars->tmem_slot;
 
@@ -176,27 +185,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         int it = 0;
         for (int u = cid; u < units; u += ncl) {
           const Work w = work_of(shape, u);
-          const int arow = w.mb * 2 * kBM + (int)rank * kBM, bcol = w.nb * kBN + (int)rank * (kBN / 2);
+          const int arow = w.mb * kTileM + (int)rank * kBM, bcol = w.nb * kBN + (int)rank * (kBN / 2);
           for (int kb = w.kb0; kb < w.kb1; ++kb, ++it) {
             const int s = it % kStages;
             if (it >= kStages && !tc::mbar_wait(&bars->empty[s], ((it - kStages) / kStages) & 1, abort, err, 301))
               goto producer_done;
-            if (rank == 0) tc::mbar_expect_tx(&bars->full[s], 2 * kStageBytes);
-            const uint32_t full0 = tc::map_cluster(tc::smem_addr(&bars->full[s]), 0);
+            uint64_t* full = &bars->full[s];
+            if (rank == 0) tc::mbar_expect_tx(full, (PAIR ? 2 : 1) * kStageBytes);
+            const uint32_t full0 = PAIR ? tc::map_cluster(tc::smem_addr(full), 0) : 0;
+            auto load = [&](uint8_t* to, const CUtensorMap* map, int x, int y) {
+              if constexpr (PAIR) tc::tma_load_2d_pair(to, map, x, y, full0);
+              else tc::tma_load_2d(to, map, x, y, full);
+            };
             uint8_t* a = smem + s * kStageBytes;
             uint8_t* b = a + kABytes;
             const int kx = kb * kBK;
             if constexpr (!A_MN) {
-              tc::tma_load_2d_pair(a, &tm_a, kx, arow, full0);  // box 64 (k) x 128 (m)
+              load(a, &tm_a, kx, arow);  // box 64 (k) x 128 (m)
             } else {
-              tc::tma_load_2d_pair(a, &tm_a, arow, kx, full0);  // [K][M]: two boxes of 64 m x 64 k
-              tc::tma_load_2d_pair(a + 64 * 128, &tm_a, arow + 64, kx, full0);
+#pragma unroll
+              for (int j = 0; j < kBM / 64; ++j) load(a + j * 64 * 128, &tm_a, arow + j * 64, kx);  // [K][M]: 64 m x 64 k
             }
             if constexpr (!B_MN) {
-              tc::tma_load_2d_pair(b, &tm_b, kx, bcol, full0);  // box 64 (k) x 128 (n)
+#pragma unroll
+              for (int j = 0; j < Ring<PAIR>::kBRows / 128; ++j)
+                load(b + j * 128 * 128, &tm_b, kx, bcol + j * 128);  // box 64 (k) x 128 (n)
             } else {
-              tc::tma_load_2d_pair(b, &tm_b, bcol, kx, full0);  // [K][N]: two boxes of 64 n x 64 k
-              tc::tma_load_2d_pair(b + 64 * 128, &tm_b, bcol + 64, kx, full0);
+#pragma unroll
+              for (int j = 0; j < Ring<PAIR>::kBRows / 64; ++j)
+                load(b + j * 64 * 128, &tm_b, bcol + j * 64, kx);  // [K][N]: 64 n x 64 k
             }
           }
         }
@@ -204,7 +221,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
     } else if (warp == 1) {
       if (lane == 0 && rank == 0) {
-        const uint32_t idesc = tc::idesc_bf16(2 * kBM, kBN, A_MN, B_MN);
+        const uint32_t idesc = tc::idesc_bf16(kTileM, kBN, A_MN, B_MN);
         int it = 0, chunk = 0;
         bool ok = true;
         for (int u = cid; ok && u < units; u += ncl) {
@@ -232,11 +249,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                                          : tc::sdesc_sw128(a + kk * 32, 16, 1024);
                 const uint64_t bd = B_MN ? tc::sdesc_sw128(b + kk * 16 * 128, 64 * 128, 1024)
                                          : tc::sdesc_sw128(b + kk * 32, 16, 1024);
-                tc::mma_bf16_pair(acc, ad, bd, idesc, kb > kc || kk > 0);
+                if constexpr (PAIR) tc::mma_bf16_pair(acc, ad, bd, idesc, kb > kc || kk > 0);
+                else tc::mma_bf16(acc, ad, bd, idesc, kb > kc || kk > 0);
               }
-              tc::mma_commit_pair(&bars->empty[s]);
+              if constexpr (PAIR) tc::mma_commit_pair(&bars->empty[s]);
+              else tc::mma_commit(&bars->empty[s]);
             }
-            if (ok) tc::mma_commit_pair(&bars->acc_full[buf]);
+            if (ok) {
+              if constexpr (PAIR) tc::mma_commit_pair(&bars->acc_full[buf]);
+              else tc::mma_commit(&bars->acc_full[buf]);
+            }
           }
         }
       }
@@ -246,14 +268,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int sub = warp & 3;            // the 32-row slab of tensor memory that this warp can read
     const int ew = warp - 4, half = ew >> 2;  // and its half of the tile's columns
     const uint32_t lane_base = tmem + ((uint32_t)(sub * 32) << 16) + half * (kBN / 2);
-    const uint32_t acc_empty0 = tc::map_cluster(tc::smem_addr(&bars->acc_empty[0]), 0);
-    const uint32_t acc_empty1 = tc::map_cluster(tc::smem_addr(&bars->acc_empty[1]), 0);
+    const uint32_t acc_empty0 = PAIR ? tc::map_cluster(tc::smem_addr(&bars->acc_empty[0]), 0) : 0;
+    const uint32_t acc_empty1 = PAIR ? tc::map_cluster(tc::smem_addr(&bars->acc_empty[1]), 0) : 0;
     const uint32_t stage = sbase + kEpiOff + (uint32_t)ew * 4096;
     bool ok = true;
-    int chunk = 0, stored = 0;
+    int chunk = 0;
+    bool busy = false;
     for (int u = cid; ok && u < units; u += ncl) {
       const Work w = work_of(shape, u);
-      const int row0 = w.mb * 2 * kBM + (int)rank * kBM + sub * 32, row = row0 + lane;
+      const int row0 = w.mb * kTileM + (int)rank * kBM + sub * 32, row = row0 + lane;
       const int col0 = w.nb * kBN + half * (kBN / 2);
       int at = 0, next = 0x7fffffff;  // the row's next entry
       const int* ids = nullptr;
@@ -289,7 +312,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
         tc::tc_fence_before();
         __syncwarp();
-        if (lane == 0) tc::mbar_arrive_cluster(buf ? acc_empty1 : acc_empty0);
+        if (lane == 0) {
+          if constexpr (PAIR) tc::mbar_arrive_cluster(buf ? acc_empty1 : acc_empty0);
+          else tc::mbar_arrive(&bars->acc_empty[buf]);
+        }
       }
       if (!ok) break;
       if (row0 >= shape.m) continue;  // the same in the whole warp
@@ -299,7 +325,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const int col = col0 + g * 32;
         float* v = acc + g * 32;
         if (col < shape.n) {
-          if constexpr (OUT != kNone) store_chunk<OUT>(stage, stored, &tm_c, v, col, w.row_off + row0);
+          if constexpr (OUT == kF32) store_chunk<OUT>(stage, busy, &tm_c, v, col, w.row_off + row0);
+          if constexpr (OUT == kBf16) {
+            if (g % 2 == 0) store_chunk<OUT>(stage, busy, &tm_c, v, col, w.row_off + row0);
+          }
           if constexpr (STATS) {
             // the entries' logits go to their places and out of the sums
             uint32_t hit = 0;
@@ -343,10 +372,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   }
   tc::tc_fence_before();
   __syncthreads();
-  tc::cluster_sync();  // no CTA leaves while its pair may still read its shared memory or arrive on it
+  if constexpr (PAIR) tc::cluster_sync();  // no CTA leaves while its pair may still read its shared memory or arrive on it
   if (warp == 1) {
     tc::tc_fence_after();
-    tc::tmem_dealloc_pair(tmem, 512);
+    if constexpr (PAIR) tc::tmem_dealloc_pair(tmem, 512);
+    else tc::tmem_dealloc(tmem, 512);
   }
 }
 
@@ -366,48 +396,75 @@ __global__ void __launch_bounds__(256) sum_slices_kernel(const float* __restrict
   }
 }
 
-// Pairs of CTAs that the device holds at one time (the persistent grid).
-template <bool A_MN, bool B_MN, int OUT, bool STATS, int kChunk>
-cudaError_t resident_pairs(const VocabLaunch& l, int& pairs) {
+template <bool PAIR>
+void fill_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute& attr, int ctas, cudaStream_t stream) {
+  cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = stream;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = PAIR ? 2 : 1;
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+}
+
+// Pairs of CTAs (or CTAs) that the device holds at one time: the persistent grid.
+template <bool A_MN, bool B_MN, int OUT, bool STATS, int kChunk, bool PAIR>
+cudaError_t resident(const VocabLaunch& l, int& held) {
   static int have[16] = {0};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   int& n = have[dev & 15];
   if (n == 0) {
-    const auto kernel = head_gemm_kernel<A_MN, B_MN, OUT, STATS, kChunk>;
+    const auto kernel = head_gemm_kernel<A_MN, B_MN, OUT, STATS, kChunk, PAIR>;
     e = l.set_smem((const void*)kernel, (int)kSmem);
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(2 * l.sms);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = kSmem;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = 2;
-    attr.val.clusterDim.y = 1;
-    attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    int most = 0;
-    e = cudaOccupancyMaxActiveClusters(&most, kernel, &cfg);
-    if (e != cudaSuccess) return e;
-    n = std::max(1, std::min(most, l.sms / 2));
+    if (PAIR) {
+      cudaLaunchConfig_t cfg;
+      cudaLaunchAttribute attr;
+      fill_config<PAIR>(cfg, attr, 2 * l.sms, 0);
+      int most = 0;
+      e = cudaOccupancyMaxActiveClusters(&most, kernel, &cfg);
+      if (e != cudaSuccess) return e;
+      n = std::max(1, std::min(most, l.sms / 2));
+    } else {
+      n = l.sms;  // one CTA an SM
+    }
   }
-  pairs = n;
+  held = n;
   return cudaSuccess;
+}
+
+template <bool A_MN, bool B_MN, int OUT, bool STATS, int kChunk, bool PAIR>
+cudaError_t launch_as(const VocabLaunch& l, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& c,
+                      Shape shape, const HeadStats& st, int* err) {
+  shape.tile = PAIR ? 2 * kBM : kBM;
+  int held = 0;
+  const cudaError_t e = resident<A_MN, B_MN, OUT, STATS, kChunk, PAIR>(l, held);
+  if (e != cudaSuccess) return e;
+  const int units = ((shape.m + shape.tile - 1) / shape.tile) * ((shape.n + kBN - 1) / kBN) * shape.splits;
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attr;
+  fill_config<PAIR>(cfg, attr, (PAIR ? 2 : 1) * std::min(units, held), l.stream);
+  return cudaLaunchKernelEx(&cfg, head_gemm_kernel<A_MN, B_MN, OUT, STATS, kChunk, PAIR>, a, b, c, shape, st, err);
+}
+
+// Pairs or single CTAs: a pair's tile takes 7% less time a row (logits of 2048 rows 1.25 ms, of single CTAs 1.35) but
+// rounds the rows up to 256 instead of 128 (97 rows 0.225 / 0.176 ms, 300 0.32 / 0.27, 600 0.47 / 0.43).
+bool in_pairs(int rows) {
+  const int pairs = (rows + 255) / 256 * 256, single = (rows + 127) / 128 * 128;
+  return 100ll * single >= 93ll * pairs;
 }
 
 template <bool A_MN, bool B_MN, int OUT, bool STATS, int kChunk>
 cudaError_t launch(const VocabLaunch& l, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& c,
                    const Shape& shape, const HeadStats& st, int* err) {
-  const auto kernel = head_gemm_kernel<A_MN, B_MN, OUT, STATS, kChunk>;
-  int pairs = 0;
-  const cudaError_t e = resident_pairs<A_MN, B_MN, OUT, STATS, kChunk>(l, pairs);
-  if (e != cudaSuccess) return e;
-  const int units = ((shape.m + 2 * kBM - 1) / (2 * kBM)) * ((shape.n + kBN - 1) / kBN) * shape.splits;
-  kernel<<<2 * std::min(units, pairs), kThreads, kSmem, l.stream>>>(a, b, c, shape, st, err);
-  return cudaGetLastError();
+  if (in_pairs(shape.m)) return launch_as<A_MN, B_MN, OUT, STATS, kChunk, true>(l, a, b, c, shape, st, err);
+  return launch_as<A_MN, B_MN, OUT, STATS, kChunk, false>(l, a, b, c, shape, st, err);
 }
 
 }  // namespace
@@ -416,13 +473,17 @@ int head_parts(int v) { return 2 * ((v + kBN - 1) / kBN); }
 
 // Slices of dH's contraction over the vocabulary: the fewest that fill the pairs' rounds to 95%, or the fullest.
 int head_splits(const VocabLaunch& l, int rows, int d, int v) {
+  const bool two = in_pairs(rows);
   int pairs = 0;
-  if (resident_pairs<false, true, kF32, false, kChunkGrad>(l, pairs) != cudaSuccess) return 1;
-  const int tiles = ((rows + 2 * kBM - 1) / (2 * kBM)) * ((d + kBN - 1) / kBN);
+  const cudaError_t e = two ? resident<false, true, kF32, false, kChunkGrad, true>(l, pairs)
+                            : resident<false, true, kF32, false, kChunkGrad, false>(l, pairs);
+  if (e != cudaSuccess) return 1;
+  const int tile = two ? 2 * kBM : kBM;
+  const int tiles = ((rows + tile - 1) / tile) * ((d + kBN - 1) / kBN);
   const int kt = (v + kBK - 1) / kBK;
   int best = 1;
   double full = 0.0;
-  for (int s = 1; s <= 16 && kt / s >= 32; ++s) {
+  for (int s = 1; s <= 32 && kt / s >= 32; ++s) {
     const int units = tiles * s, rounds = (units + pairs - 1) / pairs;
     const double f = (double)units / ((double)rounds * pairs);
     if (f > full + 1e-9) {
@@ -436,19 +497,19 @@ int head_splits(const VocabLaunch& l, int rows, int d, int v) {
 
 cudaError_t head_logits(const VocabLaunch& l, const CUtensorMap& h, const CUtensorMap& w, const CUtensorMap* out,
                         int rows, int d, int v, const HeadStats& st, int* err) {
-  const Shape s{rows, v, d, 1, 0};
+  const Shape s{rows, v, d, 0, 1, 0};
   if (out != nullptr) return launch<false, false, kF32, true, kChunkLogits>(l, h, w, *out, s, st, err);
   return launch<false, false, kNone, true, kChunkLogits>(l, h, w, h, s, st, err);
 }
 
 cudaError_t head_logits_again(const VocabLaunch& l, const CUtensorMap& h, const CUtensorMap& w, const CUtensorMap& out,
                               int rows, int d, int v, int* err) {
-  return launch<false, false, kF32, false, kChunkLogits>(l, h, w, out, Shape{rows, v, d, 1, 0}, HeadStats{}, err);
+  return launch<false, false, kF32, false, kChunkLogits>(l, h, w, out, Shape{rows, v, d, 0, 1, 0}, HeadStats{}, err);
 }
 
 cudaError_t head_dh(const VocabLaunch& l, const CUtensorMap& dl, const CUtensorMap& w, const CUtensorMap& out, int rows,
                     int d, int v, int splits, int split_rows, const float* parts, void* dh, int* err) {
-  const Shape s{rows, d, v, splits, split_rows};
+  const Shape s{rows, d, v, 0, splits, split_rows};
   if (splits == 1) return launch<false, true, kBf16, false, kChunkGrad>(l, dl, w, out, s, HeadStats{}, err);
   const cudaError_t e = launch<false, true, kF32, false, kChunkGrad>(l, dl, w, out, s, HeadStats{}, err);
   if (e != cudaSuccess) return e;
@@ -460,7 +521,7 @@ cudaError_t head_dh(const VocabLaunch& l, const CUtensorMap& dl, const CUtensorM
 
 cudaError_t head_dw(const VocabLaunch& l, const CUtensorMap& dl, const CUtensorMap& h, const CUtensorMap& out, int rows,
                     int d, int v, int* err) {
-  return launch<true, true, kBf16, false, kChunkGrad>(l, dl, h, out, Shape{v, d, rows, 1, 0}, HeadStats{}, err);
+  return launch_as<true, true, kBf16, false, kChunkGrad, true>(l, dl, h, out, Shape{v, d, rows, 0, 1, 0}, HeadStats{}, err);
 }
 
 }  // namespace ts

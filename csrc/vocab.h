@@ -73,7 +73,7 @@ cudaError_t distill_head_finish(const VocabLaunch& l, const HeadStats& st, const
                                 bool reverse, bool tail, const DistillOut& out);
 
 // Products of the head (csrc/head_tc.cu). Operand maps: bf16, boxes of 64 along the contiguous dimension and 128 rows
-// (64 where the contraction is not the contiguous dimension); output maps: boxes of 32 x 32.
+// (64 where the contraction is not the contiguous dimension); output maps: boxes of 32 rows of 128 bytes.
 int head_parts(int v);
 int head_splits(const VocabLaunch& l, int rows, int d, int v);
 cudaError_t head_logits(const VocabLaunch& l, const CUtensorMap& h, const CUtensorMap& w, const CUtensorMap* out,

@@ -183,8 +183,9 @@ CUtensorMap k_rows(const at::Tensor& t) {  // [rows, k], the contraction along t
 CUtensorMap k_cols(const at::Tensor& t) {  // [k, cols], the contraction down the columns
   return make_bf16_map(t.data_ptr(), t.size(1), t.size(0), t.size(1), 64);
 }
-CUtensorMap out_map(const at::Tensor& t) {
-  return make_out_map(t.data_ptr(), t.scalar_type() == at::kFloat, t.size(1), t.size(0), t.size(1));
+CUtensorMap out_map(const at::Tensor& t) {  // boxes of 32 rows of 128 bytes
+  if (t.scalar_type() == at::kFloat) return make_out_map(t.data_ptr(), true, t.size(1), t.size(0), t.size(1));
+  return make_bf16_map(t.data_ptr(), t.size(1), t.size(0), t.size(1), 32);
 }
 
 }  // namespace
