@@ -29,6 +29,7 @@ constexpr int kMaxTop = 256;
 constexpr int kMaxParts = 8;
 constexpr int kGroups = 4096;                // groups of a slice whose maxima are kept
 constexpr int kMaxList = 512;                // groups that are read again, at most
+constexpr int kMaxRounds = 40;               // winners of a race that are tried before the kept tokens are looked for
 constexpr float kColdest = 1e-6f;            // colder rows are greedy
 
 template <typename T, int NT>
@@ -877,6 +878,34 @@ __device__ void join_keys(Shared<T, NT>& sh, int& turn, int& count, float& mass,
   turn ^= 1;
 }
 
+// The bound before which tokens are kept by top-k and top-p (`p` of the total mass), by bisection of the 64-bit ranks;
+// the token of rank `out` is not kept.
+template <typename T, int NT>
+__device__ __noinline__ Bound kept_bound(Shared<T, NT>& sh, const Slice<T> sl, float m, float c, float total,
+                                         long long top_k, float p, uint64_t out, int& turn) {
+  uint64_t lo = out, hi = ((uint64_t)order_key(m) << 32) | 0xffffffffu;  // nothing ranks before hi
+  Bound b;
+  b.none = false;
+  auto set = [&](uint64_t x) {
+    const uint32_t order = (uint32_t)(x >> 32), id = ~(uint32_t)x;
+    b.z = key_value(order);
+    b.id = id > 0x7fffffffu || order == 0x7fffffffu ? 0x7fffffff : (int)id;  // (no logit has -0's own order)
+  };
+  while (hi - lo > 1) {
+    const uint64_t mid = lo + (hi - lo) / 2;
+    set(mid);
+    int count = 0, flag = 0;
+    float mass = 0.f;
+    uint64_t best = 0;
+    count_before<T, NT>(sh, sl, m, c, b, count, mass);
+    join_keys(sh, turn, count, mass, best, flag);
+    if (count == 0 || (count < top_k && mass < p * total)) hi = mid;
+    else lo = mid;
+  }
+  set(lo);  // a token of rank hi and those before it are kept: what ranks before lo
+  return b;
+}
+
 // The first-ranked token.
 template <typename T, int NT>
 __device__ __noinline__ int first_rank(Shared<T, NT>& sh, const Slice<T>& sl, int& turn) {
@@ -983,7 +1012,8 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) sample_kernel(const T* 
   // No token below zmin has weight min_p (the weight itself decides about those above).
   const float zmin = by_m ? m + temperature * (logf(min_p) - 1e-4f) - 1e-5f * fabsf(m) : -INFINITY;
   Bound bound;
-  int id = -1;
+  int id = -1, rounds = 0;
+  bool settled = false;  // all tokens before `bound` are kept by top-k and top-p
   for (;;) {
     // the best of y, and then of the exact keys of the tokens within its margin
     int c0 = 0, f0 = 0, tie = 0;
@@ -1002,10 +1032,11 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) sample_kernel(const T* 
       join_keys(sh, turn, c0, m0, best, f0);
     }
     if (best == 0) {  // random numbers that are none: the first of the ranks
-      if (id < 0) id = first_rank<T, NT>(sh, sl, turn);
+      id = first_rank<T, NT>(sh, sl, turn);
       break;
     }
     id = rank_id(best);
+    if (settled) break;
     const float z = to_f(lrow[id]);
     bound.none = false;
     bound.id = id;
@@ -1018,6 +1049,13 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) sample_kernel(const T* 
       best = 0;
       join_keys(sh, turn, count, mass, best, f0);
       if (count == 0 || ((!by_k || count < top_k) && (!by_p || mass < top_p * total))) break;
+    }
+    // A winner that is not kept takes about half of what ranks before the last one away, so with random numbers this
+    // goes on for 1 + log(1 / kept share) rounds. Numbers that are not random can make it a round for each token.
+    if (++rounds == kMaxRounds) {
+      bound = kept_bound<T, NT>(sh, sl, m, c, total, by_k ? top_k : (long long)v, by_p ? top_p : INFINITY,
+                                rank_key(z, id), turn);
+      settled = true;
     }
     race = Race();
     race_before<T, NT>(sh, sl, ns, m, temperature, c, min_p, zmin, bound, race);

@@ -477,6 +477,50 @@ def test_sample_masked_and_broken_rows(device):
     assert greedy.cpu().tolist() == [4321, 6000, -1, -1, -1, 123, 0, -1]
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_sample_with_numbers_that_are_not_random(device):
+    """Falling numbers put the best key on the last-ranked token each time: the kept set must not be found one token a
+    pass. Distinct logits, so that ranks are the tokens' order, in both directions."""
+    n, v = 2, 12000
+    noise = torch.linspace(2.0, 1.0, v, device=device).expand(n, v).contiguous()
+    flat = torch.zeros(n, v, device=device)
+    slope = torch.stack([-torch.arange(v), torch.arange(v)]).to(device) * 2.0 ** -26  # hardly any slope
+    for z in (flat, flat + 1.0 + slope):
+        tok, _ = sample_tokens(z, noise, top_k=300)
+        first = z.cpu().sort(dim=-1, descending=True, stable=True)[1][:, :300]
+        want = first.gather(-1, noise.cpu().gather(-1, first).argmin(-1, keepdim=True)).squeeze(-1)
+        assert torch.equal(tok.cpu(), want)
+    # half a token past a quarter of the mass: 3000 tokens
+    tok, _ = sample_tokens(flat, noise, top_p=(3000 - 0.5) / v)
+    assert tok.cpu().tolist() == [2999, 2999]
+
+
+@pytest.mark.gpu
+def test_sample_numbers_that_are_none():
+    z = _logits(3, 9000, torch.float32, "cuda")
+    nan = torch.full((3, 9000), math.nan, device="cuda")
+    for kw in (dict(), dict(top_k=20), dict(top_p=0.5), dict(top_k=1000, min_p=0.1)):
+        assert torch.equal(sample_tokens(z, nan, **kw)[0], z.argmax(-1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_topk_crowded_groups(dtype):
+    """Far more large logits than k, all in a few threads' vectors, so that the groups that are read again hold more
+    candidates than there is room for; and rows whose k-th largest lies among them or below them."""
+    n, v = 230, 151936
+    z = torch.randn(n, v, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    i = torch.arange(v, device="cuda")
+    per = 4 if dtype == torch.float32 else 8
+    crowd = ((i // per) % 256 < 200) & (i < 12288)
+    z = torch.where(crowd, 20.0 + z, z).to(dtype)
+    for k in (64, 200, 256):
+        ids, _ = topk_logprobs(z, k)
+        for r in range(0, n, 37):
+            want = z[r].float().sort(descending=True, stable=True)[1][:k]
+            assert torch.equal(ids[r], want), (k, r)
+
+
 @pytest.mark.gpu
 def test_sample_strided_and_repeatable():
     base = _logits(9, 8000, torch.float16, "cuda")
