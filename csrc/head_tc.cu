@@ -125,17 +125,22 @@ TS_DEVICE void store_chunk(uint32_t buf, bool& busy, const CUtensorMap* map, con
   if (lane == 0) store_tile(map, buf, col, row0);
 }
 
-// The row's first entry at or after `col`: the entries are sorted by token, and those that do not count are last with
-// a token past any column.
-TS_DEVICE int first_entry(const int* __restrict__ ids, int k, int col) {
-  int lo = 0, hi = k;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (__ldg(ids + mid) < col) lo = mid + 1;
-    else hi = mid;
+// The search for a row's first entry at or after a column: the entries are sorted by token, and those that do not count
+// are last with a token past any column. A step's load is begun well before its outcome is used.
+struct EntrySearch {
+  const int* ids;
+  int col, lo, hi, seen;
+  TS_DEVICE void look() {
+    if (lo < hi) seen = __ldg(ids + ((lo + hi) >> 1));
   }
-  return lo;
-}
+  TS_DEVICE void narrow() {
+    if (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (seen < col) lo = mid + 1;
+      else hi = mid;
+    }
+  }
+};
 
 template <bool A_MN, bool B_MN, int OUT, bool STATS, int kChunk, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -278,13 +283,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Work w = work_of(shape, u);
       const int row0 = w.mb * kTileM + (int)rank * kBM + sub * 32, row = row0 + lane;
       const int col0 = w.nb * kBN + half * (kBN / 2);
-      int at = 0, next = 0x7fffffff;  // the row's next entry
-      const int* ids = nullptr;
+      EntrySearch find{nullptr, col0, 0, 0, 0};
       if constexpr (STATS) {
         if (row < shape.m) {
-          ids = st.ids + (long long)row * st.k;
-          at = first_entry(ids, st.k, col0);
-          if (at < st.k) next = __ldg(ids + at);
+          find.ids = st.ids + (long long)row * st.k;
+          find.hi = st.k;
         }
       }
       float acc[kBN / 2];
@@ -293,10 +296,15 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
       for (int kc = w.kb0; kc < w.kb1; kc += kChunk, ++chunk) {
         const int buf = chunk & 1;
+        if constexpr (STATS) find.look();
         if (lane == 0) ok = tc::mbar_wait(&bars->acc_full[buf], (chunk >> 1) & 1, abort, err, 321);
         ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
         if (!ok) break;
         tc::tc_fence_after();
+        if constexpr (STATS) {
+          find.narrow();
+          find.look();
+        }
         const uint32_t from = lane_base + buf * kBN;
 #pragma unroll
         for (int g = 0; g < 4; g += 2) {
@@ -316,10 +324,21 @@ __global__ void __launch_bounds__(kThreads, 1)
           if constexpr (PAIR) tc::mbar_arrive_cluster(buf ? acc_empty1 : acc_empty0);
           else tc::mbar_arrive(&bars->acc_empty[buf]);
         }
+        if constexpr (STATS) find.narrow();
       }
       if (!ok) break;
       if (row0 >= shape.m) continue;  // the same in the whole warp
       float m = -INFINITY, s = 0.f;
+      int at = 0, next = 0x7fffffff, after = 0x7fffffff;  // the row's next entry and the one behind it
+      if constexpr (STATS) {
+        while (find.lo < find.hi) {
+          find.look();
+          find.narrow();
+        }
+        at = find.lo;
+        if (at < (find.ids ? st.k : 0)) next = __ldg(find.ids + at);
+        if (at + 1 < (find.ids ? st.k : 0)) after = __ldg(find.ids + at + 1);
+      }
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const int col = col0 + g * 32;
@@ -341,7 +360,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (q == x) z = v[q];
               st.zk[(long long)row * st.k + at] = z;
               ++at;
-              next = at < st.k ? __ldg(ids + at) : 0x7fffffff;
+              next = after;
+              after = at + 1 < st.k ? __ldg(find.ids + at + 1) : 0x7fffffff;
             }
             if (col + 32 > shape.n) hit |= 0xffffffffu << (shape.n - col);
             if (__any_sync(0xffffffffu, hit != 0)) {
