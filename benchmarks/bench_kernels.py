@@ -13,8 +13,9 @@ Families: ``attn`` (bottom-right causal GQA attention; fwd, or fwd+bwd),
 (GRPO statistic folds), ``gemm`` (tcgen05 GEMM vs the library at decoder
 shapes), ``lmhead`` (fused tcgen05 LM-head logprob fwd+bwd vs the unfused
 cuBLAS-logits path), ``baselines`` (attention vs FlashAttention-2, the reference's
-GPU path without FA4, and the gated delta rule timed alone) and
-``gemm_host`` (host cost of a library GEMM call).
+GPU path without FA4, and the gated delta rule timed alone),
+``gemm_host`` (host cost of a library GEMM call) and ``distill`` (a teacher's
+top entries, the loss against them, sampling).
 """
 
 from __future__ import annotations
@@ -435,6 +436,36 @@ def bench_lmhead(args) -> None:
     L.FUSED_TC = True
 
 
+def bench_distill(args) -> None:
+    """Teacher's top entries, the distillation loss on logits and through the LM head, and sampling."""
+    from thundersync_b200.ops.distill import lm_head_topk_distill, topk_distill_loss, topk_logprobs
+    from thundersync_b200.ops.sampling import sample_tokens
+
+    n, dmod, vocab, k = args.rows, args.cols, 151936, 64
+    g = torch.Generator(device="cuda").manual_seed(0)
+    z = torch.randn(n, vocab, device="cuda", generator=g) * 2.5
+    ids, lp = topk_logprobs(z, k)
+    up = torch.rand(n, device="cuda", generator=g)
+    for dtype in (torch.float32, torch.bfloat16):
+        x = z.to(dtype)
+        gb = x.numel() * x.element_size() / 1e9
+        ms = _time(lambda: topk_logprobs(x, k), args.iters)
+        print(f"top {k} {n}x{vocab} {dtype}: {ms:.3f} ms {gb / ms * 1e3:.0f} GB/s")
+        leaf = x.detach().requires_grad_(True)
+        ms = _time(lambda: torch.autograd.grad(topk_distill_loss(leaf, ids, lp), leaf, up), args.iters)
+        print(f"distillation loss and gradient: {ms:.3f} ms {3 * gb / ms * 1e3:.0f} GB/s")
+        noise = torch.empty(n, vocab, device="cuda").exponential_(generator=g)
+        for name, kw in (("no filter", {}), ("top-k 20, top-p 0.95", dict(top_k=20, top_p=0.95)),
+                         ("top-p 0.9", dict(top_p=0.9)), ("min-p 0.05", dict(min_p=0.05))):
+            print(f"sampling, {name}: {_time(lambda: sample_tokens(x, noise, **kw), args.iters):.3f} ms")
+        del x, leaf, noise
+    w = (torch.randn(vocab, dmod, device="cuda", generator=g) * 2.5 / dmod ** 0.5).to(torch.bfloat16).requires_grad_(True)
+    h = torch.randn(n, dmod, device="cuda", generator=g).to(torch.bfloat16).requires_grad_(True)
+    ms = _time(lambda: torch.autograd.grad(lm_head_topk_distill(h, w, ids, lp), (h, w), up), args.iters)
+    print(f"LM-head distillation {n}x{dmod}x{vocab} fwd+bwd: {ms:.3f} ms "
+          f"({6.0 * n * dmod * vocab / ms / 1e9:.0f} TFLOP/s of 3 products)")
+
+
 def bench_lora(args) -> None:
     """LoRA projection (Qwen3-8B q_proj: 4096 -> 4096, rank 64) fwd and fwd+bwd: this package's unmerged op
     vs the merged-weight form (one base GEMM forward, the reference's fused mode) and the bare base GEMM."""
@@ -587,7 +618,7 @@ def bench_gemm_host(args) -> None:
 def main(argv=None) -> None:
     ap = argparse.ArgumentParser(description=__doc__.splitlines()[0])
     ap.add_argument("family", choices=["attn", "rms", "lse", "gdn", "conv", "gemm_host", "swiglu", "rope", "dlogits",
-                                       "adamw", "fold", "gemm", "gemm_ab", "gemm_one", "packed", "lmhead", "baselines", "lora", "layer_host"])
+                                       "adamw", "fold", "gemm", "gemm_ab", "gemm_one", "packed", "lmhead", "baselines", "lora", "layer_host", "distill"])
     ap.add_argument("--mode", choices=["fwd", "bwd"], default="bwd")
     ap.add_argument("--t", type=int, default=2048)
     ap.add_argument("--s", type=int, default=2560)
@@ -608,7 +639,7 @@ def main(argv=None) -> None:
      "gemm_host": bench_gemm_host, "swiglu": bench_swiglu, "rope": bench_rope, "dlogits": bench_dlogits,
      "adamw": bench_adamw, "fold": bench_fold, "gemm": bench_gemm, "gemm_ab": bench_gemm_ab, "gemm_one": bench_gemm_one, "packed": bench_packed,
      "lmhead": bench_lmhead, "baselines": bench_baselines, "lora": bench_lora,
-     "layer_host": bench_layer_host}[args.family](args)
+     "layer_host": bench_layer_host, "distill": bench_distill}[args.family](args)
 
 
 if __name__ == "__main__":

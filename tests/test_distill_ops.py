@@ -377,6 +377,21 @@ def test_head_needs_only_what_is_asked_and_honours_the_sink():
     assert rel <= 2 ** -8, rel  # the sink is not rounded to bf16
 
 
+@pytest.mark.gpu
+def test_head_kept_and_computed_again_are_the_same(monkeypatch):
+    from thundersync_b200.ops import distill
+
+    h, w, ids, lp, g = _head_case(300, 128, 2056, 8, torch.bfloat16, 1.0)
+    got = []
+    for room in (distill.KEEP_LOGITS_BYTES, 0):
+        monkeypatch.setattr(distill, "KEEP_LOGITS_BYTES", room)
+        loss = lm_head_topk_distill(h, w, ids, lp)
+        got.append([loss.detach(), *torch.autograd.grad(loss, (h, w), g)])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    with torch.no_grad():
+        assert torch.equal(lm_head_topk_distill(h, w, ids, lp), got[0][0])
+
+
 # ------------------------------------------------------------------ sampling
 def _sample_64(z, noise, t, k, p, mp):
     """One row: (token, log-prob) from the sorted tokens in 64 bits."""
