@@ -16,9 +16,9 @@
 //
 // Both kernels move each logit once: the forward reads the row (a bitmap of S in shared memory takes its tokens out of
 // the sum), the backward reads it and writes the gradient, then overwrites the entries of S with values that the
-// forward has left per entry. Memory bounds them: 1000 x 151,936 bf16 logits with 64 entries take 79 us forward (3.9
+// forward has left per entry. Memory bounds them: 1000 x 151,936 bf16 logits with 64 entries take 82 us forward (3.7
 // TB/s; at 11 logits a clock and SM for full rate the forward's 11 instructions a logit, issued 63% of the time, come
-// close) and 102-107 us backward (5.7-6.0 TB/s). For a few rows the launches and the caller's autograd take more than
+// close) and 102 us backward (6.0 TB/s). For a few rows the launches and the caller's autograd take more than
 // the kernels (33 fp32 rows: 21 + 9 of 70 us).
 #include "bounds.cuh"
 #include "common.cuh"

@@ -287,7 +287,9 @@ def lm_head_topk_distill(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids
     entries gives no gradient, but its zeros meet the hidden row in the weight gradient.
 
     In bf16 the dlogits are rounded to bf16 before the two gradient products, as in :func:`lm_head_logprob`: the
-    tensor cores take both operands in one type, and the weight is bf16."""
+    tensor cores take both operands in one type, and the weight is bf16. The gradients are then 1.9e-3 to 3.0e-3 of
+    their norm from 64 bits, depending on the inputs, where fp32 products rounded once at the end are 1.7e-3. Two
+    bf16 halves of the dlogits would mend that and double both products (0.94 and 0.92 of 3.9 ms at 2048 rows)."""
     if hidden.dim() != 2:
         raise ValueError(f"hidden must be [N, D], got {tuple(hidden.shape)}")
     if weight.dim() != 2 or weight.shape[1] != hidden.shape[1]:
