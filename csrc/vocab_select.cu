@@ -380,29 +380,42 @@ __device__ __noinline__ Stat scan_slice(Shared<T, NT>& sh, const Slice<T> sl, in
   return st;
 }
 
-// Block-wide (m, s); all threads get it.
-template <typename T, int NT>
-__device__ void block_stat(Shared<T, NT>& sh, Stat& st, float c) {
+// The lanes' (m, s) joined; all lanes get lane 0's. An exchange by xor leaves each lane its own rounding of s: the
+// multiply-add of a merge rounds one of its two products, and the two sides of an exchange differ in which.
+TS_DEVICE void warp_stat(Stat& st, float c) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const float m2 = __shfl_xor_sync(0xffffffffu, st.m, o), s2 = __shfl_xor_sync(0xffffffffu, st.s, o);
     stat_merge(st.m, st.s, m2, s2, c);
   }
+  st.m = __shfl_sync(0xffffffffu, st.m, 0);
+  st.s = __shfl_sync(0xffffffffu, st.s, 0);
+}
+
+// Block-wide (m, s); all threads get the same bits, which they compare with sums to decide about loops with barriers.
+template <typename T, int NT>
+__device__ void block_stat(Shared<T, NT>& sh, Stat& st, float c) {
+  warp_stat(st, c);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) {
     sh.wm[threadIdx.x >> 5] = st.m;
     sh.ws[threadIdx.x >> 5] = st.s;
   }
   __syncthreads();
-  // each warp merges the warps' pairs, in the same order
-  const int lane = threadIdx.x & 31;
-  st.m = lane < NT / 32 ? sh.wm[lane] : -INFINITY;
-  st.s = lane < NT / 32 ? sh.ws[lane] : 0.f;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float m2 = __shfl_xor_sync(0xffffffffu, st.m, o), s2 = __shfl_xor_sync(0xffffffffu, st.s, o);
-    stat_merge(st.m, st.s, m2, s2, c);
+  // one warp joins the warps' pairs, and its result is everyone's
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x;
+    st.m = lane < NT / 32 ? sh.wm[lane] : -INFINITY;
+    st.s = lane < NT / 32 ? sh.ws[lane] : 0.f;
+    warp_stat(st, c);
+    if (lane == 0) {
+      sh.jm = st.m;
+      sh.js = st.s;
+    }
   }
+  __syncthreads();
+  st.m = sh.jm;
+  st.s = sh.js;
 }
 
 // The row's statistics from the parts': one warp of each part reads them. All threads get them.
