@@ -85,7 +85,10 @@ __device__ void finish_row(Block2& b, float* red, long long row, int k, float z,
   const float m_tail = m;
   m = fmaxf(m_tail, block_max(red, have ? z : -INFINITY));
   if (m == -INFINITY) m = 0.f;
-  const double st = m_tail == -INFINITY ? s_tail : s_tail * exp2(((double)m_tail - (double)m) * c);
+  // 2^-1074 is the least number of 64 bits: where the tokens outside S have less of the mass they count as having none
+  const double a_tail = m_tail == -INFINITY ? 0.0 : ((double)m_tail - (double)m) * c;
+  const double f_tail = exp2(a_tail);
+  const double st = s_tail * f_tail;
   const double a2 = ((double)z - (double)m) * c;
   const double e = have ? exp2(a2) : 0.0;
   const double q = have ? exp((double)t) : 0.0;
@@ -99,7 +102,7 @@ __device__ void finish_row(Block2& b, float* red, long long row, int k, float z,
   const bool with_tail = tail && !(tp == 0.0);
   double lt = 0.0, tq = 0.0, ltq = 0.0;
   if (with_tail) {
-    lt = log(st) - ls;
+    lt = a_tail * 0.693147180559945309417 + log(s_tail) - ls;
     tq = fmax(1.0 - sq, kLeastTail);
     ltq = log(tq);
   }
@@ -110,24 +113,27 @@ __device__ void finish_row(Block2& b, float* red, long long row, int k, float z,
   }
   double sl = l, sp = have ? p : 0.0;
   block_sum2(b, sl, sp);
-  // The sums over g_k in closed form: g_k - G p_k and G themselves would cancel where P is small.
-  double g, gsum;  // of this entry, and G
+  // The sums over g_k in closed form: g_k - G p_k and G themselves would cancel where P is small. For the tokens outside
+  // S the backward multiplies by G p_j; G may be about Q/P and p_j no more than P, each of them past fp32 where P is
+  // small, so what it gets is relative to the largest logit outside S: p_j = 2^((z_j - m_tail) c) f_tail / s, and
+  // G f_tail / s is about Q / s_tail.
+  double g, gs;  // of this entry, and G f_tail / s
   if (!reverse) {
     if (with_tail) sl += tq * (ltq - lt);
     const double mass = sq + tq;
     g = p * mass - q;
-    gsum = (with_tail ? tq / tp : 0.0) - mass;
+    gs = (with_tail ? tq / s_tail : 0.0) - mass * f_tail / s;
   } else {
     if (with_tail) sl += tp * (lt - ltq);
     const double off = with_tail ? sl : sl + sp - 1.0;
     g = p == 0.0 ? 0.0 : p * (logp - (double)t - off);
-    gsum = with_tail ? off - (lt - ltq) : sl + sp;
+    gs = (with_tail ? off - (lt - ltq) : sl + sp) * f_tail / s;
   }
   if (tid < k) out.entry[row * k + tid] = have ? (float)(g / (double)tau) : 0.f;
   if (tid == 0) {
     out.loss[row] = (float)sl;
-    out.ref[row] = m;
-    out.gs[row] = (float)(gsum / (s * (double)tau));
+    out.ref[row] = m_tail == -INFINITY ? 0.f : m_tail;
+    out.gs[row] = s_tail == 0.0 && s > 0.0 ? 0.f : (float)(gs / (double)tau);  // 0: no token outside S
   }
 }
 
@@ -257,7 +263,7 @@ __global__ void __launch_bounds__(kThreads) distill_rows_fwd_kernel(const T* __r
   finish_row(sh.b, sh.red, row, k, zk, t, slot >= 0, m, total, c, tau, reverse, tail, out);
 }
 
-// d[n, j] = -g gs 2^((z - m)·c), and g · entry at the entries of S; rows without a gradient are zeros and are not read.
+// d[n, j] = -g gs 2^((z - ref)·c) (past fp32, perhaps, at the entries of S), and then g · entry at these; rows without a gradient are zeros and are not read.
 template <typename T, typename O>
 __global__ void __launch_bounds__(kThreads) distill_rows_bwd_kernel(const T* __restrict__ logits, long long stride,
                                                                     int v, const int* __restrict__ slots,

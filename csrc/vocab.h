@@ -44,8 +44,8 @@ struct DistillArgs {
 struct DistillOut {
   float* loss;   // [n]
   int* slots;    // [n, k] the entries that count (token, or -1)
-  float* ref;    // [n] m, the largest logit: p_j = 2^((z_j - m) c) / s, c = log2(e) / tau
-  float* gs;     // [n] G / (s tau): the row's gradient outside the entries is -gs 2^((z_j - m) c)
+  float* ref;    // [n] the largest logit outside the entries: p_j is in proportion to 2^((z_j - ref) c), c = log2(e) / tau
+  float* gs;     // [n] the row's gradient outside the entries is -gs 2^((z_j - ref) c)
   float* entry;  // [n, k] the gradient at the entries
 };
 

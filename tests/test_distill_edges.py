@@ -11,7 +11,27 @@ import math
 import pytest
 import torch
 
+from thundersync_b200.ops.distill import topk_distill_loss
 from thundersync_b200.ops.sampling import sample_tokens
+
+
+def _near(got: float, want: float, rtol: float = 4e-7, atol: float = 4e-6) -> bool:
+    return got == want or abs(got - want) <= atol + rtol * abs(want)
+
+
+def _loss_64(z, ids, lp, temperature, direction):
+    """One row from the definition, with the tail where its mass is not 0 in 64 bits."""
+    logp = torch.log_softmax(z / temperature, -1)
+    a, t = logp[ids], lp.double()
+    rest = torch.ones_like(z, dtype=torch.bool)
+    rest[ids] = False
+    lpt = torch.logsumexp(logp[rest], -1)
+    q = max(1.0 - float(t.exp().sum()), 1e-7)
+    if direction == "forward":
+        loss, more = (t.exp() * (t - a)).sum(), q * (math.log(q) - lpt)
+    else:
+        loss, more = (a.exp() * (a - t)).sum(), lpt.exp() * (lpt - math.log(q))
+    return loss + more if float(lpt.detach().exp()) > 0 else loss
 
 
 # ------------------------------------------------------------------ top-p at the edge of a token's mass
@@ -84,3 +104,40 @@ def test_sample_top_p_rows_in_one_part(dtype, n, v, top_p):
         assert int(clear.sum()) >= 0.95 * len(want)
         assert torch.equal(tok[r0:r0 + 200][clear], want[clear])
         assert torch.equal(again[r0:r0 + 200][clear], want[clear])
+
+
+# ------------------------------------------------------------------ students that give the other tokens next to nothing
+GAPS = [30.0, 80.0, 85.0, 88.0, 95.0, 100.0, 300.0, 700.0, 800.0, 1e4]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("direction", ["forward", "reverse"])
+@pytest.mark.parametrize("temperature", [1.0, 0.1])
+def test_gradient_of_a_far_tail(dtype, direction, temperature):
+    """Logits outside the entries lie `gap` nats below: their gradient is about Q in all, as long as their mass is not 0
+    in 64 bits."""
+    n, v, k = len(GAPS), 3001, 4
+    g = torch.Generator().manual_seed(0)
+    z = torch.randn(n, v, generator=g) * temperature - torch.tensor(GAPS)[:, None] * temperature
+    ids = torch.tensor([5, 700, 2047, 3000]).expand(n, k).contiguous()
+    z[:, ids[0]] = torch.tensor([0.0, -1.0, -0.5, -2.0]) * temperature
+    z = z.to(dtype)
+    lp = torch.log(torch.tensor([0.5, 0.25, 0.15, 0.05])).expand(n, k).contiguous()
+    x = z.cuda().requires_grad_(True)
+    loss = topk_distill_loss(x, ids.cuda(), lp.cuda(), temperature=temperature, direction=direction)
+    (dz,) = torch.autograd.grad(loss.sum(), x)
+    outside = torch.ones(v, dtype=torch.bool)
+    outside[ids[0]] = False
+    t32 = float(torch.tensor(temperature))
+    for i in range(n):
+        z64 = z[i].double().requires_grad_(True)
+        want = _loss_64(z64, ids[i], lp[i], t32, direction)
+        (dwant,) = torch.autograd.grad(want, z64)
+        assert _near(float(loss[i].detach()), float(want.detach()), 2e-6, 1e-5), (GAPS[i], loss[i], want)
+        got = dz[i].double().cpu()
+        unit = 2e-5 if dtype == torch.float32 else 2.0 ** -8
+        for part in (outside, ~outside):  # each against its own largest
+            err = (got[part] - dwant[part]).abs()
+            allowed = 2e-5 * dwant[part].abs().max() + unit * dwant[part].abs() + 1e-37
+            assert bool((err <= allowed).all()), (GAPS[i], float((err - allowed).max()))
