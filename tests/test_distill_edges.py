@@ -14,6 +14,8 @@ import torch
 from thundersync_b200.ops.distill import topk_distill_loss
 from thundersync_b200.ops.sampling import sample_tokens
 
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
 
 def _near(got: float, want: float, rtol: float = 4e-7, atol: float = 4e-6) -> bool:
     return got == want or abs(got - want) <= atol + rtol * abs(want)
@@ -110,13 +112,13 @@ def test_sample_top_p_rows_in_one_part(dtype, n, v, top_p):
 GAPS = [30.0, 80.0, 85.0, 88.0, 95.0, 100.0, 300.0, 700.0, 800.0, 1e4]
 
 
-@pytest.mark.gpu
+@pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("direction", ["forward", "reverse"])
 @pytest.mark.parametrize("temperature", [1.0, 0.1])
-def test_gradient_of_a_far_tail(dtype, direction, temperature):
+def test_gradient_of_a_far_tail(device, dtype, direction, temperature):
     """Logits outside the entries lie `gap` nats below: their gradient is about Q in all, as long as their mass is not 0
-    in 64 bits."""
+    in 64 bits; on the CPU as in the kernels."""
     n, v, k = len(GAPS), 3001, 4
     g = torch.Generator().manual_seed(0)
     z = torch.randn(n, v, generator=g) * temperature - torch.tensor(GAPS)[:, None] * temperature
@@ -124,8 +126,8 @@ def test_gradient_of_a_far_tail(dtype, direction, temperature):
     z[:, ids[0]] = torch.tensor([0.0, -1.0, -0.5, -2.0]) * temperature
     z = z.to(dtype)
     lp = torch.log(torch.tensor([0.5, 0.25, 0.15, 0.05])).expand(n, k).contiguous()
-    x = z.cuda().requires_grad_(True)
-    loss = topk_distill_loss(x, ids.cuda(), lp.cuda(), temperature=temperature, direction=direction)
+    x = z.to(device).requires_grad_(True)
+    loss = topk_distill_loss(x, ids.to(device), lp.to(device), temperature=temperature, direction=direction)
     (dz,) = torch.autograd.grad(loss.sum(), x)
     outside = torch.ones(v, dtype=torch.bool)
     outside[ids[0]] = False

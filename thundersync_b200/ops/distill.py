@@ -9,7 +9,8 @@ set ``S``, ``q = exp(teacher log-prob)``, and ``P``, ``Q`` what ``p`` and ``q`` 
     direction "reverse":  sum_S p (log p - log q)  [+ P (log P - log Q)]      KL(student || teacher)
 
 ``tail=True`` adds the bracketed term (all other tokens as one class; ``Q`` is held at 1e-7 at least, and the term is
-left out where the student gives the others nothing). The teacher is a constant: no gradient reaches it.
+left out where ``P`` is 0 in 64 bits: the others are masked, or some 744 nats and more below the entries). The teacher is
+a constant: no gradient reaches it.
 
 An entry with id -1 or log-prob -inf is no entry, so rows may have fewer than ``K``; of entries with the same id the
 first counts. A row without entries has loss 0 and gradient 0, whatever its logits are. A row whose logits hold NaN,
@@ -121,14 +122,17 @@ def _slots(ids, logprobs, v: int):
 
 
 def _loss_reference(z, ids, logprobs, temperature, direction, tail):
-    """The definition in plain torch, differentiable in ``z`` [N, V] (fp32 or fp64)."""
+    """The definition in plain torch, differentiable in ``z`` [N, V]; computed in 64 bits, as the kernels do the entries'
+    arithmetic, so both leave the tail out of the same rows. fp32 [N] (fp64 for fp64 logits)."""
     n, v = z.shape
+    wide = torch.float64
     have = _slots(ids, logprobs, v)
     used = have.any(-1)
-    z = torch.where(used[:, None], z, torch.zeros_like(z))
+    out = torch.float64 if z.dtype == torch.float64 else torch.float32
+    z = torch.where(used[:, None], z.to(wide), torch.zeros((), dtype=wide, device=z.device))
     logp = torch.log_softmax(z / temperature, -1)
     at = torch.where(have, ids, 0)
-    t = torch.where(have, logprobs.to(z.dtype), torch.zeros((), dtype=z.dtype, device=z.device))
+    t = torch.where(have, logprobs.to(wide), torch.zeros((), dtype=wide, device=z.device))
     a = logp.gather(-1, at)
     if direction == "forward":
         loss = torch.where(have, t.exp() * (t - a), torch.zeros_like(a)).sum(-1)
@@ -147,7 +151,7 @@ def _loss_reference(z, ids, logprobs, temperature, direction, tail):
         qt = (1.0 - torch.where(have, t.exp(), torch.zeros_like(t)).sum(-1)).clamp(min=_TAIL_FLOOR)
         more = qt * (qt.log() - lpt) if direction == "forward" else lpt.exp() * (lpt - qt.log())
         loss = loss + torch.where(some, more, torch.zeros_like(more))
-    return loss
+    return loss.to(out)
 
 
 def topk_distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logprobs: torch.Tensor, *,
@@ -160,8 +164,7 @@ def topk_distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     if _native_rows(logits):
         return native().distill_rows(_rows_contiguous(logits), ids, lp, float(temperature), direction == "reverse",
                                      bool(tail))
-    z = logits if logits.dtype == torch.float64 else logits.float()
-    return _loss_reference(z, ids, lp, temperature, direction, tail)
+    return _loss_reference(logits, ids, lp, temperature, direction, tail)
 
 
 # ------------------------------------------------------------------ the loss from hidden states
