@@ -24,14 +24,19 @@ TS_DEVICE float ex2(float x) {
 // 2^((z - m)·c) for z <= m; an m of -inf (nothing but -inf so far) stands for 0
 TS_DEVICE float rel_exp(float z, float m, float c) { return ex2((z - (m == -INFINITY ? 0.f : m)) * c); }
 
-// Sum of rel_exp over N values. z·c - m·c as one multiply-add: the product is exact inside it, so what is rounded is
-// r = m·c, the same for all values (2^-24 of r; taken back from the sum to first order), and the difference. Masks of
-// a type's lowest value (m·c past fp32) subtract first.
+// |m c| up to which an exponent is one multiply-add, z·c - r with r = m·c rounded, and the sum is multiplied by
+// 1 - ln2 (m c - r) afterwards: r is off by 2^-11 at most there, so what the first order leaves out is 6e-8. Above, as
+// for masks of finite values (a thread may have seen nothing else yet), for logits with a large offset and for cold
+// rows, the difference is taken first.
+constexpr float kFusedMost = 16384.f;
+
+// Sum of rel_exp over N values. In z·c - r the product is exact inside the multiply-add, so what is rounded is r, the
+// same for all values, and the difference.
 template <int N>
 TS_DEVICE float sum_exp(const float* z, float m, float c) {
   float s0 = 0.f, s1 = 0.f;
-  if (m > -1e30f) {
-    const float r = m * c;
+  const float r = m * c;
+  if (fabsf(r) <= kFusedMost) {
 #pragma unroll
     for (int e = 0; e + 1 < N; e += 2) {
       s0 += ex2(fmaf(z[e], c, -r));

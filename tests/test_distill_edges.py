@@ -11,14 +11,35 @@ import math
 import pytest
 import torch
 
-from thundersync_b200.ops.distill import topk_distill_loss
+from thundersync_b200.ops.distill import topk_distill_loss, topk_logprobs
 from thundersync_b200.ops.sampling import sample_tokens
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
 
 
 def _near(got: float, want: float, rtol: float = 4e-7, atol: float = 4e-6) -> bool:
-    return got == want or abs(got - want) <= atol + rtol * abs(want)
+    """`got` is an fp32 number: -5e38 can only be -inf there."""
+    return got == float(torch.tensor(want, dtype=torch.float32)) or abs(got - want) <= atol + rtol * abs(want)
+
+
+def _sample_64(z, noise, t, k=0, p=1.0, mp=0.0):
+    """One row in 64 bits: (token, log-prob, whether the edge of the kept set leaves the token as it is when it moves by
+    1e-5 of the mass or of a weight, which fp32 sums may do)."""
+    logp = torch.log_softmax(z.double() / t, -1)
+    order = z.double().sort(descending=True, stable=True)[1]
+    ps = logp[order].exp()
+    race = noise[order].double().log() - logp[order]  # the order of noise / p, without its underflow
+    found = []
+    for off in (0.0, 1e-5, -1e-5):
+        kept = torch.ones_like(ps, dtype=torch.bool)
+        if k > 0:
+            kept[k:] = False
+        if p < 1:
+            kept &= ps.cumsum(0) - ps < p + off
+        kept &= ps >= mp * (1 - off) * ps[0]
+        kept[0] = True
+        found.append(int(order[torch.where(kept, race, math.inf).argmin()]))
+    return found[0], float(logp[found[0]]), len(set(found)) == 1
 
 
 def _loss_64(z, ids, lp, temperature, direction):
@@ -143,3 +164,103 @@ def test_gradient_of_a_far_tail(device, dtype, direction, temperature):
             err = (got[part] - dwant[part]).abs()
             allowed = 2e-5 * dwant[part].abs().max() + unit * dwant[part].abs() + 1e-37
             assert bool((err <= allowed).all()), (GAPS[i], float((err - allowed).max()))
+
+
+# ------------------------------------------------------------------ masks of finite values, offsets, cold rows
+def _teacher_64(v, k, seed):
+    g = torch.Generator().manual_seed(seed)
+    ids = torch.randperm(v, generator=g)[:k]
+    lp = torch.log_softmax(torch.randn(k, generator=g).double(), -1) + math.log(0.9)
+    return ids, lp.float()
+
+
+def _check_rows(z, temperature, directions=("forward", "reverse"), settings=None):
+    """topk_logprobs, sample_tokens and topk_distill_loss on rows z [N, V] against 64 bits."""
+    n, v = z.shape
+    host = z.cpu().double()
+    t32 = float(torch.tensor(temperature))  # the kernels hold it in fp32
+    k = 20
+    ids, lp = topk_logprobs(z, k, temperature=temperature)
+    want = host.sort(dim=-1, descending=True, stable=True)[1][:, :k]
+    assert torch.equal(ids.cpu(), want)
+    for i in range(n):
+        ref = torch.log_softmax(host[i] / t32, -1)[want[i]]
+        assert all(_near(float(a), float(b)) for a, b in zip(lp[i], ref)), (i, lp[i], ref)
+    noise = torch.empty(n, v).exponential_(generator=torch.Generator().manual_seed(11))
+    for kw in settings or (dict(), dict(top_k=20, top_p=0.95), dict(top_p=0.9), dict(top_k=700), dict(min_p=0.01)):
+        tok, lps = sample_tokens(z, noise.to(z.device), temperature=temperature, **kw)
+        for i in range(n):
+            a, b, clear = _sample_64(host[i], noise[i], t32, kw.get("top_k", 0), kw.get("top_p", 1.0),
+                                     kw.get("min_p", 0.0))
+            assert int(tok[i]) == a or not clear, (i, kw, int(tok[i]), a)
+            if int(tok[i]) == a:
+                assert _near(float(lps[i]), b), (i, kw, float(lps[i]), b)
+    pairs = [_teacher_64(v, 12, i) for i in range(n)]
+    tid = torch.stack([a for a, _ in pairs])
+    tlp = torch.stack([b for _, b in pairs])
+    tid[:, 0] = host.argmax(-1)  # one likely entry, all different
+    for i in range(n):
+        tlp[i, 1:][tid[i, 1:] == tid[i, 0]] = -math.inf
+    for direction in directions:
+        x = z.detach().clone().requires_grad_(True)
+        loss = topk_distill_loss(x, tid.to(z.device), tlp.to(z.device), temperature=temperature, direction=direction)
+        (dz,) = torch.autograd.grad(loss.sum(), x)
+        for i in range(n):
+            on = tlp[i] != -math.inf
+            z64 = host[i].clone().requires_grad_(True)
+            ref = _loss_64(z64, tid[i][on], tlp[i][on], t32, direction)
+            (dref,) = torch.autograd.grad(ref, z64)
+            ref = float(ref.detach())
+            assert _near(float(loss[i].detach()), ref, 2e-6, 1e-5), (i, direction, float(loss[i].detach()), ref)
+            unit = 2e-5 if z.dtype == torch.float32 else 2.0 ** -8
+            dref = dref.float().double()  # (1e-204 is 0 there)
+            err = (dz[i].cpu().double() - dref).abs()
+            # a certain row's gradient is a difference of numbers of about 8 in 64 bits, in the reference too
+            allowed = 2e-5 * dref.abs().max() + unit * dref.abs() + 2.0 ** -47 / temperature
+            assert bool((err <= allowed).all()), (i, direction, float((err - allowed).max()))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("mask", [-1e4, -1e9, -1e10, -1e18, -1e20, -3e38])
+@pytest.mark.parametrize("temperature", [1.0, 0.6, 0.3])
+def test_masks_of_finite_values(device, dtype, mask, temperature):
+    v = 20003
+    g = torch.Generator().manual_seed(4)
+    z = torch.randn(5, v, generator=g) * 2.5
+    z[0, :v // 2] = mask  # every thread's first steps
+    z[1] = torch.where(torch.rand(v, generator=g) < 0.95, mask, z[1])
+    z[2] = mask  # a row that is nothing else: uniform
+    z[3, :-1] = mask
+    z[4, 1::2] = mask
+    _check_rows(z.to(dtype).to(device), temperature)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_masks_of_finite_values_in_several_parts(dtype):
+    v = 151936
+    z = torch.randn(3, v, generator=torch.Generator().manual_seed(5)) * 2.5
+    z[0, :140000] = -1e10  # whole slices of the row
+    z[1] = -1e9
+    z[2, 7:] = -1e20
+    _check_rows(z.to(dtype).cuda(), 0.6)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("offset", [1e3, -1e5, 1e6, -3e7])
+def test_logits_with_an_offset(device, offset):
+    z = torch.randn(3, 9001, generator=torch.Generator().manual_seed(6)) * 2.5 + offset
+    _check_rows(z.to(device), 1.0)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("temperature", [0.05, 1e-2, 1e-3, 1e-4, 1e-5, 2e-6, 1.01e-6])
+def test_cold_rows(device, temperature):
+    """One token holds the mass, or a few that are nearly equal: its log-prob is 0 and its draws are its own."""
+    g = torch.Generator().manual_seed(7)
+    z = torch.randn(6, 8009, generator=g) * 2.5 + torch.tensor([0.0, 3.0, 10.0, 20.0, 30.0, -30.0])[:, None]
+    z[0, 17] = 20.0
+    z[4, [40, 4000, 8000]] = 60.0
+    _check_rows(z.to(device), temperature, settings=(dict(), dict(top_k=20, top_p=0.95), dict(top_p=0.9),
+                                                     dict(top_p=0.4), dict(min_p=0.05)))
