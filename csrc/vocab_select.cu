@@ -697,8 +697,10 @@ __device__ __noinline__ void count_before(Shared<T, NT>& sh, const Slice<T> sl, 
   Steps<T, NT> steps(sl, sh.ring);
   const float bz = bound.z;
   const int bi = bound.id;
-  const bool plain = m > -1e30f;  // as in sum_exp
+  // as in sum_exp: the mass is compared with a total that is made so
   const float r = m * c;
+  const bool fused = fabsf(r) <= kFusedMost;
+  auto power = [&](float a) { return fused ? ex2(fmaf(a, c, -r)) : rel_exp(a, m, c); };
   int n = 0;
   float s0 = 0.f, s1 = 0.f;
   if (tid < sl.head + sl.tail) {
@@ -706,7 +708,7 @@ __device__ __noinline__ void count_before(Shared<T, NT>& sh, const Slice<T> sl, 
     const float a = to_f(sl.p[i]);
     if (bound.before(a, sl.lo + i)) {
       ++n;
-      s0 += rel_exp(a, m, c);
+      s0 += power(a);
     }
   }
   for (int t = 0; t < steps.count; ++t) {
@@ -718,8 +720,7 @@ __device__ __noinline__ void count_before(Shared<T, NT>& sh, const Slice<T> sl, 
 #pragma unroll
       for (int e = 0; e < VEC; e += 2) {
         const float a = z[q][e], b = z[q][e + 1];
-        const float ea = plain ? ex2(fmaf(a, c, -r)) : rel_exp(a, m, c);
-        const float eb = plain ? ex2(fmaf(b, c, -r)) : rel_exp(b, m, c);
+        const float ea = power(a), eb = power(b);
         n += (a > bz) + (b > bz);
         s0 += a > bz ? ea : 0.f;
         s1 += b > bz ? eb : 0.f;
@@ -734,7 +735,7 @@ __device__ __noinline__ void count_before(Shared<T, NT>& sh, const Slice<T> sl, 
         for (int e = 0; e < VEC; ++e) {
           if (z[q][e] == bz && id + e < bi && steps.has(t, q)) {
             ++n;
-            s0 += rel_exp(bz, m, c);
+            s0 += power(bz);
           }
         }
       }
@@ -742,7 +743,8 @@ __device__ __noinline__ void count_before(Shared<T, NT>& sh, const Slice<T> sl, 
   }
   copy_wait<0>();
   count = n;
-  mass = s0 + s1;
+  s0 += s1;
+  mass = fused ? fmaf(s0, -kLn2 * fmaf(m, c, -r), s0) : s0;
 }
 
 // The race among the tokens before `bound` with weight min_p at least (none is below zmin). Random numbers are read

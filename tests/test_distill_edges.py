@@ -93,6 +93,31 @@ def test_sample_top_p_one_rounding_apart(n, v, width):
         assert torch.equal(kept[far], (top_p.double() > mass)[far])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("temperature,top", [(0.05, 60.0), (0.01, 60.0), (1e-4, 60.0), (1e-4, 0.0), (1.0, 9000.0), (1.0, -2e4)])
+def test_sample_top_p_of_cold_and_offset_rows(temperature, top):
+    """The edge of the kept set where the scaled logits are large: the winner is kept from a top-p of the mass before it
+    on, within 6e-6 (3e-6 as above, and 2^-24 of exponents of up to 40 for the rounded log2(e) / temperature)."""
+    n, v = 900, 9001
+    g = torch.Generator().manual_seed(2)
+    z = (top + temperature * 2.5 * torch.randn(v, generator=g).double()).float()
+    order = z.double().sort(descending=True, stable=True)[1]
+    p = torch.softmax(z.double() / float(torch.tensor(temperature)), -1)[order]
+    rank = int((p.cumsum(0) < 0.8).sum())
+    mass = float(p[:rank].sum())
+    noise = torch.ones(v)
+    noise[order[rank]] = 1e-20  # wins where it is kept
+    noise[order[0]] = 1e-6  # and this one where it is not
+    top_p = (mass * (1 + torch.cat([torch.linspace(-1e-2, 1e-2, 300).double(), torch.linspace(-1e-4, 1e-4, 600).double()]))).float()
+    for parts in (z.expand(n, v), z.expand(n, v)[:100]):  # rows in one part, and in several
+        tok, _ = sample_tokens(parts.cuda(), noise.expand(n, v)[:len(parts)].cuda(), temperature=temperature,
+                               top_p=top_p[:len(parts)].cuda())
+        kept = tok.cpu() == order[rank]
+        assert bool((kept | (tok.cpu() == order[0])).all())
+        far = (top_p[:len(parts)].double() / mass - 1).abs() > 6e-6
+        assert torch.equal(kept[far], (top_p[:len(parts)].double() > mass)[far])
+
+
 def _sample_rows_64(z, noise, top_p):
     """(tokens, whether the kept set is clear of the rounding of sums) of rows at temperature 1, on their device."""
     zd = z.double()
