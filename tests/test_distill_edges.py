@@ -11,7 +11,7 @@ import math
 import pytest
 import torch
 
-from thundersync_b200.ops.distill import topk_distill_loss, topk_logprobs
+from thundersync_b200.ops.distill import lm_head_topk_distill, topk_distill_loss, topk_logprobs
 from thundersync_b200.ops.sampling import sample_tokens
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
@@ -289,3 +289,32 @@ def test_cold_rows(device, temperature):
     z[4, [40, 4000, 8000]] = 60.0
     _check_rows(z.to(device), temperature, settings=(dict(), dict(top_k=20, top_p=0.95), dict(top_p=0.9),
                                                      dict(top_p=0.4), dict(min_p=0.05)))
+
+
+# ------------------------------------------------------------------ what the LM head's node holds
+def _head_inputs(n, d, v, k, device, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    w = (torch.randn(v, d, generator=g) * (2.5 / math.sqrt(d))).to(dtype).to(device)
+    h = torch.randn(n, d, generator=g).to(dtype).to(device)
+    ids = torch.stack([torch.randperm(v, generator=g)[:k] for _ in range(n)]).to(device)
+    lp = (torch.log_softmax(torch.randn(n, k, generator=g), -1) + math.log(0.9)).to(device)
+    return h.requires_grad_(True), torch.nn.Parameter(w), ids, lp
+
+
+@pytest.mark.gpu
+def test_head_without_a_graph_holds_no_logits():
+    n, v = 640, 20480
+    h, w, ids, lp = _head_inputs(n, 64, v, 4, "cuda", torch.bfloat16)
+    logits = 4 * n * v
+    used = {}
+    for name in ("graph", "no graph"):
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        with torch.set_grad_enabled(name == "graph"):
+            loss = lm_head_topk_distill(h, w, ids, lp)
+        used[name] = torch.cuda.max_memory_allocated() - before
+        assert loss.requires_grad == (name == "graph")
+        del loss
+    # a few numbers per row and 128 columns beside them
+    assert used["graph"] >= logits and used["no graph"] <= logits // 8, used

@@ -194,7 +194,7 @@ def _to_eight(d: torch.Tensor, h: torch.Tensor):
 
 class _HeadTopkDistill(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hidden, weight, ids, logprobs, rows, temperature, direction, tail):
+    def forward(ctx, hidden, weight, ids, logprobs, rows, temperature, direction, tail, differentiated):
         n = hidden.shape[0]
         ctx.conf = (rows, temperature, direction, tail)
         ctx.weight = weight
@@ -202,7 +202,7 @@ class _HeadTopkDistill(torch.autograd.Function):
         ctx.blocks = []
         fused = _fused_ok(hidden, weight)
         reverse = direction == "reverse"
-        room = KEEP_LOGITS_BYTES if hidden.requires_grad or weight.requires_grad else 0
+        room = KEEP_LOGITS_BYTES if differentiated else 0
         loss = []
         for r0 in range(0, n, rows):
             r1 = min(n, r0 + rows)
@@ -276,7 +276,7 @@ class _HeadTopkDistill(torch.autograd.Function):
                     gemm_accumulate(dw, d8, h8, a_t=True, b_t=False)
         ctx.weight = None
         ctx.blocks = None
-        return dh, None if dw is None else dw.to(weight.dtype), None, None, None, None, None, None
+        return dh, None if dw is None else dw.to(weight.dtype), None, None, None, None, None, None, None
 
 
 def lm_head_topk_distill(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torch.Tensor,
@@ -304,4 +304,5 @@ def lm_head_topk_distill(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids
     h = hidden.contiguous()
     if h.is_cuda and h.data_ptr() % 16:  # the GEMMs' loads begin on 16-byte boundaries
         h = h.clone()
-    return _HeadTopkDistill.apply(h, weight, ids, lp, rows, float(temperature), direction, bool(tail))
+    differentiated = torch.is_grad_enabled() and (h.requires_grad or weight.requires_grad)
+    return _HeadTopkDistill.apply(h, weight, ids, lp, rows, float(temperature), direction, bool(tail), differentiated)
