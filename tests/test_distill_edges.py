@@ -318,3 +318,15 @@ def test_head_without_a_graph_holds_no_logits():
         del loss
     # a few numbers per row and 128 columns beside them
     assert used["graph"] >= logits and used["no graph"] <= logits // 8, used
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("change", ["weight", "hidden"])
+def test_head_operands_changed_before_the_backward(device, change):
+    """The backward reads hidden rows and weight again: one that has been changed in place is refused."""
+    h, w, ids, lp = _head_inputs(6, 64, 104, 4, device, torch.bfloat16 if device == "cuda" else torch.float32)
+    loss = lm_head_topk_distill(h, w, ids, lp)
+    with torch.no_grad():
+        (w if change == "weight" else h).mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.sum().backward()

@@ -197,8 +197,8 @@ class _HeadTopkDistill(torch.autograd.Function):
     def forward(ctx, hidden, weight, ids, logprobs, rows, temperature, direction, tail, differentiated):
         n = hidden.shape[0]
         ctx.conf = (rows, temperature, direction, tail)
-        ctx.weight = weight
-        ctx.save_for_backward(hidden, ids, logprobs)
+        ctx.param = weight  # for the sink, which knows its parameters by identity
+        ctx.save_for_backward(hidden, weight, ids, logprobs)
         ctx.blocks = []
         fused = _fused_ok(hidden, weight)
         reverse = direction == "reverse"
@@ -229,15 +229,14 @@ class _HeadTopkDistill(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        hidden, ids, logprobs = ctx.saved_tensors
-        weight = ctx.weight
+        hidden, weight, ids, logprobs = ctx.saved_tensors
         rows, temperature, direction, tail = ctx.conf
         n = hidden.shape[0]
         need_h, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
         fused = _fused_ok(hidden, weight)
         dh = torch.empty_like(hidden) if need_h else None
         s = _sink.active()
-        sink_w = need_w and s is not None and s.owns(weight)
+        sink_w = need_w and s is not None and s.owns(ctx.param)
         at_once = fused and need_w and not sink_w and 0 < n <= rows  # one block: no fp32 sum of blocks
         dw = None
         if need_w and not sink_w and not at_once:
@@ -271,10 +270,9 @@ class _HeadTopkDistill(torch.autograd.Function):
             elif need_w:
                 d8, h8 = _to_eight(d, h) if d.is_cuda else (d, h)
                 if sink_w:
-                    s.addmm_(s.view(weight), d8, h8)
+                    s.addmm_(s.view(ctx.param), d8, h8)
                 else:
                     gemm_accumulate(dw, d8, h8, a_t=True, b_t=False)
-        ctx.weight = None
         ctx.blocks = None
         return dh, None if dw is None else dw.to(weight.dtype), None, None, None, None, None, None, None
 
