@@ -330,3 +330,16 @@ def test_head_operands_changed_before_the_backward(device, change):
         (w if change == "weight" else h).mul_(2.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.sum().backward()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("rows", [128, 4096])
+def test_head_second_backward(device, rows):
+    """A retained graph gives the same gradients again; one that was not retained says so."""
+    h, w, ids, lp = _head_inputs(300, 64, 104, 4, device, torch.bfloat16 if device == "cuda" else torch.float32)
+    loss = lm_head_topk_distill(h, w, ids, lp, rows=rows).sum()
+    first = torch.autograd.grad(loss, (h, w), retain_graph=True)
+    second = torch.autograd.grad(loss, (h, w))
+    assert all(torch.equal(a, b) for a, b in zip(first, second))
+    with pytest.raises(RuntimeError, match="backward through the graph a second time"):
+        torch.autograd.grad(loss, (h, w))

@@ -198,8 +198,8 @@ class _HeadTopkDistill(torch.autograd.Function):
         n = hidden.shape[0]
         ctx.conf = (rows, temperature, direction, tail)
         ctx.param = weight  # for the sink, which knows its parameters by identity
-        ctx.save_for_backward(hidden, weight, ids, logprobs)
-        ctx.blocks = []
+        ctx.logits = []  # of the blocks that keep theirs: the first backward uses them up, another computes them again
+        saved = []       # four small tensors of each block
         fused = _fused_ok(hidden, weight)
         reverse = direction == "reverse"
         room = KEEP_LOGITS_BYTES if differentiated else 0
@@ -210,18 +210,20 @@ class _HeadTopkDistill(torch.autograd.Function):
                 size = 4 * (r1 - r0) * weight.shape[0]
                 keep = size <= room
                 room -= size if keep else 0
-                part, *kept = native().distill_head_fwd(hidden[r0:r1], weight, ids[r0:r1], logprobs[r0:r1], temperature,
-                                                        reverse, tail, keep)
-                ctx.blocks.append(kept)
+                part, *kept, logits = native().distill_head_fwd(hidden[r0:r1], weight, ids[r0:r1], logprobs[r0:r1],
+                                                                temperature, reverse, tail, keep)
+                saved += kept
+                ctx.logits.append(logits)
                 loss.append(part)
                 continue
             logits = _logits_fp32(hidden[r0:r1], weight)
             if _native_rows(logits):
                 part, *kept = native().distill_rows_fwd(logits, ids[r0:r1], logprobs[r0:r1], temperature, reverse, tail)
-                ctx.blocks.append([*kept, None])
+                saved += kept
             else:
                 part = _loss_reference(logits, ids[r0:r1], logprobs[r0:r1], temperature, direction, tail)
             loss.append(part)
+        ctx.save_for_backward(hidden, weight, ids, logprobs, *saved)
         if len(loss) == 1:
             return loss[0]
         return torch.cat(loss) if loss else hidden.new_zeros(0, dtype=torch.float32)
@@ -229,7 +231,7 @@ class _HeadTopkDistill(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        hidden, weight, ids, logprobs = ctx.saved_tensors
+        hidden, weight, ids, logprobs, *saved = ctx.saved_tensors
         rows, temperature, direction, tail = ctx.conf
         n = hidden.shape[0]
         need_h, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
@@ -246,13 +248,14 @@ class _HeadTopkDistill(torch.autograd.Function):
         for i, r0 in enumerate(range(0, n, rows)):
             r1 = min(n, r0 + rows)
             h = hidden[r0:r1]
-            logits = ctx.blocks[i][-1] if ctx.blocks else None
+            logits = None
+            if ctx.logits:
+                logits, ctx.logits[i] = ctx.logits[i], None
             if logits is None:
                 logits = native().distill_head_logits(h, weight) if fused else _logits_fp32(h, weight)
             if _native_rows(logits):
                 d = torch.empty(logits.shape, dtype=hidden.dtype, device=hidden.device)
-                native().distill_rows_bwd(logits, *ctx.blocks[i][:-1], g[r0:r1].float(), temperature, d)
-                ctx.blocks[i] = None
+                native().distill_rows_bwd(logits, *saved[4 * i:4 * i + 4], g[r0:r1].float(), temperature, d)
             else:
                 with torch.enable_grad():
                     z = logits.requires_grad_(True)
@@ -273,7 +276,6 @@ class _HeadTopkDistill(torch.autograd.Function):
                     s.addmm_(s.view(ctx.param), d8, h8)
                 else:
                     gemm_accumulate(dw, d8, h8, a_t=True, b_t=False)
-        ctx.blocks = None
         return dh, None if dw is None else dw.to(weight.dtype), None, None, None, None, None, None, None
 
 
