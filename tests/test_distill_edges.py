@@ -343,3 +343,36 @@ def test_head_second_backward(device, rows):
     assert all(torch.equal(a, b) for a, b in zip(first, second))
     with pytest.raises(RuntimeError, match="backward through the graph a second time"):
         torch.autograd.grad(loss, (h, w))
+
+
+@pytest.mark.gpu
+def test_head_graphs_share_the_room_for_logits(monkeypatch):
+    """Several losses before one backward hold no more logits than one may, and their gradients do not depend on it."""
+    from thundersync_b200.ops import distill
+
+    n, v = 256, 20480
+    size = 4 * n * v
+    monkeypatch.setattr(distill, "KEEP_LOGITS_BYTES", 2 * size + 1000)
+    h, w, ids, lp = _head_inputs(n, 64, v, 4, "cuda", torch.bfloat16)
+
+    def six():
+        return [lm_head_topk_distill(h * (1.0 + 0.25 * i), w, ids, lp) for i in range(6)]
+
+    one = torch.autograd.grad(six()[0].sum(), (h, w))
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    losses = six()
+    held = torch.cuda.memory_allocated() - before
+    assert 2 * size <= held <= 2 * size + size // 2, held / size
+    grads = [torch.autograd.grad(x.sum(), (h, w)) for x in losses]
+    assert all(torch.equal(a, b) for a, b in zip(grads[0], one))
+    monkeypatch.setattr(distill, "KEEP_LOGITS_BYTES", 0)
+    for a, b in zip(grads, [torch.autograd.grad(x.sum(), (h, w)) for x in six()]):
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+    del losses
+    monkeypatch.setattr(distill, "KEEP_LOGITS_BYTES", 2 * size + 1000)
+    losses = six()[:1]  # the others' room is free again
+    assert torch.cuda.memory_allocated() - before >= size
+    again = lm_head_topk_distill(h, w, ids, lp)
+    assert torch.cuda.memory_allocated() - before >= 2 * size
+    del losses, again

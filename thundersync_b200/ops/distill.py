@@ -24,6 +24,8 @@ to the logits' type.
 from __future__ import annotations
 
 import math
+import threading
+import weakref
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -172,10 +174,35 @@ def topk_distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
 # 151,936-token vocabulary) and bf16 dlogits (half of that). One block writes the weight gradient in bf16 at once;
 # several add fp32 products and round at the end.
 BLOCK_ROWS = 4096
-# The forward's fp32 logits that a call may keep for its backward, in bytes. A block past it computes them again,
-# which at 2048 rows x 2048 x 151,936 takes a third of the backward's time on top; keeping them holds that memory from
-# the forward to the backward.
+# The forwards' fp32 logits that a process keeps on a device for their backwards, in bytes, of all graphs that are alive
+# together. A block past it computes them again, which at 2048 rows x 2048 x 151,936 takes a third of the backward's time
+# on top; keeping them holds that memory from the forward to the backward.
 KEEP_LOGITS_BYTES = 3 << 30
+_kept_lock = threading.Lock()
+
+
+class _KeptLogits:
+    """A block's logits from its forward to its backward; they count as kept until they are taken or the graph is gone."""
+
+    _alive: "weakref.WeakSet[_KeptLogits]" = weakref.WeakSet()
+
+    def __init__(self, device: torch.device, size: int) -> None:
+        self.device, self.size, self.logits = device, size, None
+
+    @classmethod
+    def room(cls, device: torch.device, size: int) -> "_KeptLogits | None":
+        """A place for ``size`` bytes of logits, or None."""
+        with _kept_lock:
+            if size + sum(k.size for k in cls._alive if k.device == device) > KEEP_LOGITS_BYTES:
+                return None
+            kept = cls(device, size)
+            cls._alive.add(kept)
+            return kept
+
+    def take(self) -> torch.Tensor | None:
+        """The logits, once."""
+        logits, self.logits, self.size = self.logits, None, 0
+        return logits
 
 
 def _fused_ok(hidden: torch.Tensor, weight: torch.Tensor) -> bool:
@@ -198,28 +225,27 @@ class _HeadTopkDistill(torch.autograd.Function):
         n = hidden.shape[0]
         ctx.conf = (rows, temperature, direction, tail)
         ctx.param = weight  # for the sink, which knows its parameters by identity
-        ctx.logits = []  # of the blocks that keep theirs: the first backward uses them up, another computes them again
-        saved = []       # four small tensors of each block
+        ctx.kept = []  # logits of the blocks that keep theirs: a first backward uses them up, another computes them again
+        saved = []  # four small tensors of each block
         fused = _fused_ok(hidden, weight)
         reverse = direction == "reverse"
-        room = KEEP_LOGITS_BYTES if differentiated else 0
         loss = []
         for r0 in range(0, n, rows):
             r1 = min(n, r0 + rows)
             if fused:
-                size = 4 * (r1 - r0) * weight.shape[0]
-                keep = size <= room
-                room -= size if keep else 0
-                part, *kept, logits = native().distill_head_fwd(hidden[r0:r1], weight, ids[r0:r1], logprobs[r0:r1],
-                                                                temperature, reverse, tail, keep)
-                saved += kept
-                ctx.logits.append(logits)
+                kept = _KeptLogits.room(hidden.device, 4 * (r1 - r0) * weight.shape[0]) if differentiated else None
+                part, *small, logits = native().distill_head_fwd(hidden[r0:r1], weight, ids[r0:r1], logprobs[r0:r1],
+                                                                 temperature, reverse, tail, kept is not None)
+                if kept is not None:
+                    kept.logits = logits
+                saved += small
+                ctx.kept.append(kept)
                 loss.append(part)
                 continue
             logits = _logits_fp32(hidden[r0:r1], weight)
             if _native_rows(logits):
-                part, *kept = native().distill_rows_fwd(logits, ids[r0:r1], logprobs[r0:r1], temperature, reverse, tail)
-                saved += kept
+                part, *small = native().distill_rows_fwd(logits, ids[r0:r1], logprobs[r0:r1], temperature, reverse, tail)
+                saved += small
             else:
                 part = _loss_reference(logits, ids[r0:r1], logprobs[r0:r1], temperature, direction, tail)
             loss.append(part)
@@ -248,9 +274,7 @@ class _HeadTopkDistill(torch.autograd.Function):
         for i, r0 in enumerate(range(0, n, rows)):
             r1 = min(n, r0 + rows)
             h = hidden[r0:r1]
-            logits = None
-            if ctx.logits:
-                logits, ctx.logits[i] = ctx.logits[i], None
+            logits = ctx.kept[i].take() if ctx.kept and ctx.kept[i] is not None else None
             if logits is None:
                 logits = native().distill_head_logits(h, weight) if fused else _logits_fp32(h, weight)
             if _native_rows(logits):
@@ -285,8 +309,9 @@ def lm_head_topk_distill(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids
     """Loss [N] (fp32) of the student ``hidden`` [N, D] · ``weight`` [V, D]ᵀ against the teacher's entries [N, K],
     differentiable in ``hidden`` and ``weight`` (whose gradient honours an active gradient sink).
 
-    ``rows`` rows are worked at a time (default ``BLOCK_ROWS``), and up to ``KEEP_LOGITS_BYTES`` of fp32 logits stay
-    from the forward to the backward; both are attributes of this module. Hidden rows must be finite: a row without
+    ``rows`` rows are worked at a time (default ``BLOCK_ROWS``), and up to ``KEEP_LOGITS_BYTES`` of fp32 logits, of all
+    graphs of a process on a device together, stay from their forwards to their backwards; both are attributes of this
+    module. Hidden rows must be finite: a row without
     entries gives no gradient, but its zeros meet the hidden row in the weight gradient.
 
     In bf16 the dlogits are rounded to bf16 before the two gradient products, as in :func:`lm_head_logprob`: the
