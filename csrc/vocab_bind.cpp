@@ -140,6 +140,18 @@ void distill_rows_bwd(const at::Tensor& logits, const at::Tensor& slots, const a
 
 namespace {
 
+// The gradient as the end of what can be differentiated: it depends on the logits and the upstream gradient, but asking
+// for that dependence is an error.
+struct DifferentiatedOnce : torch::autograd::Function<DifferentiatedOnce> {
+  static at::Tensor forward(torch::autograd::AutogradContext*, const at::Tensor& d, const at::Tensor&, const at::Tensor&) {
+    return d;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext*, torch::autograd::variable_list) {
+    TS_CHECK(false, "topk_distill_loss is differentiable once: its gradient on CUDA has no gradient of its own");
+    return {};
+  }
+};
+
 // The loss on logits as a native autograd node: its backward needs no interpreter, which for a few rows was most of
 // the call's time.
 struct DistillRows : torch::autograd::Function<DistillRows> {
@@ -155,9 +167,13 @@ struct DistillRows : torch::autograd::Function<DistillRows> {
     at::Tensor d;
     if (grads[0].defined()) {
       const auto s = ctx->get_saved_variables();
-      d = at::empty(s[0].sizes(), s[0].options());
-      distill_rows_bwd(s[0], s[1], s[2], s[3], s[4], grads[0].to(at::kFloat).contiguous(),
-                       ctx->saved_data["tau"].toDouble(), d);
+      {
+        const at::AutoGradMode off(false);
+        d = at::empty(s[0].sizes(), s[0].options());
+        distill_rows_bwd(s[0], s[1], s[2], s[3], s[4], grads[0].to(at::kFloat).contiguous(),
+                         ctx->saved_data["tau"].toDouble(), d);
+      }
+      if (at::GradMode::is_enabled()) d = DifferentiatedOnce::apply(d, s[0], grads[0]);  // (create_graph)
     }
     return {d, {}, {}, {}, {}, {}};
   }

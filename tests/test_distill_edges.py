@@ -376,3 +376,41 @@ def test_head_graphs_share_the_room_for_logits(monkeypatch):
     again = lm_head_topk_distill(h, w, ids, lp)
     assert torch.cuda.memory_allocated() - before >= 2 * size
     del losses, again
+
+
+# ------------------------------------------------------------------ derivatives of derivatives
+@pytest.mark.gpu
+@pytest.mark.parametrize("head", [False, True])
+def test_a_second_derivative_is_refused_on_cuda(head):
+    """With create_graph the gradient is the same; what depends on it cannot be differentiated as if it were constant."""
+    h, w, ids, lp = _head_inputs(5, 64, 104, 4, "cuda", torch.bfloat16)
+    if head:
+        x, loss = h, lambda: lm_head_topk_distill(h, w, ids, lp).sum()
+    else:
+        x = torch.randn(5, 104, device="cuda", requires_grad=True)
+        loss = lambda: topk_distill_loss(x, ids, lp).sum()  # noqa: E731
+    (plain,) = torch.autograd.grad(loss(), x)
+    (d,) = torch.autograd.grad(loss(), x, create_graph=True)
+    assert torch.equal(d, plain) and d.requires_grad
+    with pytest.raises(RuntimeError, match="differentia"):
+        (d.float() ** 2).sum().backward()
+    # a penalty on other terms of the same graph is not in the way
+    (d,) = torch.autograd.grad(loss() + (x ** 3).sum(), x, create_graph=True)
+    assert torch.allclose(d.detach(), plain + 3 * x.detach() ** 2, rtol=1e-2, atol=1e-2)
+
+
+def test_a_second_derivative_through_the_head_is_refused():
+    h, w, ids, lp = _head_inputs(5, 64, 104, 4, "cpu", torch.float32)
+    loss = lm_head_topk_distill(h, w, ids, lp).sum()
+    plain = torch.autograd.grad(loss, (h, w), retain_graph=True)
+    dh, dw = torch.autograd.grad(loss, (h, w), create_graph=True)
+    assert torch.equal(dh, plain[0]) and torch.equal(dw, plain[1])
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        dw.sum().backward()
+
+
+def test_second_derivative_on_the_cpu():
+    z = torch.randn(2, 9, dtype=torch.float64, generator=torch.Generator().manual_seed(0)).requires_grad_(True)
+    ids = torch.tensor([[0, 3, 5], [8, 2, 1]])
+    lp = torch.log(torch.tensor([[0.5, 0.2, 0.1], [0.3, 0.3, 0.2]]))
+    assert torch.autograd.gradgradcheck(lambda x: topk_distill_loss(x, ids, lp), (z,))

@@ -28,7 +28,6 @@ import threading
 import weakref
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from thundersync_b200.ops import sink as _sink
 from thundersync_b200.ops._ext import native
@@ -219,6 +218,18 @@ def _to_eight(d: torch.Tensor, h: torch.Tensor):
     return (torch.cat((d, d.new_zeros(pad, d.shape[1]))), torch.cat((h, h.new_zeros(pad, h.shape[1]))))
 
 
+class _DifferentiatedOnce(torch.autograd.Function):
+    """A gradient as the end of what can be differentiated: asking how it depends on the inputs is an error."""
+
+    @staticmethod
+    def forward(ctx, gradient, *inputs):
+        return gradient
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("lm_head_topk_distill is differentiable once: its gradients have no gradients of their own")
+
+
 class _HeadTopkDistill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, ids, logprobs, rows, temperature, direction, tail, differentiated):
@@ -255,8 +266,16 @@ class _HeadTopkDistill(torch.autograd.Function):
         return torch.cat(loss) if loss else hidden.new_zeros(0, dtype=torch.float32)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g):
+        hidden, weight = ctx.saved_tensors[:2]
+        with torch.no_grad():
+            grads = _HeadTopkDistill._gradients(ctx, g)
+        if torch.is_grad_enabled():  # (create_graph)
+            grads = [None if d is None else _DifferentiatedOnce.apply(d, hidden, weight, g) for d in grads]
+        return (*grads, None, None, None, None, None, None, None)
+
+    @staticmethod
+    def _gradients(ctx, g):
         hidden, weight, ids, logprobs, *saved = ctx.saved_tensors
         rows, temperature, direction, tail = ctx.conf
         n = hidden.shape[0]
@@ -300,7 +319,7 @@ class _HeadTopkDistill(torch.autograd.Function):
                     s.addmm_(s.view(ctx.param), d8, h8)
                 else:
                     gemm_accumulate(dw, d8, h8, a_t=True, b_t=False)
-        return dh, None if dw is None else dw.to(weight.dtype), None, None, None, None, None, None, None
+        return dh, None if dw is None else dw.to(weight.dtype)
 
 
 def lm_head_topk_distill(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torch.Tensor,
