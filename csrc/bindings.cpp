@@ -74,8 +74,8 @@ std::vector<c10::optional<at::Tensor>> distill_head_fwd(const at::Tensor& h, con
                                                         const at::Tensor& lp, double tau, bool reverse, bool tail,
                                                         bool keep);
 at::Tensor distill_head_logits(const at::Tensor& h, const at::Tensor& w);
-void distill_head_dh(const at::Tensor& dl, const at::Tensor& w, at::Tensor& dh);
-at::Tensor distill_head_dw(const at::Tensor& dl, const at::Tensor& h);
+void distill_head_dh(const at::Tensor& dl, const c10::optional<at::Tensor>& lo, const at::Tensor& w, at::Tensor& dh);
+at::Tensor distill_head_dw(const at::Tensor& dl, const c10::optional<at::Tensor>& lo, const at::Tensor& h);
 void register_ipc(pybind11::module& m);
 uint64_t bounds_word_rowops(bool reset);
 uint64_t bounds_word_fold(bool reset);
@@ -89,7 +89,8 @@ std::vector<at::Tensor> sample_tokens(const at::Tensor& logits, const c10::optio
 std::vector<at::Tensor> distill_rows_fwd(const at::Tensor& logits, const at::Tensor& ids, const at::Tensor& lp,
                                          double tau, bool reverse, bool tail);
 void distill_rows_bwd(const at::Tensor& logits, const at::Tensor& slots, const at::Tensor& ref, const at::Tensor& gs,
-                      const at::Tensor& entry, const at::Tensor& grad, double tau, at::Tensor& out);
+                      const at::Tensor& entry, const at::Tensor& grad, double tau, at::Tensor& out,
+                      const c10::optional<at::Tensor>& lo);
 void register_pinned(pybind11::module& m);
 void gemm_tc(at::Tensor& out, const at::Tensor& a, const at::Tensor& b, bool a_t, bool b_t, int64_t mode,
              double alpha, const c10::optional<at::Tensor>& residual);

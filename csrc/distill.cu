@@ -263,15 +263,18 @@ __global__ void __launch_bounds__(kThreads) distill_rows_fwd_kernel(const T* __r
   finish_row(sh.b, sh.red, row, k, zk, t, slot >= 0, m, total, c, tau, reverse, tail, out);
 }
 
-// d[n, j] = -g gs 2^((z - ref)·c) (past fp32, perhaps, at the entries of S), and then g · entry at these; rows without a gradient are zeros and are not read.
-template <typename T, typename O>
+// d[n, j] = -g gs 2^((z - ref)·c) (past fp32, perhaps, at the entries of S), and then g · entry at these; rows without a
+// gradient are zeros and are not read. TWO: `out` gets d rounded to bf16 and `lo` what the rounding leaves, rounded to
+// bf16, which together hold 16 bits of it.
+template <typename T, typename O, bool TWO>
 __global__ void __launch_bounds__(kThreads) distill_rows_bwd_kernel(const T* __restrict__ logits, long long stride,
                                                                     int v, const int* __restrict__ slots,
                                                                     const float* __restrict__ ref,
                                                                     const float* __restrict__ gs,
                                                                     const float* __restrict__ entry,
                                                                     const float* __restrict__ grad, int k, float tau,
-                                                                    int parts, O* __restrict__ out, long long ostride) {
+                                                                    int parts, O* __restrict__ out, O* __restrict__ lo,
+                                                                    long long ostride) {
   constexpr int VEC = Slice<T>::kVec;
   const long long row = blockIdx.x / parts;
   const int part = blockIdx.x % parts;
@@ -282,15 +285,35 @@ __global__ void __launch_bounds__(kThreads) distill_rows_bwd_kernel(const T* __r
   const float m = ref[row];
   Slice<T> sl(logits + row * stride, v, part, parts);
   O* o = out + row * ostride + sl.lo;
+  O* o2 = TWO ? lo + row * ostride + sl.lo : nullptr;
   auto d = [&](float z) { return coef * ex2((z - m) * c); };
+  auto put = [&](int i, float x) {
+    o[i] = from_f<O>(x);
+    if constexpr (TWO) o2[i] = from_f<O>(x - to_f(from_f<O>(x)));
+  };
   if (tid < sl.head + sl.tail) {
     const int i = tid < sl.head ? tid : sl.nvec * VEC + tid;
-    o[i] = from_f<O>(coef == 0.f ? 0.f : d(to_f(sl.p[i])));
+    put(i, coef == 0.f ? 0.f : d(to_f(sl.p[i])));
   }
   const T* body = sl.body();
-  O* ob = o + sl.head;
   constexpr int OB = VEC * sizeof(O);  // output bytes of a vector: 8, 16 or 32
-  const bool wide = (reinterpret_cast<uintptr_t>(ob) % (OB < 16 ? OB : 16)) == 0;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(o + sl.head) | (TWO ? reinterpret_cast<uintptr_t>(o2 + sl.head) : 0);
+  const bool wide = at % (OB < 16 ? OB : 16) == 0;
+  auto put_vec = [&](O* w, const float* x) {
+    union {
+      O e[VEC];
+      uint4 q[OB >= 16 ? OB / 16 : 1];
+      uint2 h;
+    } u;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) u.e[e] = from_f<O>(x[e]);
+    if constexpr (OB == 8) {
+      *reinterpret_cast<uint2*>(w) = u.h;
+    } else {
+#pragma unroll
+      for (int q = 0; q < OB / 16; ++q) reinterpret_cast<uint4*>(w)[q] = u.q[q];
+    }
+  };
   constexpr int U = 16 / VEC;
   for (int i0 = tid; i0 < sl.nvec; i0 += U * kThreads) {
     uint4 raw[U];
@@ -310,32 +333,24 @@ __global__ void __launch_bounds__(kThreads) distill_rows_bwd_kernel(const T* __r
 #pragma unroll
         for (int e = 0; e < VEC; ++e) z[e] = d(z[e]);
       }
-      O* w = ob + (long long)i * VEC;
+      const int w = sl.head + i * VEC;
       if (wide) {
-        union {
-          O e[VEC];
-          uint4 q[OB >= 16 ? OB / 16 : 1];
-          uint2 h;
-        } u;
+        put_vec(o + w, z);
+        if constexpr (TWO) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) u.e[e] = from_f<O>(z[e]);
-        if constexpr (OB == 8) {
-          *reinterpret_cast<uint2*>(w) = u.h;
-        } else {
-#pragma unroll
-          for (int q = 0; q < OB / 16; ++q) reinterpret_cast<uint4*>(w)[q] = u.q[q];
+          for (int e = 0; e < VEC; ++e) z[e] -= to_f(from_f<O>(z[e]));
+          put_vec(o2 + w, z);
         }
       } else {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) w[e] = from_f<O>(z[e]);
+        for (int e = 0; e < VEC; ++e) put(w + e, z[e]);
       }
     }
   }
   __syncthreads();
   if (tid < k) {
     const int slot = slots[row * k + tid];
-    if (slot >= sl.lo && slot < sl.lo + sl.n)
-      o[slot - sl.lo] = from_f<O>(g == 0.f ? 0.f : g * entry[row * k + tid]);
+    if (slot >= sl.lo && slot < sl.lo + sl.n) put(slot - sl.lo, g == 0.f ? 0.f : g * entry[row * k + tid]);
   }
 }
 
@@ -421,12 +436,12 @@ cudaError_t fwd_of(const VocabLaunch& l, const VocabRows& x, const DistillArgs& 
                             a.reverse, a.tail, out, words);
 }
 
-template <typename T, typename O>
+template <typename T, typename O, bool TWO = false>
 cudaError_t bwd_of(const VocabLaunch& l, const VocabRows& x, const DistillArgs& a, const DistillOut& f,
-                   const float* grad, void* out, long long ostride) {
+                   const float* grad, void* out, void* lo, long long ostride) {
   const int parts = std::max(row_parts(x.n, x.v, l.sms, 1 << 20, 16384), row_parts(x.n, x.v, l.sms, 6, 4096));
-  distill_rows_bwd_kernel<T, O><<<(unsigned)(x.n * parts), kThreads, 0, l.stream>>>(
-      (const T*)x.logits, x.stride, x.v, f.slots, f.ref, f.gs, f.entry, grad, a.k, a.tau, parts, (O*)out, ostride);
+  distill_rows_bwd_kernel<T, O, TWO><<<(unsigned)(x.n * parts), kThreads, 0, l.stream>>>(
+      (const T*)x.logits, x.stride, x.v, f.slots, f.ref, f.gs, f.entry, grad, a.k, a.tau, parts, (O*)out, (O*)lo, ostride);
   return cudaGetLastError();
 }
 
@@ -441,15 +456,19 @@ cudaError_t distill_rows_forward(const VocabLaunch& l, const VocabRows& x, const
 }
 
 cudaError_t distill_rows_backward(const VocabLaunch& l, const VocabRows& x, const DistillArgs& a, const DistillOut& f,
-                                  const float* grad, RowType otype, void* out, long long ostride) {
+                                  const float* grad, RowType otype, void* out, void* lo, long long ostride) {
+  if (lo != nullptr) {
+    if (x.type != kRowsF32 || otype != kRowsBf16) return cudaErrorInvalidValue;
+    return bwd_of<float, __nv_bfloat16, true>(l, x, a, f, grad, out, lo, ostride);
+  }
   if (x.type == kRowsF32) {
-    if (otype == kRowsF32) return bwd_of<float, float>(l, x, a, f, grad, out, ostride);
-    if (otype == kRowsBf16) return bwd_of<float, __nv_bfloat16>(l, x, a, f, grad, out, ostride);
-    return bwd_of<float, __half>(l, x, a, f, grad, out, ostride);
+    if (otype == kRowsF32) return bwd_of<float, float>(l, x, a, f, grad, out, lo, ostride);
+    if (otype == kRowsBf16) return bwd_of<float, __nv_bfloat16>(l, x, a, f, grad, out, lo, ostride);
+    return bwd_of<float, __half>(l, x, a, f, grad, out, lo, ostride);
   }
   if (otype != x.type) return cudaErrorInvalidValue;
-  if (x.type == kRowsBf16) return bwd_of<__nv_bfloat16, __nv_bfloat16>(l, x, a, f, grad, out, ostride);
-  return bwd_of<__half, __half>(l, x, a, f, grad, out, ostride);
+  if (x.type == kRowsBf16) return bwd_of<__nv_bfloat16, __nv_bfloat16>(l, x, a, f, grad, out, lo, ostride);
+  return bwd_of<__half, __half>(l, x, a, f, grad, out, lo, ostride);
 }
 
 cudaError_t distill_sort_entries(const VocabLaunch& l, const DistillArgs& a, int64_t n, int v, int* ids, float* lp) {

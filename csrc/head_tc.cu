@@ -3,7 +3,9 @@
 //
 // CTA pairs (cta_group::2): a cluster of two CTAs computes a 256 x 256 tile, each staging 128 rows of A and 128 of B
 // per 64-deep K block through a six-stage TMA ring. Where too many of such tiles' rows would be past the last one,
-// single CTAs compute 128 x 256 tiles, each staging 128 rows of A and 256 of B through four stages.
+// single CTAs compute 128 x 256 tiles, each staging 128 rows of A and 256 of B through four stages. d may come as two
+// bf16 halves, d = hi + lo (16 bits): a stage then holds both (four and three stages), and B is read once for the two
+// products that add into one accumulator.
 //   warp 0  TMA producer, warp 1 MMA issuer (one lane each; the even CTA issues for the pair), warps 2-3 idle
 //   warps 4-11  epilogue: two warps for each 32-row slab of tensor memory, half of the tile's columns each
 // The contraction is accumulated in chunks: tensor memory holds one chunk's sum (two buffers, used in turn), and the
@@ -13,11 +15,13 @@
 // the MMAs about 1000 clocks, so 2048 x 151,936 logits take 0.98 ms in chunks of 512 and 1.17 in chunks of 256. The
 // logits go by 256, the gradients, which are rounded to bf16, by 2048.
 //
-// Measured at 2048 rows x 2048 x 151,936: logits with statistics 1.17 ms (1088 TFLOP/s), kept in fp32 as well 1.25, dH
-// 0.94 ms (1360), dW 0.92 ms (1390); the library's bf16 products take 0.87 each. dH and dW keep the tensor pipe 78% and
-// 70% busy and move 14 TB/s from L2 (62 of 64 bytes a clock and SM at full rate), which bounds them; the statistics
-// themselves are hidden. At 97 rows x 2560 the weight's 778 MB bound all three (0.16, 0.14 and 0.24 ms, the last a
-// write: clearing that much memory takes 0.20).
+// Measured at 2048 rows x 2048 x 151,936: logits with statistics 1.17 ms (1088 TFLOP/s), kept in fp32 as well 1.24; with
+// d in halves dH 1.57 ms and dW 1.56 (1630 TFLOP/s of the four products), which the tensor cores bound; with d rounded
+// 0.94 and 0.93 (1360), bound by 14 TB/s from L2 (62 of 64 bytes a clock and SM at full rate). The library's bf16 products
+// take 0.87 each. What the halves are for: rounded, a row's dlogits do not sum to 0 any more, and dH is 1.1e-2 off where
+// the entries' weight rows are nearly the same, and 1.9e-3 to 3.3e-3 on random ones; in halves 1.7e-3, which is its own
+// rounding. At 97 rows x 2560 the weight's 778 MB bound all three (0.17, 0.17 and 0.31 ms, the last a write: clearing
+// that much memory takes 0.20; d rounded 0.15 and 0.28).
 //
 // Every wait is bounded (tc::mbar_wait); tensor memory is always freed. Loads have no multicast.
 #include "common.cuh"
@@ -35,11 +39,12 @@ using namespace vocab;
 constexpr int kBM = 128, kBN = 256, kBK = 64;
 constexpr int kChunkLogits = 4, kChunkGrad = 32;  // K blocks of a chunk
 constexpr uint32_t kABytes = kBM * kBK * 2;  // 16 KB
-template <bool PAIR>
+template <bool PAIR, bool TWO>  // TWO: a stage holds both halves of A
 struct Ring {
-  static constexpr int kStages = PAIR ? 6 : 4;
+  static constexpr int kStages = (PAIR ? 6 : 4) - (TWO ? (PAIR ? 2 : 1) : 0);
   static constexpr int kBRows = PAIR ? 128 : 256;  // of B in each CTA
-  static constexpr uint32_t kStageBytes = kABytes + kBRows * kBK * 2;
+  static constexpr uint32_t kAll = (TWO ? 2 : 1) * kABytes;
+  static constexpr uint32_t kStageBytes = kAll + kBRows * kBK * 2;
   static_assert(kStages * kStageBytes == 6 * 32768, "the rings take the same room");
 };
 constexpr int kEpiWarps = 8;
@@ -150,17 +155,18 @@ struct EntrySearch {
   }
 };
 
-template <bool A_MN, bool B_MN, int OUT, bool STATS, int kChunk, bool PAIR>
+template <bool A_MN, bool B_MN, int OUT, bool STATS, int kChunk, bool PAIR, bool TWO>
 __global__ void __launch_bounds__(kThreads, 1)
-    head_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
-                     const __grid_constant__ CUtensorMap tm_c, Shape shape, HeadStats st, int* __restrict__ err) {
+    head_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_a2,
+                     const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ CUtensorMap tm_c, Shape shape,
+                     HeadStats st, int* __restrict__ err) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   Bars* bars = reinterpret_cast<Bars*>(smem + kBarOff);
   const uint32_t sbase = tc::smem_addr(smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int kStages = Ring<PAIR>::kStages;
-  constexpr uint32_t kStageBytes = Ring<PAIR>::kStageBytes;
+  constexpr int kStages = Ring<PAIR, TWO>::kStages;
+  constexpr uint32_t kStageBytes = Ring<PAIR, TWO>::kStageBytes, kAll = Ring<PAIR, TWO>::kAll;
   constexpr int kTileM = PAIR ? 2 * kBM : kBM;
   const uint32_t rank = PAIR ? tc::cluster_rank() : 0;
   const int units = ((shape.m + kTileM - 1) / kTileM) * ((shape.n + kBN - 1) / kBN) * shape.splits;
@@ -194,6 +200,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 0) {
       if (lane == 0) {
         tc::prefetch_tmap(&tm_a);
+        if constexpr (TWO) tc::prefetch_tmap(&tm_a2);
         tc::prefetch_tmap(&tm_b);
         int it = 0;
         for (int u = cid; u < units; u += ncl) {
@@ -211,21 +218,25 @@ __global__ void __launch_bounds__(kThreads, 1)
               else tc::tma_load_2d(to, map, x, y, full);
             };
             uint8_t* a = smem + s * kStageBytes;
-            uint8_t* b = a + kABytes;
+            uint8_t* b = a + kAll;
             const int kx = kb * kBK;
-            if constexpr (!A_MN) {
-              load(a, &tm_a, kx, arow);  // box 64 (k) x 128 (m)
-            } else {
+            auto load_a = [&](uint8_t* to, const CUtensorMap* map) {
+              if constexpr (!A_MN) {
+                load(to, map, kx, arow);  // box 64 (k) x 128 (m)
+              } else {
 #pragma unroll
-              for (int j = 0; j < kBM / 64; ++j) load(a + j * 64 * 128, &tm_a, arow + j * 64, kx);  // [K][M]: 64 m x 64 k
-            }
+                for (int j = 0; j < kBM / 64; ++j) load(to + j * 64 * 128, map, arow + j * 64, kx);  // [K][M]: 64 m x 64 k
+              }
+            };
+            load_a(a, &tm_a);
+            if constexpr (TWO) load_a(a + kABytes, &tm_a2);
             if constexpr (!B_MN) {
 #pragma unroll
-              for (int j = 0; j < Ring<PAIR>::kBRows / 128; ++j)
+              for (int j = 0; j < Ring<PAIR, TWO>::kBRows / 128; ++j)
                 load(b + j * 128 * 128, &tm_b, kx, bcol + j * 128);  // box 64 (k) x 128 (n)
             } else {
 #pragma unroll
-              for (int j = 0; j < Ring<PAIR>::kBRows / 64; ++j)
+              for (int j = 0; j < Ring<PAIR, TWO>::kBRows / 64; ++j)
                 load(b + j * 64 * 128, &tm_b, bcol + j * 64, kx);  // [K][N]: 64 n x 64 k
             }
           }
@@ -255,15 +266,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                 break;
               }
               tc::tc_fence_after();
-              const uint32_t a = sbase + s * kStageBytes, b = a + kABytes;
-  #pragma unroll
+              const uint32_t a = sbase + s * kStageBytes, b = a + kAll;
+#pragma unroll
               for (int kk = 0; kk < kBK / 16; ++kk) {
-                const uint64_t ad = A_MN ? tc::sdesc_sw128(a + kk * 16 * 128, 64 * 128, 1024)
-                                         : tc::sdesc_sw128(a + kk * 32, 16, 1024);
                 const uint64_t bd = B_MN ? tc::sdesc_sw128(b + kk * 16 * 128, 64 * 128, 1024)
                                          : tc::sdesc_sw128(b + kk * 32, 16, 1024);
-                if constexpr (PAIR) tc::mma_bf16_pair(acc, ad, bd, idesc, kb > kc || kk > 0);
-                else tc::mma_bf16(acc, ad, bd, idesc, kb > kc || kk > 0);
+                auto product = [&](uint32_t from, bool add) {
+                  const uint64_t ad = A_MN ? tc::sdesc_sw128(from + kk * 16 * 128, 64 * 128, 1024)
+                                           : tc::sdesc_sw128(from + kk * 32, 16, 1024);
+                  if constexpr (PAIR) tc::mma_bf16_pair(acc, ad, bd, idesc, add);
+                  else tc::mma_bf16(acc, ad, bd, idesc, add);
+                };
+                product(a, kb > kc || kk > 0);
+                if constexpr (TWO) product(a + kABytes, true);
               }
               if constexpr (PAIR) tc::mma_commit_pair(&bars->empty[s]);
               else tc::mma_commit(&bars->empty[s]);
@@ -440,7 +455,7 @@ void fill_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute& attr, int ctas, c
 }
 
 // Pairs of CTAs (or CTAs) that the device holds at one time: the persistent grid.
-template <bool A_MN, bool B_MN, int OUT, bool STATS, int kChunk, bool PAIR>
+template <bool A_MN, bool B_MN, int OUT, bool STATS, int kChunk, bool PAIR, bool TWO>
 cudaError_t resident(const VocabLaunch& l, int& held) {
   static int have[16] = {0};
   int dev = 0;
@@ -448,7 +463,7 @@ cudaError_t resident(const VocabLaunch& l, int& held) {
   if (e != cudaSuccess) return e;
   int& n = have[dev & 15];
   if (n == 0) {
-    const auto kernel = head_gemm_kernel<A_MN, B_MN, OUT, STATS, kChunk, PAIR>;
+    const auto kernel = head_gemm_kernel<A_MN, B_MN, OUT, STATS, kChunk, PAIR, TWO>;
     e = l.set_smem((const void*)kernel, (int)kSmem);
     if (e != cudaSuccess) return e;
     if (PAIR) {
@@ -467,18 +482,19 @@ cudaError_t resident(const VocabLaunch& l, int& held) {
   return cudaSuccess;
 }
 
-template <bool A_MN, bool B_MN, int OUT, bool STATS, int kChunk, bool PAIR>
-cudaError_t launch_as(const VocabLaunch& l, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& c,
-                      Shape shape, const HeadStats& st, int* err) {
+template <bool A_MN, bool B_MN, int OUT, bool STATS, int kChunk, bool PAIR, bool TWO>
+cudaError_t launch_as(const VocabLaunch& l, const CUtensorMap& a, const CUtensorMap& a2, const CUtensorMap& b,
+                      const CUtensorMap& c, Shape shape, const HeadStats& st, int* err) {
   shape.tile = PAIR ? 2 * kBM : kBM;
   int held = 0;
-  const cudaError_t e = resident<A_MN, B_MN, OUT, STATS, kChunk, PAIR>(l, held);
+  const cudaError_t e = resident<A_MN, B_MN, OUT, STATS, kChunk, PAIR, TWO>(l, held);
   if (e != cudaSuccess) return e;
   const int units = ((shape.m + shape.tile - 1) / shape.tile) * ((shape.n + kBN - 1) / kBN) * shape.splits;
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute attr;
   fill_config<PAIR>(cfg, attr, (PAIR ? 2 : 1) * std::min(units, held), l.stream);
-  return cudaLaunchKernelEx(&cfg, head_gemm_kernel<A_MN, B_MN, OUT, STATS, kChunk, PAIR>, a, b, c, shape, st, err);
+  return cudaLaunchKernelEx(&cfg, head_gemm_kernel<A_MN, B_MN, OUT, STATS, kChunk, PAIR, TWO>, a, a2, b, c, shape, st,
+                            err);
 }
 
 // Pairs or single CTAs: a pair's tile takes 7% less time a row (logits of 2048 rows 1.25 ms, of single CTAs 1.35) but
@@ -488,11 +504,11 @@ bool in_pairs(int rows) {
   return 100ll * single >= 93ll * pairs;
 }
 
-template <bool A_MN, bool B_MN, int OUT, bool STATS, int kChunk>
-cudaError_t launch(const VocabLaunch& l, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& c,
-                   const Shape& shape, const HeadStats& st, int* err) {
-  if (in_pairs(shape.m)) return launch_as<A_MN, B_MN, OUT, STATS, kChunk, true>(l, a, b, c, shape, st, err);
-  return launch_as<A_MN, B_MN, OUT, STATS, kChunk, false>(l, a, b, c, shape, st, err);
+template <bool A_MN, bool B_MN, int OUT, bool STATS, int kChunk, bool TWO>
+cudaError_t launch(const VocabLaunch& l, const CUtensorMap& a, const CUtensorMap& a2, const CUtensorMap& b,
+                   const CUtensorMap& c, const Shape& shape, const HeadStats& st, int* err) {
+  if (in_pairs(shape.m)) return launch_as<A_MN, B_MN, OUT, STATS, kChunk, true, TWO>(l, a, a2, b, c, shape, st, err);
+  return launch_as<A_MN, B_MN, OUT, STATS, kChunk, false, TWO>(l, a, a2, b, c, shape, st, err);
 }
 
 }  // namespace
@@ -503,8 +519,8 @@ int head_parts(int v) { return 2 * ((v + kBN - 1) / kBN); }
 int head_splits(const VocabLaunch& l, int rows, int d, int v) {
   const bool two = in_pairs(rows);
   int pairs = 0;
-  const cudaError_t e = two ? resident<false, true, kF32, false, kChunkGrad, true>(l, pairs)
-                            : resident<false, true, kF32, false, kChunkGrad, false>(l, pairs);
+  const cudaError_t e = two ? resident<false, true, kF32, false, kChunkGrad, true, false>(l, pairs)
+                            : resident<false, true, kF32, false, kChunkGrad, false, false>(l, pairs);
   if (e != cudaSuccess) return 1;
   const int tile = two ? 2 * kBM : kBM;
   const int tiles = ((rows + tile - 1) / tile) * ((d + kBN - 1) / kBN);
@@ -526,20 +542,26 @@ int head_splits(const VocabLaunch& l, int rows, int d, int v) {
 cudaError_t head_logits(const VocabLaunch& l, const CUtensorMap& h, const CUtensorMap& w, const CUtensorMap* out,
                         int rows, int d, int v, const HeadStats& st, int* err) {
   const Shape s{rows, v, d, 0, 1, 0};
-  if (out != nullptr) return launch<false, false, kF32, true, kChunkLogits>(l, h, w, *out, s, st, err);
-  return launch<false, false, kNone, true, kChunkLogits>(l, h, w, h, s, st, err);
+  if (out != nullptr) return launch<false, false, kF32, true, kChunkLogits, false>(l, h, h, w, *out, s, st, err);
+  return launch<false, false, kNone, true, kChunkLogits, false>(l, h, h, w, h, s, st, err);
 }
 
 cudaError_t head_logits_again(const VocabLaunch& l, const CUtensorMap& h, const CUtensorMap& w, const CUtensorMap& out,
                               int rows, int d, int v, int* err) {
-  return launch<false, false, kF32, false, kChunkLogits>(l, h, w, out, Shape{rows, v, d, 0, 1, 0}, HeadStats{}, err);
+  return launch<false, false, kF32, false, kChunkLogits, false>(l, h, h, w, out, Shape{rows, v, d, 0, 1, 0}, HeadStats{},
+                                                                err);
 }
 
-cudaError_t head_dh(const VocabLaunch& l, const CUtensorMap& dl, const CUtensorMap& w, const CUtensorMap& out, int rows,
-                    int d, int v, int splits, int split_rows, const float* parts, void* dh, int* err) {
+cudaError_t head_dh(const VocabLaunch& l, const CUtensorMap& dl, const CUtensorMap* lo, const CUtensorMap& w,
+                    const CUtensorMap& out, int rows, int d, int v, int splits, int split_rows, const float* parts,
+                    void* dh, int* err) {
   const Shape s{rows, d, v, 0, splits, split_rows};
-  if (splits == 1) return launch<false, true, kBf16, false, kChunkGrad>(l, dl, w, out, s, HeadStats{}, err);
-  const cudaError_t e = launch<false, true, kF32, false, kChunkGrad>(l, dl, w, out, s, HeadStats{}, err);
+  const HeadStats none{};
+  if (splits == 1)
+    return lo ? launch<false, true, kBf16, false, kChunkGrad, true>(l, dl, *lo, w, out, s, none, err)
+              : launch<false, true, kBf16, false, kChunkGrad, false>(l, dl, dl, w, out, s, none, err);
+  const cudaError_t e = lo ? launch<false, true, kF32, false, kChunkGrad, true>(l, dl, *lo, w, out, s, none, err)
+                           : launch<false, true, kF32, false, kChunkGrad, false>(l, dl, dl, w, out, s, none, err);
   if (e != cudaSuccess) return e;
   const long long n4 = (long long)rows * d / 4;
   const int blocks = (int)std::min<long long>((n4 + 255) / 256, 8ll * l.sms);
@@ -547,9 +569,11 @@ cudaError_t head_dh(const VocabLaunch& l, const CUtensorMap& dl, const CUtensorM
   return cudaGetLastError();
 }
 
-cudaError_t head_dw(const VocabLaunch& l, const CUtensorMap& dl, const CUtensorMap& h, const CUtensorMap& out, int rows,
-                    int d, int v, int* err) {
-  return launch_as<true, true, kBf16, false, kChunkGrad, true>(l, dl, h, out, Shape{v, d, rows, 0, 1, 0}, HeadStats{}, err);
+cudaError_t head_dw(const VocabLaunch& l, const CUtensorMap& dl, const CUtensorMap* lo, const CUtensorMap& h,
+                    const CUtensorMap& out, int rows, int d, int v, int* err) {
+  const Shape s{v, d, rows, 0, 1, 0};
+  return lo ? launch_as<true, true, kBf16, false, kChunkGrad, true, true>(l, dl, *lo, h, out, s, HeadStats{}, err)
+            : launch_as<true, true, kBf16, false, kChunkGrad, true, false>(l, dl, dl, h, out, s, HeadStats{}, err);
 }
 
 }  // namespace ts

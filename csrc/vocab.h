@@ -65,7 +65,7 @@ cudaError_t vocab_sample(const VocabLaunch& l, const VocabRows& x, const float* 
                          const SampleArgs& a, int64_t* tokens, float* lp);
 cudaError_t distill_rows_forward(const VocabLaunch& l, const VocabRows& x, const DistillArgs& a, const DistillOut& out);
 cudaError_t distill_rows_backward(const VocabLaunch& l, const VocabRows& x, const DistillArgs& a, const DistillOut& f,
-                                  const float* grad, RowType otype, void* out, long long ostride);
+                                  const float* grad, RowType otype, void* out, void* lo, long long ostride);
 // entries in ascending order of their tokens, those that do not count last (token 0x7fffffff)
 cudaError_t distill_sort_entries(const VocabLaunch& l, const DistillArgs& a, int64_t n, int v, int* ids, float* lp);
 // loss and gradient coefficients from the head's statistics; `lp` sorted as st.ids
@@ -80,10 +80,12 @@ cudaError_t head_logits(const VocabLaunch& l, const CUtensorMap& h, const CUtens
                         int rows, int d, int v, const HeadStats& st, int* err);
 cudaError_t head_logits_again(const VocabLaunch& l, const CUtensorMap& h, const CUtensorMap& w, const CUtensorMap& out,
                               int rows, int d, int v, int* err);
-cudaError_t head_dh(const VocabLaunch& l, const CUtensorMap& dl, const CUtensorMap& w, const CUtensorMap& out, int rows,
-                    int d, int v, int splits, int split_rows, const float* parts, void* dh, int* err);
-cudaError_t head_dw(const VocabLaunch& l, const CUtensorMap& dl, const CUtensorMap& h, const CUtensorMap& out, int rows,
-                    int d, int v, int* err);
+// dlogits in two bf16 halves, or (`lo` null) rounded to bf16
+cudaError_t head_dh(const VocabLaunch& l, const CUtensorMap& dl, const CUtensorMap* lo, const CUtensorMap& w,
+                    const CUtensorMap& out, int rows, int d, int v, int splits, int split_rows, const float* parts,
+                    void* dh, int* err);
+cudaError_t head_dw(const VocabLaunch& l, const CUtensorMap& dl, const CUtensorMap* lo, const CUtensorMap& h,
+                    const CUtensorMap& out, int rows, int d, int v, int* err);
 
 cudaError_t distill_bounds(unsigned long long* word, bool reset);
 

@@ -121,13 +121,21 @@ std::vector<at::Tensor> distill_rows_fwd(const at::Tensor& logits, const at::Ten
 }
 
 // The gradient of the logits for upstream gradients grad [N] fp32, in `out` [N, V] (its rows may be strided): the
-// logits' type, or bf16 / fp16 for fp32 logits.
+// logits' type, or bf16 / fp16 for fp32 logits. With `lo` (fp32 logits, both bf16) the two add up to the gradient.
 void distill_rows_bwd(const at::Tensor& logits, const at::Tensor& slots, const at::Tensor& ref, const at::Tensor& gs,
-                      const at::Tensor& entry, const at::Tensor& grad, double tau, at::Tensor& out) {
+                      const at::Tensor& entry, const at::Tensor& grad, double tau, at::Tensor& out,
+                      const c10::optional<at::Tensor>& lo) {
   const VocabRows x = rows_of(logits, "logits");
   check_rows(out, "gradient");
   check_cuda(grad, "grad");
   TS_CHECK(out.sizes() == logits.sizes() && out.device() == logits.device(), "the gradient must have the logits' shape");
+  if (lo) {
+    check_rows(*lo, "gradient");
+    TS_CHECK(lo->sizes() == out.sizes() && lo->device() == out.device() && lo->strides() == out.strides() &&
+                 lo->scalar_type() == at::kBFloat16 && out.scalar_type() == at::kBFloat16 &&
+                 logits.scalar_type() == at::kFloat,
+             "the gradient's halves must be two bf16 tensors of one layout, of fp32 logits");
+  }
   TS_CHECK(grad.scalar_type() == at::kFloat && grad.dim() == 1 && grad.size(0) == x.n, "grad must be fp32 [N]");
   const c10::cuda::CUDAGuard guard(logits.device());
   if (x.n == 0) return;
@@ -135,7 +143,7 @@ void distill_rows_bwd(const at::Tensor& logits, const at::Tensor& slots, const a
   const DistillOut f{nullptr, slots.data_ptr<int>(), ref.data_ptr<float>(), gs.data_ptr<float>(),
                      entry.data_ptr<float>()};
   TS_CUDA_CHECK(distill_rows_backward(launch_on(logits), x, a, f, grad.data_ptr<float>(), row_type(out, "gradient"),
-                                      out.data_ptr(), (long long)out.stride(0)));
+                                      out.data_ptr(), lo ? lo->data_ptr() : nullptr, (long long)out.stride(0)));
 }
 
 namespace {
@@ -171,7 +179,7 @@ struct DistillRows : torch::autograd::Function<DistillRows> {
         const at::AutoGradMode off(false);
         d = at::empty(s[0].sizes(), s[0].options());
         distill_rows_bwd(s[0], s[1], s[2], s[3], s[4], grads[0].to(at::kFloat).contiguous(),
-                         ctx->saved_data["tau"].toDouble(), d);
+                         ctx->saved_data["tau"].toDouble(), d, c10::nullopt);
       }
       if (at::GradMode::is_enabled()) d = DifferentiatedOnce::apply(d, s[0], grads[0]);  // (create_graph)
     }
@@ -268,9 +276,18 @@ at::Tensor distill_head_logits(const at::Tensor& h, const at::Tensor& w) {
   return out;
 }
 
-// dH [N, D] = d [N, V] · weight [V, D], bf16
-void distill_head_dh(const at::Tensor& dl, const at::Tensor& w, at::Tensor& dh) {
+namespace {
+void check_halves(const at::Tensor& dl, const c10::optional<at::Tensor>& lo) {
   check_bf16(dl, "dlogits");
+  if (!lo) return;
+  check_bf16(*lo, "dlogits");
+  TS_CHECK(lo->sizes() == dl.sizes() && lo->device() == dl.device(), "the halves of the dlogits differ in shape");
+}
+}  // namespace
+
+// dH [N, D] = (d + lo) [N, V] · weight [V, D], bf16
+void distill_head_dh(const at::Tensor& dl, const c10::optional<at::Tensor>& lo, const at::Tensor& w, at::Tensor& dh) {
+  check_halves(dl, lo);
   check_bf16(w, "weight");
   check_bf16(dh, "dhidden");
   const int64_t n = dl.size(0), v = dl.size(1), d = w.size(1);
@@ -284,20 +301,25 @@ void distill_head_dh(const at::Tensor& dl, const at::Tensor& w, at::Tensor& dh) 
   const int split_rows = (int)((n + 255) / 256 * 256);  // whole tiles: a slice's last one writes no row of the next
   at::Tensor parts;
   if (splits > 1) parts = at::empty({(int64_t)splits * split_rows, d}, dl.options().dtype(at::kFloat));
-  TS_CUDA_CHECK(head_dh(l, k_rows(dl), k_cols(w), out_map(splits > 1 ? parts : dh), (int)n, (int)d, (int)v, splits,
-                        split_rows, splits > 1 ? parts.data_ptr<float>() : nullptr, dh.data_ptr(), error_word(dl)));
+  CUtensorMap low{};
+  if (lo) low = k_rows(*lo);
+  TS_CUDA_CHECK(head_dh(l, k_rows(dl), lo ? &low : nullptr, k_cols(w), out_map(splits > 1 ? parts : dh), (int)n, (int)d,
+                        (int)v, splits, split_rows, splits > 1 ? parts.data_ptr<float>() : nullptr, dh.data_ptr(),
+                        error_word(dl)));
 }
 
-// dW [V, D] = dᵀ [V, N] · hidden [N, D], bf16
-at::Tensor distill_head_dw(const at::Tensor& dl, const at::Tensor& h) {
-  check_bf16(dl, "dlogits");
+// dW [V, D] = (d + lo)ᵀ [V, N] · hidden [N, D], bf16
+at::Tensor distill_head_dw(const at::Tensor& dl, const c10::optional<at::Tensor>& lo, const at::Tensor& h) {
+  check_halves(dl, lo);
   check_bf16(h, "hidden");
   TS_CHECK(dl.size(0) == h.size(0) && dl.device() == h.device(), "distill_head_dw shapes");
   const c10::cuda::CUDAGuard guard(dl.device());
   auto dw = at::empty({dl.size(1), h.size(1)}, dl.options());
   if (h.size(0) == 0) return dw.zero_();
-  TS_CUDA_CHECK(head_dw(launch_on(dl), k_cols(dl), k_cols(h), out_map(dw), (int)h.size(0), (int)h.size(1),
-                        (int)dl.size(1), error_word(dl)));
+  CUtensorMap low{};
+  if (lo) low = k_cols(*lo);
+  TS_CUDA_CHECK(head_dw(launch_on(dl), k_cols(dl), lo ? &low : nullptr, k_cols(h), out_map(dw), (int)h.size(0),
+                        (int)h.size(1), (int)dl.size(1), error_word(dl)));
   return dw;
 }
 

@@ -191,6 +191,41 @@ def test_gradient_of_a_far_tail(device, dtype, direction, temperature):
             assert bool((err <= allowed).all()), (GAPS[i], float((err - allowed).max()))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("direction", ["forward", "reverse"])
+@pytest.mark.parametrize("temperature", [1.0, 0.125])
+def test_head_gradient_of_a_far_tail(direction, temperature):
+    """The same through the LM head: logits of the entries are a column of the weight times the gap, exact in bf16.
+    Tolerances of the bf16 head: 5e-3 of the norm, for the entries' rows of the weight gradient and for the others'."""
+    n, d, v, k = len(GAPS), 64, 2056, 4
+    g = torch.Generator().manual_seed(1)
+    w = torch.randn(v, d, generator=g) * 0.1
+    ids = torch.tensor([5, 700, 1535, v - 1])
+    w[:, 0] = 0.0
+    w[ids] = 0.0
+    w[ids, 0] = torch.tensor([1.0, 0.984375, 0.9921875, 0.96875])
+    h = torch.randn(n, d, generator=g)
+    h[:, 0] = torch.tensor(GAPS)
+    h = h * temperature
+    w, h = w.to(torch.bfloat16), h.to(torch.bfloat16)
+    ids = ids.expand(n, k).contiguous()
+    lp = torch.log(torch.tensor([0.5, 0.25, 0.15, 0.05])).expand(n, k).contiguous()
+    for r in range(n):  # one row at a time: each row's own part of the weight gradient
+        hr, wr = h[r:r + 1].cuda().requires_grad_(True), w.cuda().requires_grad_(True)
+        loss = lm_head_topk_distill(hr, wr, ids[:1].cuda(), lp[:1].cuda(), temperature=temperature,
+                                    direction=direction)
+        got = torch.autograd.grad(loss.sum(), (hr, wr))
+        h64, w64 = h[r:r + 1].double().requires_grad_(True), w.double().requires_grad_(True)
+        want = _loss_64((h64 @ w64.t())[0], ids[0], lp[0], temperature, direction)
+        ref = torch.autograd.grad(want, (h64, w64))
+        assert _near(float(loss.detach()), float(want.detach()), 5e-6, 3e-5), (GAPS[r], loss, want)
+        outside = torch.ones(v, dtype=torch.bool)
+        outside[ids[0]] = False
+        for a, b in ((got[0], ref[0]), (got[1].cpu()[outside], ref[1][outside]), (got[1].cpu()[~outside], ref[1][~outside])):
+            off = float((a.cpu().double() - b).norm())
+            assert off <= 5e-3 * float(b.norm()) + 1e-36, (GAPS[r], off, float(b.norm()))
+
+
 # ------------------------------------------------------------------ masks of finite values, offsets, cold rows
 def _teacher_64(v, k, seed):
     g = torch.Generator().manual_seed(seed)
@@ -289,6 +324,124 @@ def test_cold_rows(device, temperature):
     z[4, [40, 4000, 8000]] = 60.0
     _check_rows(z.to(device), temperature, settings=(dict(), dict(top_k=20, top_p=0.95), dict(top_p=0.9),
                                                      dict(top_p=0.4), dict(min_p=0.05)))
+
+
+# ------------------------------------------------------------------ the LM head's products at more shapes
+def _head_shape(n, d, v, k, dtype, seed):
+    """Random rows with entries at the edges of the products' tiles, some short, some without any."""
+    g = torch.Generator().manual_seed(seed)
+    w = (torch.randn(v, d, generator=g) * (2.5 / math.sqrt(d))).to(dtype).cuda()
+    h = torch.randn(n, d, generator=g).to(dtype).cuda()
+    z = h.double() @ w.double().t()
+    lp, ids = torch.log_softmax(z + torch.randn(n, v, generator=g).cuda(), -1).topk(k)
+    edges = torch.tensor([0, 127, 128, 255, 256, v - 1], device="cuda")
+    ids[::2, -6:], lp[::2, -6:] = edges, -6.0
+    for j in range(k - 6):  # (an edge that was among the others already counts once)
+        ids[::2, j] = torch.where((ids[::2, j, None] == edges).any(-1), -1, ids[::2, j])
+    ids[1::5, k // 2:] = -1
+    ids[3::7] = -1
+    lp[4::9, 1] = -math.inf
+    up = torch.rand(n, generator=g).cuda()
+    return h.requires_grad_(True), w.requires_grad_(True), ids, lp.float(), up
+
+
+def _head_64(h, w, ids, lp, up, temperature, direction):
+    """(loss, d hidden, d weight) in 64 bits, from the definition."""
+    h, w = (x.detach().double().requires_grad_(True) for x in (h, w))
+    logp = torch.log_softmax(h @ w.t() / temperature, -1)
+    have = (ids >= 0) & (lp > -math.inf)
+    t = torch.where(have, lp.double(), 0.0)
+    at = ids.clamp(min=0)
+    a = torch.where(have, logp.gather(-1, at), 0.0)
+    weight = torch.where(have, (t if direction == "forward" else a).exp(), 0.0)
+    inside = torch.zeros_like(logp, dtype=torch.bool)
+    rows = torch.arange(len(ids), device=ids.device)[:, None].expand_as(ids)
+    inside[rows[have], ids[have]] = True
+    lpt = torch.logsumexp(logp.masked_fill(inside, -math.inf), -1)
+    q = (1.0 - torch.where(have, t.exp(), 0.0).sum(-1)).clamp(min=1e-7)
+    if direction == "forward":
+        loss = (weight * (t - a)).sum(-1) + q * (q.log() - lpt)
+    else:
+        loss = (weight * (a - t)).sum(-1) + lpt.exp() * (lpt - q.log())
+    loss = torch.where(have.any(-1), loss, 0.0)
+    return (loss.detach(), *torch.autograd.grad(loss, (h, w), up.double()))
+
+
+HEADS = [  # rows by pairs of CTAs (512, 2100, 2304, 1024) and by single ones, contractions of several chunks, odd tiles
+    (300, 1032, 5008, 16), (257, 2048, 4104, 32), (512, 1000, 4104, 16), (600, 1024, 2056, 8), (2304, 264, 1032, 8),
+    (2100, 520, 2056, 16), (97, 2560, 4104, 64), (40, 4096, 8200, 256), (1024, 1304, 1288, 12), (1, 2048, 12296, 8)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,d,v,k", HEADS)
+@pytest.mark.parametrize("direction,temperature", [("forward", 1.0), ("reverse", 1.4)])
+@pytest.mark.parametrize("rounded", [False, True])
+def test_head_products(n, d, v, k, direction, temperature, rounded):
+    """The loss as in ``test_head_gpu``. Gradients: the dlogits' halves hold 2^-17 of them, so what counts is the rounding
+    to bf16, a relative 2^-8 / sqrt(3) of a norm at most where all its values lie at the foot of their binade, and 2^-8
+    for the worst value; rounded dlogits add as much again, and are held to 5e-3 as there."""
+    h, w, ids, lp, up = _head_shape(n, d, v, k, torch.bfloat16, n + d)
+    loss = lm_head_topk_distill(h, w, ids, lp, temperature=temperature, direction=direction, round_dlogits=rounded)
+    got = torch.autograd.grad(loss, (h, w), up)
+    want, *grads = _head_64(h, w, ids, lp, up, temperature, direction)
+    torch.testing.assert_close(loss.detach().double(), want, rtol=5e-6, atol=3e-5)
+    for a, b in zip(got, grads):
+        assert a.dtype == torch.bfloat16 and a.shape == b.shape
+        rel = float((a.double() - b).norm() / b.norm())
+        assert rel <= (5e-3 if rounded else 2.3e-3), rel
+        if not rounded:
+            off, size = (a.double() - b).norm(dim=-1), b.norm(dim=-1)
+            assert bool((off <= 2.0 ** -8 * size).all()), float((off / size).nan_to_num().max())
+            assert not bool(a[size == 0].any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,d,v,rows", [(700, 264, 2056, 256), (60, 256, 1003, 2048), (300, 1032, 1003, 128)])
+@pytest.mark.parametrize("sink", [False, True])
+def test_head_in_blocks_and_odd_vocabularies(n, d, v, rows, sink):
+    """Several blocks, and vocabularies that are no multiple of 8, whose gradients are formed in fp32. A sink holds the
+    weight gradient in fp32: 2^-17 of each dlogit, and fp32 sums."""
+    from thundersync_b200.ops.sink import GradSink, ParamArena, grad_sink
+
+    h, w, ids, lp, up = _head_shape(n, d, v, 16, torch.bfloat16, n + v)
+    _, dh, dw = _head_64(h, w, ids, lp, up, 1.0, "forward")
+    if not sink:
+        got = torch.autograd.grad(lm_head_topk_distill(h, w, ids, lp, rows=rows), (h, w), up)
+        for a, b in zip(got, (dh, dw)):
+            assert float((a.double() - b).norm() / b.norm()) <= 2.3e-3
+        return
+    lin = torch.nn.Linear(d, v, bias=False, device="cuda", dtype=torch.bfloat16)
+    lin.weight.data.copy_(w.detach())
+    arena = ParamArena(list(lin.parameters()))
+    into = GradSink(arena, arena.new_buffer(torch.float32))
+    with grad_sink(into):
+        lm_head_topk_distill(h, lin.weight, ids, lp, rows=rows).backward(up)
+    assert float((into.view(lin.weight).double() - dw).norm() / dw.norm()) <= 2e-5
+    assert float((h.grad.double() - dh).norm() / dh.norm()) <= 2.3e-3
+
+
+@pytest.mark.gpu
+def test_head_fp16():
+    """Gradients rounded once to fp16: 2^-11 / sqrt(3) of the norm, and half of the least subnormal number a value."""
+    h, w, ids, lp, up = _head_shape(90, 128, 1000, 16, torch.float16, 3)
+    loss = lm_head_topk_distill(h, w, ids, lp)
+    got = torch.autograd.grad(loss, (h, w), up)
+    want, *grads = _head_64(h, w, ids, lp, up, 1.0, "forward")
+    torch.testing.assert_close(loss.detach().double(), want, rtol=5e-6, atol=3e-5)
+    for a, b in zip(got, grads):
+        assert a.dtype == torch.float16
+        allowed = 2.0 ** -11 / math.sqrt(3) * float(b.norm()) + 2.0 ** -25 * math.sqrt(b.numel())
+        assert float((a.double() - b).norm()) <= allowed
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_head_cpu_rounds_gradients_once(dtype):
+    h, w, ids, lp = _head_inputs(9, 40, 203, 6, "cpu", dtype)
+    got = torch.autograd.grad(lm_head_topk_distill(h, w, ids, lp).sum(), (h, w))
+    _, *grads = _head_64(h, w, ids, lp, torch.ones(9), 1.0, "forward")
+    eps = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -11
+    for a, b in zip(got, grads):
+        assert bool(((a.double() - b).abs() <= 0.51 * eps * 2 * b.abs() + 1e-6 * b.abs().max() + 2.0 ** -25).all())
 
 
 # ------------------------------------------------------------------ what the LM head's node holds

@@ -170,8 +170,8 @@ def topk_distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
 
 # ------------------------------------------------------------------ the loss from hidden states
 # Rows of a block, where the caller names none: a block's buffers are its fp32 logits (2.5 GB at 4096 rows of a
-# 151,936-token vocabulary) and bf16 dlogits (half of that). One block writes the weight gradient in bf16 at once;
-# several add fp32 products and round at the end.
+# 151,936-token vocabulary) and the two bf16 halves of its dlogits (as much again). One block writes the weight gradient
+# in bf16 at once; several add fp32 products and round at the end.
 BLOCK_ROWS = 4096
 # The forwards' fp32 logits that a process keeps on a device for their backwards, in bytes, of all graphs that are alive
 # together. A block past it computes them again, which at 2048 rows x 2048 x 151,936 takes a third of the backward's time
@@ -232,9 +232,10 @@ class _DifferentiatedOnce(torch.autograd.Function):
 
 class _HeadTopkDistill(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hidden, weight, ids, logprobs, rows, temperature, direction, tail, differentiated):
+    def forward(ctx, hidden, weight, ids, logprobs, rows, temperature, direction, tail, round_dlogits,
+                differentiated):
         n = hidden.shape[0]
-        ctx.conf = (rows, temperature, direction, tail)
+        ctx.conf = (rows, temperature, direction, tail, round_dlogits)
         ctx.param = weight  # for the sink, which knows its parameters by identity
         ctx.kept = []  # logits of the blocks that keep theirs: a first backward uses them up, another computes them again
         saved = []  # four small tensors of each block
@@ -272,12 +273,12 @@ class _HeadTopkDistill(torch.autograd.Function):
             grads = _HeadTopkDistill._gradients(ctx, g)
         if torch.is_grad_enabled():  # (create_graph)
             grads = [None if d is None else _DifferentiatedOnce.apply(d, hidden, weight, g) for d in grads]
-        return (*grads, None, None, None, None, None, None, None)
+        return (*grads, None, None, None, None, None, None, None, None)
 
     @staticmethod
     def _gradients(ctx, g):
         hidden, weight, ids, logprobs, *saved = ctx.saved_tensors
-        rows, temperature, direction, tail = ctx.conf
+        rows, temperature, direction, tail, round_dlogits = ctx.conf
         n = hidden.shape[0]
         need_h, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
         fused = _fused_ok(hidden, weight)
@@ -296,47 +297,56 @@ class _HeadTopkDistill(torch.autograd.Function):
             logits = ctx.kept[i].take() if ctx.kept and ctx.kept[i] is not None else None
             if logits is None:
                 logits = native().distill_head_logits(h, weight) if fused else _logits_fp32(h, weight)
+            parts = []  # of the dlogits, which are their sum
             if _native_rows(logits):
-                d = torch.empty(logits.shape, dtype=hidden.dtype, device=hidden.device)
-                native().distill_rows_bwd(logits, *saved[4 * i:4 * i + 4], g[r0:r1].float(), temperature, d)
+                dtype = hidden.dtype if fused or round_dlogits else torch.float32
+                parts.append(torch.empty(logits.shape, dtype=dtype, device=hidden.device))
+                if fused and not round_dlogits:
+                    parts.append(torch.empty_like(parts[0]))
+                native().distill_rows_bwd(logits, *saved[4 * i:4 * i + 4], g[r0:r1].float(), temperature, parts[0],
+                                          parts[1] if len(parts) > 1 else None)
             else:
                 with torch.enable_grad():
                     z = logits.requires_grad_(True)
                     part = _loss_reference(z, ids[r0:r1], logprobs[r0:r1], temperature, direction, tail)
                 (d,) = torch.autograd.grad(part, z, g[r0:r1].to(part.dtype))
-                d = d.to(hidden.dtype)
+                parts.append(d.to(hidden.dtype) if round_dlogits else d)
             del logits
             if need_h:
                 if fused:
-                    native().distill_head_dh(d, weight, dh[r0:r1])
+                    native().distill_head_dh(parts[0], parts[1] if len(parts) > 1 else None, weight, dh[r0:r1])
+                elif parts[0].dtype == weight.dtype:
+                    gemm(parts[0], weight, b_t=False, out=dh[r0:r1])
                 else:
-                    gemm(d, weight, b_t=False, out=dh[r0:r1])
+                    dh[r0:r1] = torch.mm(parts[0], weight.to(parts[0].dtype))
             if at_once:
-                dw = native().distill_head_dw(d, h)
+                dw = native().distill_head_dw(parts[0], parts[1] if len(parts) > 1 else None, h)
             elif need_w:
-                d8, h8 = _to_eight(d, h) if d.is_cuda else (d, h)
-                if sink_w:
-                    s.addmm_(s.view(ctx.param), d8, h8)
-                else:
-                    gemm_accumulate(dw, d8, h8, a_t=True, b_t=False)
+                for d in parts:
+                    d8, h8 = _to_eight(d, h) if d.is_cuda else (d, h)
+                    if sink_w:
+                        s.addmm_(s.view(ctx.param), d8, h8)
+                    else:
+                        gemm_accumulate(dw, d8, h8, a_t=True, b_t=False)
         return dh, None if dw is None else dw.to(weight.dtype)
 
 
 def lm_head_topk_distill(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torch.Tensor,
                          teacher_logprobs: torch.Tensor, *, temperature: float = 1.0, direction: str = "forward",
-                         tail: bool = True, rows: int | None = None) -> torch.Tensor:
+                         tail: bool = True, rows: int | None = None, round_dlogits: bool = False) -> torch.Tensor:
     """Loss [N] (fp32) of the student ``hidden`` [N, D] · ``weight`` [V, D]ᵀ against the teacher's entries [N, K],
     differentiable in ``hidden`` and ``weight`` (whose gradient honours an active gradient sink).
 
     ``rows`` rows are worked at a time (default ``BLOCK_ROWS``), and up to ``KEEP_LOGITS_BYTES`` of fp32 logits, of all
     graphs of a process on a device together, stay from their forwards to their backwards; both are attributes of this
-    module. Hidden rows must be finite: a row without
-    entries gives no gradient, but its zeros meet the hidden row in the weight gradient.
+    module. Hidden rows must be finite: a row without entries gives no gradient, but its zeros meet the hidden row in the
+    weight gradient.
 
-    In bf16 the dlogits are rounded to bf16 before the two gradient products, as in :func:`lm_head_logprob`: the
-    tensor cores take both operands in one type, and the weight is bf16. The gradients are then 1.9e-3 to 3.0e-3 of
-    their norm from 64 bits, depending on the inputs, where fp32 products rounded once at the end are 1.7e-3. Two
-    bf16 halves of the dlogits would mend that and double both products (0.94 and 0.92 of 3.9 ms at 2048 rows)."""
+    The tensor cores take both operands of a product in one type, and the weight is bf16. So the dlogits go into the two
+    gradient products as two bf16 halves (16 bits), and the gradients are rounded once, to their type: about 1.7e-3 of
+    their norm in bf16. ``round_dlogits=True`` rounds the dlogits to the hidden states' type instead, as
+    :func:`lm_head_logprob` does, for half the arithmetic: the gradients are then 1.9e-3 to 3.3e-3 from 64 bits, and more
+    where the dlogits of a row cancel in ``d · weight`` (1.1e-2 where the entries' weight rows are nearly the same)."""
     if hidden.dim() != 2:
         raise ValueError(f"hidden must be [N, D], got {tuple(hidden.shape)}")
     if weight.dim() != 2 or weight.shape[1] != hidden.shape[1]:
@@ -349,4 +359,5 @@ def lm_head_topk_distill(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids
     if h.is_cuda and h.data_ptr() % 16:  # the GEMMs' loads begin on 16-byte boundaries
         h = h.clone()
     differentiated = torch.is_grad_enabled() and (h.requires_grad or weight.requires_grad)
-    return _HeadTopkDistill.apply(h, weight, ids, lp, rows, float(temperature), direction, bool(tail), differentiated)
+    return _HeadTopkDistill.apply(h, weight, ids, lp, rows, float(temperature), direction, bool(tail),
+                                  bool(round_dlogits), differentiated)
