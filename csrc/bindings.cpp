@@ -80,6 +80,7 @@ void register_ipc(pybind11::module& m);
 uint64_t bounds_word_rowops(bool reset);
 uint64_t bounds_word_fold(bool reset);
 uint64_t bounds_word_distill(bool reset);
+int64_t more_launches(bool reset);
 std::vector<at::Tensor> topk_logprobs(const at::Tensor& logits, int64_t k, double temperature);
 std::vector<at::Tensor> sample_tokens(const at::Tensor& logits, const c10::optional<at::Tensor>& noise,
                                       const c10::optional<at::Tensor>& temperature_t, double temperature,
@@ -245,6 +246,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("distill_rows_fwd", &ts::distill_rows_fwd);
   m.def("distill_rows_bwd", &ts::distill_rows_bwd);
   m.def("distill_rows", &ts::distill_rows);
+  m.def("more_launches", &ts::more_launches);
   m.def("distill_head_fwd", &ts::distill_head_fwd);
   m.def("distill_head_logits", &ts::distill_head_logits);
   m.def("distill_head_dh", &ts::distill_head_dh);

@@ -2,6 +2,8 @@
 #include "common.h"
 #include "vocab.h"
 
+#include <atomic>
+
 namespace ts {
 
 CUtensorMap make_bf16_map(const void* base, uint64_t inner, uint64_t outer, uint64_t row_stride_elems,
@@ -10,6 +12,8 @@ CUtensorMap make_out_map(void* base, bool f32, uint64_t cols, uint64_t rows, uin
 at::Tensor& tc_error_flag(const at::Device& dev);
 
 namespace {
+
+std::atomic<int64_t> g_more_launches{0};
 
 void check_rows(const at::Tensor& t, const char* name) {
   TS_CHECK(t.is_cuda() && t.dim() == 2, name, " must be a CUDA matrix");
@@ -180,6 +184,7 @@ struct DistillRows : torch::autograd::Function<DistillRows> {
         d = at::empty(s[0].sizes(), s[0].options());
         distill_rows_bwd(s[0], s[1], s[2], s[3], s[4], grads[0].to(at::kFloat).contiguous(),
                          ctx->saved_data["tau"].toDouble(), d, c10::nullopt);
+        if (d.size(0) > 0) ++g_more_launches;
       }
       if (at::GradMode::is_enabled()) d = DifferentiatedOnce::apply(d, s[0], grads[0]);  // (create_graph)
     }
@@ -306,6 +311,7 @@ void distill_head_dh(const at::Tensor& dl, const c10::optional<at::Tensor>& lo, 
   TS_CUDA_CHECK(head_dh(l, k_rows(dl), lo ? &low : nullptr, k_cols(w), out_map(splits > 1 ? parts : dh), (int)n, (int)d,
                         (int)v, splits, split_rows, splits > 1 ? parts.data_ptr<float>() : nullptr, dh.data_ptr(),
                         error_word(dl)));
+  if (splits > 1) ++g_more_launches;  // the sum of the slices
 }
 
 // dW [V, D] = (d + lo)ᵀ [V, N] · hidden [N, D], bf16
@@ -322,6 +328,10 @@ at::Tensor distill_head_dw(const at::Tensor& dl, const c10::optional<at::Tensor>
                         (int)h.size(1), (int)dl.size(1), error_word(dl)));
   return dw;
 }
+
+// Kernels since the last reset that no call of an entry point stands for: the loss rows' gradient, which autograd calls,
+// and those that only some calls launch.
+int64_t more_launches(bool reset) { return reset ? g_more_launches.exchange(0) : g_more_launches.load(); }
 
 uint64_t bounds_word_distill(bool reset) {
   unsigned long long w = 0;

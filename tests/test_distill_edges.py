@@ -567,3 +567,27 @@ def test_second_derivative_on_the_cpu():
     ids = torch.tensor([[0, 3, 5], [8, 2, 1]])
     lp = torch.log(torch.tensor([[0.5, 0.2, 0.1], [0.3, 0.3, 0.2]]))
     assert torch.autograd.gradgradcheck(lambda x: topk_distill_loss(x, ids, lp), (z,))
+
+
+# ------------------------------------------------------------------ counted launches
+@pytest.mark.gpu
+def test_launch_counts():
+    from thundersync_b200.ops._ext import launch_counts, reset_launch_counts
+
+    def kernels(fn):
+        reset_launch_counts()
+        fn()
+        torch.cuda.synchronize()
+        return launch_counts()["kernels"]
+
+    h, w, ids, lp = _head_inputs(5, 64, 8 * 64 * 64, 4, "cuda", torch.bfloat16)  # a contraction that is worth slicing
+    z = torch.randn(5, 300, device="cuda", requires_grad=True)
+    loss = topk_distill_loss(z, ids % 300, lp)
+    assert kernels(lambda: topk_distill_loss(z, ids % 300, lp)) == 1
+    assert kernels(lambda: loss.sum().backward()) == 1
+    head = lm_head_topk_distill(h, w, ids, lp)
+    assert kernels(lambda: lm_head_topk_distill(h, w, ids, lp)) == 3  # entries, logits, the rows' end
+    assert kernels(lambda: torch.autograd.grad(head.sum(), (h, w))) == 4  # dlogits, dH and the sum of its slices, dW
+    h1, w1, ids1, lp1 = _head_inputs(5, 64, 1024, 4, "cuda", torch.bfloat16)  # 16 K blocks: one slice
+    head = lm_head_topk_distill(h1, w1, ids1, lp1)
+    assert kernels(lambda: torch.autograd.grad(head.sum(), (h1, w1))) == 3

@@ -14,7 +14,8 @@ from functools import lru_cache
 
 _LOAD_ERROR: BaseException | None = None
 
-# kernels launched per call of each native entry point
+# kernels launched per call of each native entry point; those that only some calls launch, or autograd, are counted
+# natively (more_launches)
 KERNELS_PER_CALL = {
     "rms_norm_fwd": 1, "rms_norm_bwd": 2, "qk_norm_rope_fwd": 1, "qk_norm_rope_bwd": 2,
     "swiglu_fwd": 1, "swiglu_bwd": 1, "embedding_bwd_accumulate": 1, "fold_stats": 1, "axpby": 1,
@@ -24,7 +25,7 @@ KERNELS_PER_CALL = {
     "conv1d_silu_fwd": 1, "conv1d_silu_bwd": 2, "gdn_fwd": 2, "gdn_bwd": 2, "gdn_chunk_fwd": 3, "gdn_chunk_bwd": 3,
     "topk_logprobs": 1, "sample_tokens": 1, "distill_rows_fwd": 1, "distill_rows_bwd": 1, "distill_rows": 1,
     "distill_head_fwd": 3,
-    "distill_head_logits": 1, "distill_head_dh": 2, "distill_head_dw": 1,
+    "distill_head_logits": 1, "distill_head_dh": 1, "distill_head_dw": 1, "more_launches": 0,
 }
 
 _lock = threading.Lock()
@@ -85,14 +86,19 @@ def so_path() -> str | None:
     return None if mod is None else os.path.abspath(mod.__file__)
 
 
+def _more_launches(reset: bool) -> int:
+    return _load()._mod.more_launches(reset) if _load.cache_info().currsize and _load() is not None else 0
+
+
 def reset_launch_counts() -> None:
     with _lock:
         _calls.clear()
+    _more_launches(True)
 
 
 def launch_counts() -> dict[str, int]:
     """Native calls since the last reset, and the kernel launches they made."""
     with _lock:
         calls = dict(_calls)
-    kernels = sum(KERNELS_PER_CALL.get(k, 1) * v for k, v in calls.items())
+    kernels = sum(KERNELS_PER_CALL.get(k, 1) * v for k, v in calls.items()) + _more_launches(False)
     return {"calls": calls, "kernels": kernels}
