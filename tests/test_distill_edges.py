@@ -591,3 +591,18 @@ def test_launch_counts():
     h1, w1, ids1, lp1 = _head_inputs(5, 64, 1024, 4, "cuda", torch.bfloat16)  # 16 K blocks: one slice
     head = lm_head_topk_distill(h1, w1, ids1, lp1)
     assert kernels(lambda: torch.autograd.grad(head.sum(), (h1, w1))) == 3
+
+
+# ------------------------------------------------------------------ a top-k that is no usual whole number
+@pytest.mark.parametrize("device", DEVICES)
+def test_sample_top_k_values(device):
+    g = torch.Generator().manual_seed(1)
+    z = (torch.randn(4, 700, generator=g) * 2).to(device)
+    noise = torch.empty(4, 700).exponential_(generator=g).to(device)
+    free = sample_tokens(z, noise)[0]
+    for none in (0, -3, 700, 10 ** 6, 1 << 70, math.inf, -math.inf):
+        assert torch.equal(sample_tokens(z, noise, top_k=none)[0], free)
+    assert torch.equal(sample_tokens(z, noise, top_k=3.0)[0], sample_tokens(z, noise, top_k=3)[0])
+    for bad in (2.5, math.nan):
+        with pytest.raises(ValueError, match="top_k"):
+            sample_tokens(z, noise, top_k=bad)

@@ -44,6 +44,13 @@ def _setting(value, name: str, n: int, device, dtype, low: float, high: float):
     return None, value
 
 
+def _whole(top_k, v: int) -> int:
+    """A number of tokens in [0, v]: 0 and v are no limit, and what is below or above them none either."""
+    if math.isnan(top_k) or (math.isfinite(top_k) and top_k != int(top_k)):
+        raise ValueError(f"top_k must be a whole number, got {top_k}")
+    return int(min(max(top_k, 0), v))
+
+
 def sample_tokens(logits: torch.Tensor, noise: torch.Tensor | None, *, temperature: float | torch.Tensor = 1.0,
                   top_k: int | torch.Tensor = 0, top_p: float | torch.Tensor = 1.0,
                   min_p: float | torch.Tensor = 0.0) -> tuple[torch.Tensor, torch.Tensor]:
@@ -62,7 +69,8 @@ def sample_tokens(logits: torch.Tensor, noise: torch.Tensor | None, *, temperatu
         raise ValueError(f"noise must be fp32 {tuple(logits.shape)} on {dev}, got {noise.dtype} {tuple(noise.shape)} "
                          f"on {noise.device}")
     t = _setting(temperature, "temperature", n, dev, torch.float32, 0.0, math.inf)
-    k = _setting(top_k, "top_k", n, dev, torch.int64, -math.inf, math.inf)
+    k = _setting(top_k if isinstance(top_k, torch.Tensor) else _whole(top_k, logits.shape[1]), "top_k", n, dev,
+                 torch.int64, 0, math.inf)
     p = _setting(top_p, "top_p", n, dev, torch.float32, 0.0, math.inf)
     mp = _setting(min_p, "min_p", n, dev, torch.float32, 0.0, 1.0)
     logits = logits.detach()
